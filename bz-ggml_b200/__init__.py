@@ -124,6 +124,13 @@ SIGNATURES = {
     "bzb_generator_bench_gemv": (ctypes.c_double, [ctypes.c_void_p, ctypes.c_char_p, ctypes.c_int, ctypes.c_int,
                                                     ctypes.c_int, ctypes.c_int]),
     "bzb_generator_depth_trace": (ctypes.c_int, [ctypes.c_void_p, _c_double_p, ctypes.c_int]),
+    "bzb_kv8_append": (ctypes.c_int, [ctypes.c_void_p] * 8 + [ctypes.c_float, ctypes.c_void_p, ctypes.c_int,
+                                                               ctypes.c_void_p]),
+    "bzb_kv8_read": (ctypes.c_int, [ctypes.c_void_p] * 5),
+    "bzb_kv8_attention_workspace": (ctypes.c_longlong, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int,
+                                                        ctypes.c_int]),
+    "bzb_kv8_attention": (ctypes.c_int, [ctypes.c_void_p] * 5 + [ctypes.c_float, ctypes.c_int, ctypes.c_int,
+                                                                 ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p]),
     "bzb_generator_gemm_noalloc": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_char_p, ctypes.c_int, ctypes.c_void_p,
                                                   ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]),
     "bzb_gguf_inspect": (ctypes.c_int, [ctypes.c_char_p, _c_int_p, _c_int_p, _c_int_p]),
@@ -749,3 +756,6 @@ def synth_model(out_path: str, preset: str = "full", nc: int = 0, quant: str = "
 def ids_to_text(ids: Sequence[int]) -> str:
     """Text whose synthetic-vocabulary tokenisation is exactly `ids` (ids >= 264)."""
     return "".join(f"<|t{int(i)}|>" for i in ids)
+
+
+from .kv8 import KV8Batch, KV8Cache  # noqa: E402  (after lib(), which it uses)

@@ -5,6 +5,7 @@
 #include "../../include/bzb_ext.h"
 #include "engine.h"
 #include "generate.h"
+#include "kv8.h"
 #include "vocoder.h"
 
 #include <cerrno>
@@ -161,6 +162,25 @@ int burst_impl(breeze_generator * gen, const int * ids, int n, int K, const unsi
         if (r.steps_executed < k) break;
     }
     return done;
+}
+}  // namespace
+
+namespace {
+// one call of the 8-bit cache's operators on the cache's device; f may throw
+template <typename F>
+int kv8_call(const char * what, const bzb_kv8_cache * cache, const bzb_kv8_batch * batch, F && f) {
+    if (!cache || !batch) {
+        set_error(std::string(what) + ": null cache or batch");
+        return -1;
+    }
+    try {
+        OnDevice on_device_(cache->device);
+        f();
+        return 0;
+    } catch (const std::exception & e) {
+        set_error(std::string(what) + ": " + e.what());
+        return -1;
+    }
 }
 }  // namespace
 
@@ -973,6 +993,42 @@ int bzb_generator_gemm_noalloc(breeze_generator * gen, const char * tensor, int 
         set_error(e.what());
         return -1;
     }
+}
+
+int bzb_kv8_append(const bzb_kv8_cache * cache, const bzb_kv8_batch * batch, const bzb_kv8_rows * q,
+                   const bzb_kv8_rows * k, const bzb_kv8_rows * v, const bzb_kv8_rows * q_out, const float * q_norm,
+                   const float * k_norm, float eps, const float * rope, int rope_len, void * stream) {
+    return kv8_call("kv8_append", cache, batch, [&] {
+        if (!k || !v) throw std::runtime_error("null key or value rows");
+        bzb::kv8_append(*cache, *batch, q, *k, *v, q_out, q_norm, k_norm, eps, rope, rope_len,
+                        static_cast<cudaStream_t>(stream));
+    });
+}
+
+int bzb_kv8_read(const bzb_kv8_cache * cache, const bzb_kv8_batch * batch, const bzb_kv8_rows * k_out,
+                 const bzb_kv8_rows * v_out, void * stream) {
+    return kv8_call("kv8_read", cache, batch, [&] {
+        if (!k_out || !v_out) throw std::runtime_error("null key or value rows");
+        bzb::kv8_read(*cache, *batch, *k_out, *v_out, static_cast<cudaStream_t>(stream));
+    });
+}
+
+long long bzb_kv8_attention_workspace(const bzb_kv8_cache * cache, const bzb_kv8_batch * batch, int n_head, int causal,
+                                      int window) {
+    long long bytes = -1;
+    kv8_call("kv8_attention_workspace", cache, batch,
+             [&] { bytes = bzb::kv8_attention_workspace(*cache, *batch, n_head, causal, window); });
+    return bytes;
+}
+
+int bzb_kv8_attention(const bzb_kv8_cache * cache, const bzb_kv8_batch * batch, const bzb_kv8_rows * q,
+                      const bzb_kv8_rows * out, float * lse, float scale, int causal, int window, void * workspace,
+                      long long workspace_bytes, void * stream) {
+    return kv8_call("kv8_attention", cache, batch, [&] {
+        if (!q || !out) throw std::runtime_error("null query or output rows");
+        bzb::kv8_attention(*cache, *batch, *q, *out, lse, scale, causal, window, workspace, workspace_bytes,
+                           static_cast<cudaStream_t>(stream));
+    });
 }
 
 int bzb_generator_depth_trace(breeze_generator * gen, double * out, int capacity) {

@@ -1,0 +1,1056 @@
+// Kernels of the 8-bit paged key/value cache (include/bzb_ext.h, bzb_kv8_*): appending with the q/k
+// norms and the rotation in the same pass, reading back, and attention over the cache.
+//
+// Numbers. A cached value is an e4m3 byte times its block's scale 2^e (16 positions of one head). e4m3
+// converts to f16 exactly, so the attention kernels multiply the bytes as f16 and bring the scales in
+// where they are one number for a whole block: 2^e of the keys multiplies the scores, 2^e of the
+// values goes into the exponent of the weights (see attention below). A power of two costs e4m3 no
+// precision, since its relative spacing is the same at every magnitude, and lets an append
+// rescale a block's earlier values without rounding them again (except below the smallest normal).
+#include "kv8.h"
+#include "tc_ptx.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <cstdint>
+#include <stdexcept>
+#include <string>
+#include <utility>
+
+namespace bzb {
+namespace {
+
+constexpr int kExpMin = -24, kExpMax = 40;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+void check_cuda(cudaError_t e, const char * what) {
+    if (e != cudaSuccess) throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(e));
+}
+
+// what every kernel needs of the cache and the batch
+struct Kv {
+    uint8_t * pages;
+    float * scales;
+    const int * table;
+    int * status;
+    long long page_stride, scale_stride;
+    int n_pages, n_slots, max_pages, page_tokens, page_shift, n_kv;
+    const int * q_start, * kv_len, * slots;
+    int n_seq, n_tok, max_new, max_len;
+};
+
+struct Rows {
+    void * p;
+    long long row, head;  // strides in elements
+};
+
+struct Seq {
+    int row0, n, len, slot;  // first packed row, rows, cached positions, page table row (-1: skip the sequence)
+};
+
+__device__ __forceinline__ void complain(const Kv & kv) {
+    if (kv.status) atomicExch(kv.status, 1);
+}
+
+__device__ __forceinline__ Seq load_seq(const Kv & kv, int b) {
+    Seq s;
+    s.row0 = kv.q_start[b];
+    const int end = kv.q_start[b + 1];
+    s.n = end - s.row0;
+    s.len = kv.kv_len[b];
+    s.slot = kv.slots ? kv.slots[b] : b;
+    // (end and row0 are compared before their difference is used: it may overflow)
+    if (s.row0 < 0 || end < s.row0 || end > kv.n_tok || s.n > kv.max_new || s.len < 0 || s.len > kv.max_len || s.slot < 0 ||
+        s.slot >= kv.n_slots) {
+        complain(kv);
+        s.slot = -1;
+    }
+    return s;
+}
+
+// the page of block `blk` (16 positions) of a sequence, or -1
+__device__ __forceinline__ int page_of(const Kv & kv, int slot, int blk) {
+    const int pg = __ldg(kv.table + (size_t) slot * kv.max_pages + (blk >> (kv.page_shift - 4)));
+    if ((unsigned) pg >= (unsigned) kv.n_pages) {
+        complain(kv);
+        return -1;
+    }
+    return pg;
+}
+__device__ __forceinline__ uint8_t * block_ptr(const Kv & kv, int pg, int blk, int plane, int head, int hd) {
+    const int at = (blk << 4) & (kv.page_tokens - 1);
+    return kv.pages + pg * kv.page_stride + ((size_t) (plane * kv.n_kv + head) * kv.page_tokens + at) * hd;
+}
+__device__ __forceinline__ float * scale_ptr(const Kv & kv, int pg, int blk, int plane, int head) {
+    const int per = kv.page_tokens >> 4;
+    return kv.scales + pg * kv.scale_stride + (plane * kv.n_kv + head) * per + (blk & (per - 1));
+}
+
+__device__ __forceinline__ float pow2f(int e) { return __int_as_float((e + 127) << 23); }
+__device__ __forceinline__ int exponent_of(float pow2) { return (__float_as_int(pow2) >> 23) - 127; }
+// smallest e with 448 2^e >= x (448 = 1.75 2^8), clamped; x >= 0 and finite
+__device__ __forceinline__ int block_exponent(float x) {
+    const int bits = __float_as_int(x);
+    const int e = (bits >> 23) - 127 - 8 + ((bits & 0x7fffff) > 0x600000);
+    return max(kExpMin, min(kExpMax, e));  // (subnormals and zero have exponent field 0: clamped)
+}
+
+// four floats -> four e4m3 bytes, nearest with ties to even; NaN stays NaN
+__device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d) {
+    uint16_t lo, hi;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+    return (uint32_t) lo | ((uint32_t) hi << 16);
+}
+__device__ __forceinline__ uint32_t e4m3x2_to_h2(uint16_t v) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
+    return r;
+}
+__device__ __forceinline__ float4 e4m3x4_to_f4(uint32_t w) {
+    const uint32_t lo = e4m3x2_to_h2((uint16_t) w), hi = e4m3x2_to_h2((uint16_t) (w >> 16));
+    const float2 a = __half22float2(*reinterpret_cast<const half2 *>(&lo));
+    const float2 b = __half22float2(*reinterpret_cast<const half2 *>(&hi));
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+
+// ---- four consecutive elements of a row, by type; VEC: they are aligned to their size ----
+template <int TYPE, bool VEC>
+__device__ __forceinline__ float4 load4(const void * p, long long i) {
+    if constexpr (TYPE == BZB_F32) {
+        const float * f = static_cast<const float *>(p) + i;
+        if constexpr (VEC) return __ldg(reinterpret_cast<const float4 *>(f));
+        return make_float4(f[0], f[1], f[2], f[3]);
+    } else if constexpr (TYPE == BZB_F16) {
+        const half * h = static_cast<const half *>(p) + i;
+        if constexpr (VEC) {
+            const uint2 u = __ldg(reinterpret_cast<const uint2 *>(h));
+            const float2 a = __half22float2(*reinterpret_cast<const half2 *>(&u.x));
+            const float2 b = __half22float2(*reinterpret_cast<const half2 *>(&u.y));
+            return make_float4(a.x, a.y, b.x, b.y);
+        }
+        return make_float4(__half2float(h[0]), __half2float(h[1]), __half2float(h[2]), __half2float(h[3]));
+    } else {
+        const __nv_bfloat16 * h = static_cast<const __nv_bfloat16 *>(p) + i;
+        if constexpr (VEC) {
+            const uint2 u = __ldg(reinterpret_cast<const uint2 *>(h));
+            return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                               __uint_as_float(u.y & 0xffff0000u));
+        }
+        return make_float4(__bfloat162float(h[0]), __bfloat162float(h[1]), __bfloat162float(h[2]), __bfloat162float(h[3]));
+    }
+}
+__device__ __forceinline__ uint32_t pack_half(float a, float b) {
+    const half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ void store4(int type, bool vec, void * p, long long i, float4 x) {
+    if (type == BZB_F32) {
+        float * f = static_cast<float *>(p) + i;
+        if (vec) *reinterpret_cast<float4 *>(f) = x;
+        else f[0] = x.x, f[1] = x.y, f[2] = x.z, f[3] = x.w;
+    } else {
+        const uint2 u = type == BZB_F16 ? make_uint2(pack_half(x.x, x.y), pack_half(x.z, x.w))
+                                        : make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
+        uint16_t * h = static_cast<uint16_t *>(p) + i;
+        if (vec) *reinterpret_cast<uint2 *>(h) = u;
+        else {
+            h[0] = (uint16_t) u.x, h[1] = (uint16_t) (u.x >> 16);
+            h[2] = (uint16_t) u.y, h[3] = (uint16_t) (u.y >> 16);
+        }
+    }
+}
+
+// ---- append and read: one warp per (sequence, block of 16 positions, head of q, k or v) ----
+//
+// A lane holds, of each of its rows, the four elements from 4c and the four from hd/2 + 4c, c its
+// column of hd/8: the two members of four rotated pairs, so the rotation needs no exchange and
+// each (cos, sin) is read by one lane. Its rows are consecutive positions (4 of 16 for head_dim 64, 8 of 16 for 128), so that of
+// the values it holds whole 4 x 4 patches and stores them as 16 bytes. All rows' loads are issued
+// before the first is used. The maximum of a block is one warp reduction, and no other warp
+// touches the block: no atomics, and the same bytes whatever the launch's shape.
+struct AppendArgs {
+    Kv kv;
+    Rows q, k, v, q_out;
+    const float * q_norm, * k_norm;
+    const float2 * rope;
+    float eps;
+    int n_head, n_blk, q_out_type, rope_len;
+    bool q_out_vec;
+};
+
+constexpr int kRowWarps = 4;
+
+template <int HD, int TYPE, bool VEC>
+__global__ void __launch_bounds__(32 * kRowWarps) kv8_append_kernel(const AppendArgs a) {
+    constexpr int LPR = HD / 8, RPL = HD / 16;  // lanes per row, rows per lane
+    const Kv & kv = a.kv;
+    const int tasks = a.n_head + 2 * kv.n_kv;
+    const int lane = threadIdx.x & 31, c = lane % LPR, r0 = lane / LPR * RPL;
+    const long long task = (long long) blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+    const int unit = (int) (task % tasks);
+    const long long sb = task / tasks;
+    const int b = (int) (sb / a.n_blk);
+    if (b >= kv.n_seq) return;
+    const Seq s = load_seq(kv, b);
+    if (s.slot < 0) return;
+    const int first = s.len - s.n;  // position of the sequence's first row (negative: padding rows)
+    const int blk = (max(first, 0) >> 4) + (int) (sb % a.n_blk), p0 = blk << 4;
+    if (p0 >= s.len || s.n == 0) return;
+    const int kind = unit < a.n_head ? 0 : unit < a.n_head + kv.n_kv ? 1 : 2;
+    const int head = kind == 0 ? unit : kind == 1 ? unit - a.n_head : unit - a.n_head - kv.n_kv;
+    const Rows src = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
+
+    float4 lo[RPL], hi[RPL];
+#pragma unroll
+    for (int i = 0; i < RPL; i++) {
+        const int pos = p0 + r0 + i;
+        lo[i] = hi[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (pos >= first && pos < s.len) {
+            const long long at = (long long) (s.row0 + pos - first) * src.row + head * src.head + 4 * c;
+            lo[i] = load4<TYPE, VEC>(src.p, at);
+            hi[i] = load4<TYPE, VEC>(src.p, at + HD / 2);
+        }
+    }
+    const float * w = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
+    if (w) {
+        // (the weights' pointers are only 4-byte aligned)
+        const float4 wl = load4<BZB_F32, false>(w, 4 * c), wh = load4<BZB_F32, false>(w, HD / 2 + 4 * c);
+#pragma unroll
+        for (int i = 0; i < RPL; i++) {
+            float4 & x = lo[i], & y = hi[i];
+            float ss = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w + y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w;
+#pragma unroll
+            for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            const float r = 1.0f / sqrtf(ss * (1.0f / HD) + a.eps);
+            x = make_float4(x.x * r * wl.x, x.y * r * wl.y, x.z * r * wl.z, x.w * r * wl.w);
+            y = make_float4(y.x * r * wh.x, y.y * r * wh.y, y.z * r * wh.z, y.w * r * wh.w);
+        }
+    }
+    if (kind < 2 && a.rope) {
+#pragma unroll
+        for (int i = 0; i < RPL; i++) {
+            const int pos = p0 + r0 + i;
+            if (pos < first || pos >= s.len) continue;
+            const float2 * t = a.rope + (size_t) pos * (HD / 2) + 4 * c;
+            const float2 t0 = __ldg(t), t1 = __ldg(t + 1), t2 = __ldg(t + 2), t3 = __ldg(t + 3);
+            const float4 x = lo[i], y = hi[i];
+            lo[i] = make_float4(x.x * t0.x - y.x * t0.y, x.y * t1.x - y.y * t1.y, x.z * t2.x - y.z * t2.y, x.w * t3.x - y.w * t3.y);
+            hi[i] = make_float4(x.x * t0.y + y.x * t0.x, x.y * t1.y + y.y * t1.x, x.z * t2.y + y.z * t2.x, x.w * t3.y + y.w * t3.x);
+        }
+    }
+    if (kind == 0) {
+#pragma unroll
+        for (int i = 0; i < RPL; i++) {
+            const int pos = p0 + r0 + i;
+            if (pos < first || pos >= s.len) continue;
+            const long long at = (long long) (s.row0 + pos - first) * a.q_out.row + head * a.q_out.head + 4 * c;
+            store4(a.q_out_type, a.q_out_vec, a.q_out.p, at, lo[i]);
+            store4(a.q_out_type, a.q_out_vec, a.q_out.p, at + HD / 2, hi[i]);
+        }
+        return;
+    }
+
+    const int pg = page_of(kv, s.slot, blk);
+    if (pg < 0) return;
+    uint8_t * dst = block_ptr(kv, pg, blk, kind - 1, head, HD);
+    float * sp = scale_ptr(kv, pg, blk, kind - 1, head);
+    const bool older = p0 < first;  // the block holds earlier positions of this sequence
+    // the block's largest finite magnitude; what is not finite becomes NaN
+    float top = 0.0f;
+    auto finite = [&](float & x) {
+        const float m = fabsf(x);
+        if (m < INFINITY) top = fmaxf(top, m);
+        else x = __int_as_float(0x7fffffff);
+    };
+#pragma unroll
+    for (int i = 0; i < RPL; i++) {
+        finite(lo[i].x), finite(lo[i].y), finite(lo[i].z), finite(lo[i].w);
+        finite(hi[i].x), finite(hi[i].y), finite(hi[i].z), finite(hi[i].w);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    int e = block_exponent(top);
+    float keep = 1.0f;  // factor of the earlier values' bytes
+    if (older) {
+        const int e_old = min(kExpMax, max(kExpMin, exponent_of(*sp)));
+        e = max(e, e_old);
+        keep = pow2f(e_old - e);
+    }
+    const float inv = pow2f(-e);
+    uint32_t wl[RPL], wh[RPL];
+    if (kind == 1) {
+#pragma unroll
+        for (int i = 0; i < RPL; i++) {
+            uint32_t * row = reinterpret_cast<uint32_t *>(dst + (r0 + i) * HD);
+            wl[i] = to_e4m3x4(lo[i].x * inv, lo[i].y * inv, lo[i].z * inv, lo[i].w * inv);
+            wh[i] = to_e4m3x4(hi[i].x * inv, hi[i].y * inv, hi[i].z * inv, hi[i].w * inv);
+            if (older && p0 + r0 + i < first) {
+                const float4 x = e4m3x4_to_f4(row[c]), y = e4m3x4_to_f4(row[c + HD / 8]);
+                wl[i] = to_e4m3x4(x.x * keep, x.y * keep, x.z * keep, x.w * keep);
+                wh[i] = to_e4m3x4(y.x * keep, y.y * keep, y.z * keep, y.w * keep);
+            }
+            row[c] = wl[i];
+            row[c + HD / 8] = wh[i];
+        }
+    } else {
+#pragma unroll
+        for (int g = 0; g < RPL; g += 4) {
+            // patch (element quad c or c + hd/8, position group): word j holds element j of the four positions
+            uint4 * pl = reinterpret_cast<uint4 *>(dst + c * 64 + (r0 + g) * 4), * ph = pl + HD / 8 * 4;
+            uint4 ol = make_uint4(0, 0, 0, 0), oh = ol;
+            if (older && p0 + r0 + g < first) ol = *pl, oh = *ph;
+            auto patch = [&](const float4 (&x)[RPL], uint4 old) {
+                const int kept = older ? min(4, max(0, first - (p0 + r0 + g))) : 0;
+                auto word = [&](float v0, float v1, float v2, float v3, uint32_t was) {
+                    uint32_t n = to_e4m3x4(v0 * inv, v1 * inv, v2 * inv, v3 * inv);
+                    if (kept > 0) {
+                        const float4 f = e4m3x4_to_f4(was);
+                        const uint32_t o = to_e4m3x4(f.x * keep, f.y * keep, f.z * keep, f.w * keep);
+                        const uint32_t m = kept == 4 ? 0xffffffffu : (1u << (8 * kept)) - 1;
+                        n = (o & m) | (n & ~m);
+                    }
+                    return n;
+                };
+                return make_uint4(word(x[g].x, x[g + 1].x, x[g + 2].x, x[g + 3].x, old.x),
+                                  word(x[g].y, x[g + 1].y, x[g + 2].y, x[g + 3].y, old.y),
+                                  word(x[g].z, x[g + 1].z, x[g + 2].z, x[g + 3].z, old.z),
+                                  word(x[g].w, x[g + 1].w, x[g + 2].w, x[g + 3].w, old.w));
+            };
+            *pl = patch(lo, ol);
+            *ph = patch(hi, oh);
+        }
+    }
+    // (a block's scale is read above by every lane of the one warp that owns it)
+    __syncwarp();
+    if (lane == 0) *sp = pow2f(e);
+}
+
+struct ReadArgs {
+    Kv kv;
+    Rows k, v;
+    int n_blk, type;
+    bool vec;
+};
+
+template <int HD>
+__global__ void __launch_bounds__(32 * kRowWarps) kv8_read_kernel(const ReadArgs a) {
+    constexpr int LPR = HD / 8, RPL = HD / 16;
+    const Kv & kv = a.kv;
+    const int lane = threadIdx.x & 31, c = lane % LPR, r0 = lane / LPR * RPL;
+    const long long task = (long long) blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+    const int unit = (int) (task % (2 * kv.n_kv));
+    const long long sb = task / (2 * kv.n_kv);
+    const int b = (int) (sb / a.n_blk);
+    if (b >= kv.n_seq) return;
+    const Seq s = load_seq(kv, b);
+    if (s.slot < 0 || s.n == 0) return;
+    // blocks count from the first row's position; `first` may be negative (padding rows, read as zeros)
+    const int first = s.len - s.n, blk = (first >> 4) + (int) (sb % a.n_blk), p0 = blk << 4;
+    if (p0 >= s.len) return;
+    const int plane = unit >= kv.n_kv, head = unit - plane * kv.n_kv;
+    float4 lo[RPL], hi[RPL];
+#pragma unroll
+    for (int i = 0; i < RPL; i++) lo[i] = hi[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (blk >= 0) {
+        const int pg = max(page_of(kv, s.slot, blk), 0);
+        const uint8_t * src = block_ptr(kv, pg, blk, plane, head, HD);
+        const float scale = *scale_ptr(kv, pg, blk, plane, head);
+        if (plane == 0) {
+            uint32_t wl[RPL], wh[RPL];
+#pragma unroll
+            for (int i = 0; i < RPL; i++) {
+                const uint32_t * row = reinterpret_cast<const uint32_t *>(src + (r0 + i) * HD);
+                wl[i] = row[c];
+                wh[i] = row[c + HD / 8];
+            }
+#pragma unroll
+            for (int i = 0; i < RPL; i++) lo[i] = e4m3x4_to_f4(wl[i]), hi[i] = e4m3x4_to_f4(wh[i]);
+        } else {
+#pragma unroll
+            for (int g = 0; g < RPL; g += 4) {
+                const uint4 * pl = reinterpret_cast<const uint4 *>(src + c * 64 + (r0 + g) * 4);
+                auto patch = [&](float4 (&x)[RPL], uint4 w) {
+                    const float4 e0 = e4m3x4_to_f4(w.x), e1 = e4m3x4_to_f4(w.y), e2 = e4m3x4_to_f4(w.z), e3 = e4m3x4_to_f4(w.w);
+                    x[g] = make_float4(e0.x, e1.x, e2.x, e3.x);
+                    x[g + 1] = make_float4(e0.y, e1.y, e2.y, e3.y);
+                    x[g + 2] = make_float4(e0.z, e1.z, e2.z, e3.z);
+                    x[g + 3] = make_float4(e0.w, e1.w, e2.w, e3.w);
+                };
+                patch(lo, pl[0]);
+                patch(hi, pl[HD / 8 * 4]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < RPL; i++) {
+            lo[i] = make_float4(lo[i].x * scale, lo[i].y * scale, lo[i].z * scale, lo[i].w * scale);
+            hi[i] = make_float4(hi[i].x * scale, hi[i].y * scale, hi[i].z * scale, hi[i].w * scale);
+        }
+    }
+    const Rows dst = plane ? a.v : a.k;
+#pragma unroll
+    for (int i = 0; i < RPL; i++) {
+        const int pos = p0 + r0 + i;
+        if (pos < first || pos >= s.len) continue;
+        const long long at = (long long) (s.row0 + pos - first) * dst.row + head * dst.head + 4 * c;
+        store4(a.type, a.vec, dst.p, at, lo[i]);
+        store4(a.type, a.vec, dst.p, at + HD / 2, hi[i]);
+    }
+}
+
+// ---- attention ----
+//
+// For a row with scores s_j (in powers of two: scale log2(e) q.k_j) and values 2^{e_j} v_j, the weights
+// are kept relative to M = max_j (s_j + e_j):
+//   w_j = 2^(s_j + e_j - M) <= 1,  O = sum_j w_j v_j,  l = sum_j w_j 2^-e_j,  out = O / l,
+//   log-sum-exp = ln 2 (M + log2 l),
+// so the f16 weights of the second product carry the values' block scales, and the sum undoes them
+// in f32 (|e| <= 40: no weight that matters underflows). M, l and O are f32 and updated
+// block by block.
+struct AttnArgs {
+    Kv kv;
+    Rows q, out;
+    float * lse;
+    float scale2;  // scale log2(e)
+    int n_head, group, causal, window;
+    int type;      // of q and out
+    bool q_vec, out_vec;
+    int row_tiles, chunks, chunk_blocks;
+    float * part;
+    int * counters;
+};
+
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint4 load_stream(const void * p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+// bytes of w that are e4m3 NaN (0x7f or 0xff) become 0xff, the others 0
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
+
+// 16 elements of a query row from element i as f16 pairs: f16 rows as they are, bf16 rows times f (and
+// their largest magnitude into amax)
+__device__ __forceinline__ void load_q16(const AttnArgs & a, long long i, float f, uint32_t (&o)[8], float * amax) {
+    float x[16];
+    if (a.type == BZB_F16) {
+        const half * h = static_cast<const half *>(a.q.p) + i;
+        if (a.q_vec) {
+            const uint4 u = *reinterpret_cast<const uint4 *>(h), v = *reinterpret_cast<const uint4 *>(h + 8);
+            o[0] = u.x, o[1] = u.y, o[2] = u.z, o[3] = u.w, o[4] = v.x, o[5] = v.y, o[6] = v.z, o[7] = v.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const half2 p = __halves2half2(h[2 * j], h[2 * j + 1]);
+                o[j] = *reinterpret_cast<const uint32_t *>(&p);
+            }
+        }
+        return;
+    }
+    const __nv_bfloat16 * h = static_cast<const __nv_bfloat16 *>(a.q.p) + i;
+    if (a.q_vec) {
+        const uint4 u = *reinterpret_cast<const uint4 *>(h), v = *reinterpret_cast<const uint4 *>(h + 8);
+        const uint32_t w[8] = { u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w };
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[2 * j] = __uint_as_float(w[j] << 16), x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; j++) x[j] = __bfloat162float(h[j]);
+    }
+    if (amax) {
+#pragma unroll
+        for (int j = 0; j < 16; j++) *amax = fmaxf(*amax, fabsf(x[j]));
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) o[j] = pack_half(x[2 * j] * f, x[2 * j + 1] * f);
+}
+
+// Few query rows (a step of each sequence, or a few guessed tokens): one CTA per (sequence, kv head, tile
+// of 8 NT query rows, range of the cache), its warps taking the range's blocks in turn. The rows of a
+// kv head are (token, head of the group) pairs, so a block read once serves the whole group.
+//
+// The matrix products are m16n8k16 with the cache as the 16-row operand: S^T = K Q^T (16 positions x 8
+// rows) and O^T = V^T W^T (16 of head_dim x 8 rows): no half of a tile is empty when a group has at
+// most 8 rows. Both operands come straight from global memory into the MMA's register layout: a lane's 16
+// bytes of a key row are the four k-steps' values of head_dim for it (the queries are read in the same
+// order, so any order of the sum's terms will do), and the value patches are stored in operand order. No shared memory, no
+// transposition but the 8x8 one of the weights; per lane 4 loads of 16 bytes a block for head_dim 64.
+template <int HD, int NT, int WARPS>
+struct SmallTile {
+    static constexpr int ROWS = 8 * NT, KS = HD / 64, VS = HD / 32, MT = HD / 16, PL = HD + 2;
+};
+
+template <int HD, int NT, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) kv8_attn_small_kernel(const AttnArgs a) {
+    using T = SmallTile<HD, NT, WARPS>;
+    __shared__ float sm_o[WARPS][T::ROWS][HD + 4];
+    __shared__ float sm_ml[WARPS][T::ROWS][2];
+    const Kv & kv = a.kv;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    // (heads fastest: neighbouring CTAs read neighbouring bytes of the same pages)
+    long long id = blockIdx.x;
+    const int h = (int) (id % kv.n_kv);
+    id /= kv.n_kv;
+    const int chunk = (int) (id % a.chunks);
+    id /= a.chunks;
+    const int tile = (int) (id % a.row_tiles), b = (int) (id / a.row_tiles);
+    const Seq s = load_seq(kv, b);
+    if (s.slot < 0) return;
+    const int rows = s.n * a.group, row0 = tile * T::ROWS;
+    if (row0 >= rows) return;
+    const int first = s.len - s.n;
+    const int pos_lo = first + row0 / a.group, pos_hi = first + min(rows - 1, row0 + T::ROWS - 1) / a.group;
+    // the keys that any row of the tile looks at: [key_lo, key_hi)
+    const int key_hi = max(0, a.causal ? pos_hi + 1 : s.len);
+    const int key_lo = a.window > 0 ? max(0, pos_lo - a.window + 1) : 0;
+    // every row sees [full_lo, full_hi)
+    const int full_hi = a.causal ? pos_lo + 1 : s.len, full_lo = a.window > 0 ? max(0, pos_hi - a.window + 1) : 0;
+    const int blk_lo = key_lo >> 4, blk_hi = (key_hi + 15) >> 4;
+    const int my_chunks = max(1, (blk_hi - blk_lo + a.chunk_blocks - 1) / a.chunk_blocks);
+    if (chunk >= my_chunks) return;
+    const int c_lo = blk_lo + chunk * a.chunk_blocks, c_hi = min(blk_hi, c_lo + a.chunk_blocks);
+
+    // queries as the 8-column operand: lane (g, t) holds row 8 nt + g, elements 64 k + 16 t ..+15
+    uint32_t qf[NT][T::KS][8];
+    float coef[NT][2];      // the score's factor for the lane's two columns (rows 8 nt + 2 t, + 1)
+    int lim_hi[NT][2], lim_lo[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        const int r = row0 + 8 * nt + g;
+        float unit = 1.0f;
+        if (r < rows) {
+            const long long at = (long long) (s.row0 + r / a.group) * a.q.row + (h * a.group + r % a.group) * a.q.head + 16 * t;
+            float amax = 0.0f;
+#pragma unroll
+            for (int k = 0; k < T::KS; k++) load_q16(a, at + 64 * k, 1.0f, qf[nt][k], &amax);
+            // bf16 may lie outside f16: the row is brought to about [1, 2) by a power of two (which the
+            // scores' factor takes back), so at most its elements below 2^-25 of the largest are lost
+            if (a.type == BZB_BF16) {
+                const unsigned quad = 0xfu << (lane & 28);
+                amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 2));
+                const int e = amax < INFINITY && amax > 0.0f ? min(126, max(-125, (__float_as_int(amax) >> 23) - 127)) : 0;
+                unit = pow2f(e);
+#pragma unroll
+                for (int k = 0; k < T::KS; k++) load_q16(a, at + 64 * k, pow2f(-e), qf[nt][k], nullptr);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < T::KS; k++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) qf[nt][k][j] = 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int rr = row0 + 8 * nt + 2 * t + i, pos = first + rr / a.group;
+            coef[nt][i] = a.scale2 * __shfl_sync(0xffffffffu, unit, (2 * t + i) * 4);
+            lim_hi[nt][i] = rr < rows ? (a.causal ? pos + 1 : s.len) : 0;
+            lim_lo[nt][i] = a.window > 0 ? pos - a.window + 1 : 0;
+        }
+    }
+
+    float o[NT][T::MT][4] = {}, m[NT][2], l[NT][2] = {};
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) m[nt][0] = m[nt][1] = -INFINITY;
+
+    const int kpos = (g >> 1) * 4 + (g & 1);  // the lane's key rows: kpos and kpos + 2 (see the patches' position order)
+    for (int base = c_lo + warp; base < c_hi; base += 32 * WARPS) {
+        // pages and scales of this warp's next 32 blocks, one block per lane
+        int my_pg = 0;
+        float my_ks = 0.0f, my_vs = 1.0f;
+        if (base + lane * WARPS < c_hi) {
+            const int blk = base + lane * WARPS;
+            my_pg = max(page_of(kv, s.slot, blk), 0);
+            my_ks = __ldg(scale_ptr(kv, my_pg, blk, 0, h));
+            my_vs = __ldg(scale_ptr(kv, my_pg, blk, 1, h));
+        }
+        const int n = min(32, (c_hi - base + WARPS - 1) / WARPS);
+        uint4 kf[2][T::KS][2], vf[2][T::VS];
+        auto fetch = [&](int i, uint4 (&kk)[T::KS][2], uint4 (&vv)[T::VS]) {
+            const int pg = __shfl_sync(0xffffffffu, my_pg, i), blk = base + i * WARPS;
+            const uint8_t * kp = block_ptr(kv, pg, blk, 0, h, HD) + kpos * HD + 16 * t;
+            const uint8_t * vp = block_ptr(kv, pg, blk, 1, h, HD) + 16 * lane;
+#pragma unroll
+            for (int k = 0; k < T::KS; k++) kk[k][0] = load_stream(kp + 64 * k), kk[k][1] = load_stream(kp + 2 * HD + 64 * k);
+#pragma unroll
+            for (int j = 0; j < T::VS; j++) vv[j] = load_stream(vp + 512 * j);
+        };
+        auto use = [&](int i, const uint4 (&kk)[T::KS][2], const uint4 (&vv)[T::VS]) {
+            const float ks = __shfl_sync(0xffffffffu, my_ks, i), vs = __shfl_sync(0xffffffffu, my_vs, i);
+            const int key0 = (base + i * WARPS) << 4;
+            float sc[NT][4] = {};
+#pragma unroll
+            for (int k = 0; k < T::KS; k++) {
+                const uint32_t w0[4] = { kk[k][0].x, kk[k][0].y, kk[k][0].z, kk[k][0].w };
+                const uint32_t w1[4] = { kk[k][1].x, kk[k][1].y, kk[k][1].z, kk[k][1].w };
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t a0 = e4m3x2_to_h2((uint16_t) w0[j]), a2 = e4m3x2_to_h2((uint16_t) (w0[j] >> 16));
+                    const uint32_t a1 = e4m3x2_to_h2((uint16_t) w1[j]), a3 = e4m3x2_to_h2((uint16_t) (w1[j] >> 16));
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) mma16816(sc[nt], a0, a1, a2, a3, qf[nt][k][2 * j], qf[nt][k][2 * j + 1]);
+                }
+            }
+            const float ev = (float) exponent_of(vs), inv_vs = 1.0f / vs;
+            const bool whole = key0 >= full_lo && key0 + 16 <= full_hi;
+            uint32_t seen[NT][2];  // (positions x rows) the rows that see each position, as f16 ones
+            uint32_t wb[NT][2];
+            bool moved = false;
+            float corr[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                float x[4];  // columns 2t, 2t+1 at key kpos, then at key kpos + 2
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    x[j] = fmaf(sc[nt][j], coef[nt][j & 1] * ks, ev);
+                    if (!whole) {
+                        const int key = key0 + kpos + (j >> 1) * 2;
+                        if (key < lim_lo[nt][j & 1] || key >= lim_hi[nt][j & 1]) x[j] = -INFINITY;
+                    }
+                }
+                if (!whole) {
+                    auto one = [&](int j) {
+                        const int key = key0 + kpos + (j >> 1) * 2;
+                        return key >= lim_lo[nt][j & 1] && key < lim_hi[nt][j & 1] ? 0x3c00u : 0u;
+                    };
+                    seen[nt][0] = one(0) | (one(1) << 16);
+                    seen[nt][1] = one(2) | (one(3) << 16);
+                }
+#pragma unroll
+                for (int i2 = 0; i2 < 2; i2++) {
+                    float mx = fmaxf(x[i2], x[i2 + 2]);
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                    const float to = fmaxf(m[nt][i2], mx), ref = to == -INFINITY ? 0.0f : to;
+                    corr[nt][i2] = exp2_approx(m[nt][i2] - ref);
+                    moved |= to != m[nt][i2];
+                    m[nt][i2] = to;
+                    x[i2] = exp2_approx(x[i2] - ref);
+                    x[i2 + 2] = exp2_approx(x[i2 + 2] - ref);
+                    l[nt][i2] = fmaf(l[nt][i2], corr[nt][i2], (x[i2] + x[i2 + 2]) * inv_vs);
+                }
+                wb[nt][0] = transpose8x8(pack_half(x[0], x[1]));
+                wb[nt][1] = transpose8x8(pack_half(x[2], x[3]));
+            }
+            if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int j = 0; j < T::MT; j++)
+#pragma unroll
+                        for (int i2 = 0; i2 < 4; i2++) o[nt][j][i2] *= corr[nt][i2 & 1];
+            }
+            uint4 vw[T::VS];
+            uint32_t bad = 0;
+#pragma unroll
+            for (int j = 0; j < T::VS; j++) {
+                vw[j] = vv[j];
+                if (!whole) bad |= nan_bytes(vv[j].x) | nan_bytes(vv[j].y) | nan_bytes(vv[j].z) | nan_bytes(vv[j].w);
+            }
+            // a NaN at a position that some row does not see must not reach that row (0 x NaN):
+            // NaNs are taken out of the product and given to the rows that see them
+            const bool poisoned = !whole && __any_sync(0xffffffffu, bad != 0);
+            if (poisoned) {
+                uint32_t sb0[NT], sb1[NT];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) sb0[nt] = transpose8x8(seen[nt][0]), sb1[nt] = transpose8x8(seen[nt][1]);
+#pragma unroll
+                for (int j = 0; j < T::VS; j++) {
+                    uint32_t w[4] = { vw[j].x, vw[j].y, vw[j].z, vw[j].w };
+#pragma unroll
+                    for (int half_ = 0; half_ < 2; half_++) {
+                        uint32_t f[4];  // f16 ones at NaNs
+#pragma unroll
+                        for (int i2 = 0; i2 < 2; i2++) {
+                            const uint32_t nb = nan_bytes(w[2 * half_ + i2]);
+                            f[i2] = ((nb & 1u) ? 0x3c00u : 0u) | ((nb & 0x100u) ? 0x3c000000u : 0u);
+                            f[2 + i2] = ((nb & 0x10000u) ? 0x3c00u : 0u) | ((nb & 0x1000000u) ? 0x3c000000u : 0u);
+                            w[2 * half_ + i2] &= ~nb;
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            float hit[4] = {};
+                            mma16816(hit, f[0], f[1], f[2], f[3], sb0[nt], sb1[nt]);
+#pragma unroll
+                            for (int i2 = 0; i2 < 4; i2++)
+                                if (hit[i2] > 0.0f) o[nt][2 * j + half_][i2] = __int_as_float(0x7fffffff);
+                        }
+                    }
+                    vw[j] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < T::VS; j++) {
+                const uint32_t w[4] = { vw[j].x, vw[j].y, vw[j].z, vw[j].w };
+#pragma unroll
+                for (int half_ = 0; half_ < 2; half_++) {
+                    const uint32_t a0 = e4m3x2_to_h2((uint16_t) w[2 * half_]), a2 = e4m3x2_to_h2((uint16_t) (w[2 * half_] >> 16));
+                    const uint32_t a1 = e4m3x2_to_h2((uint16_t) w[2 * half_ + 1]), a3 = e4m3x2_to_h2((uint16_t) (w[2 * half_ + 1] >> 16));
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) mma16816(o[nt][2 * j + half_], a0, a1, a2, a3, wb[nt][0], wb[nt][1]);
+                }
+            }
+        };
+        fetch(0, kf[0], vf[0]);
+        for (int i = 0; i < n; i += 2) {
+            if (i + 1 < n) fetch(i + 1, kf[1], vf[1]);
+            use(i, kf[0], vf[0]);
+            if (i + 1 < n) {
+                if (i + 2 < n) fetch(i + 2, kf[0], vf[0]);
+                use(i + 1, kf[1], vf[1]);
+            }
+        }
+    }
+
+    // the warps' states to shared memory: [row][element]; element of (mt, half, g): 32 (mt/2) + 4 g + 2 (mt%2) + half
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            float x = l[nt][i];
+            x += __shfl_xor_sync(0xffffffffu, x, 4);
+            x += __shfl_xor_sync(0xffffffffu, x, 8);
+            x += __shfl_xor_sync(0xffffffffu, x, 16);
+            if (g == 0) sm_ml[warp][8 * nt + 2 * t + i][0] = m[nt][i], sm_ml[warp][8 * nt + 2 * t + i][1] = x;
+        }
+#pragma unroll
+        for (int j = 0; j < T::VS; j++)
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                *reinterpret_cast<float4 *>(&sm_o[warp][8 * nt + 2 * t + i][32 * j + 4 * g]) =
+                    make_float4(o[nt][2 * j][i], o[nt][2 * j][2 + i], o[nt][2 * j + 1][i], o[nt][2 * j + 1][2 + i]);
+    }
+    __syncthreads();
+    const int live = min(T::ROWS, rows - row0);
+    const size_t unit = ((size_t) b * a.row_tiles + tile) * kv.n_kv + h;
+    float * part = a.part ? a.part + unit * a.chunks * (T::ROWS * T::PL) : nullptr;
+    auto finish = [&](int r, int d, float4 x, float mm, float ll) {
+        const float inv = ll > 0.0f ? 1.0f / ll : (ll == 0.0f ? 0.0f : ll);  // (NaN stays NaN)
+        const int rr = row0 + r, tok = s.row0 + rr / a.group, qh = h * a.group + rr % a.group;
+        store4(a.type, a.out_vec, a.out.p, (long long) tok * a.out.row + qh * a.out.head + d,
+               make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+        if (a.lse && d == 0) a.lse[(size_t) tok * a.n_head + qh] = ll == 0.0f ? -INFINITY : kLn2 * (mm + log2f(ll));
+    };
+    for (int i = threadIdx.x; i < live * (HD / 4); i += 32 * WARPS) {
+        const int r = i / (HD / 4), d = i % (HD / 4) * 4;
+        float mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) mm = fmaxf(mm, sm_ml[w][r][0]);
+        const float ref = mm == -INFINITY ? 0.0f : mm;
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) {
+            const float f = exp2_approx(sm_ml[w][r][0] - ref);
+            const float4 y = *reinterpret_cast<const float4 *>(&sm_o[w][r][d]);
+            ll = fmaf(sm_ml[w][r][1], f, ll);
+            x.x = fmaf(y.x, f, x.x), x.y = fmaf(y.y, f, x.y), x.z = fmaf(y.z, f, x.z), x.w = fmaf(y.w, f, x.w);
+        }
+        if (my_chunks == 1) {
+            finish(r, d, x, mm, ll);
+        } else {
+            float * pp = part + ((size_t) chunk * T::ROWS + r) * T::PL;
+            *reinterpret_cast<float2 *>(pp + d) = make_float2(x.x, x.y);
+            *reinterpret_cast<float2 *>(pp + d + 2) = make_float2(x.z, x.w);
+            if (d == 0) pp[HD] = mm, pp[HD + 1] = ll;
+        }
+    }
+    if (my_chunks == 1) return;
+    // the last range of this (sequence, tile, head) to finish joins them all, in the ranges' order
+    __shared__ int last;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        last = atomicAdd(a.counters + unit, 1) == my_chunks - 1;
+        if (last) a.counters[unit] = 0;
+    }
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+    for (int i = threadIdx.x; i < live * (HD / 4); i += 32 * WARPS) {
+        const int r = i / (HD / 4), d = i % (HD / 4) * 4;
+        float mm = -INFINITY, ll = 0.0f;
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int c = 0; c < my_chunks; c++) {
+            const float * pp = part + ((size_t) c * T::ROWS + r) * T::PL;
+            const float mc = __ldcg(pp + HD), lc = __ldcg(pp + HD + 1);
+            const float to = fmaxf(mm, mc), ref = to == -INFINITY ? 0.0f : to;
+            const float f = exp2_approx(mm - ref), fc = exp2_approx(mc - ref);
+            const float2 y0 = __ldcg(reinterpret_cast<const float2 *>(pp + d)), y1 = __ldcg(reinterpret_cast<const float2 *>(pp + d + 2));
+            mm = to;
+            ll = ll * f + lc * fc;
+            x = make_float4(x.x * f + y0.x * fc, x.y * f + y0.y * fc, x.z * f + y1.x * fc, x.w * f + y1.y * fc);
+        }
+        finish(r, d, x, mm, ll);
+    }
+}
+
+// ---- host side ----
+
+void fail(const std::string & what) { throw std::runtime_error(what); }
+
+Kv view(const bzb_kv8_cache & c, const bzb_kv8_batch & b) {
+    if (!c.pages || !c.scales || !c.page_table) fail("null pages, scales or page_table");
+    if (c.head_dim != 64 && c.head_dim != 128) fail("head_dim must be 64 or 128");
+    if (c.page_tokens < 16 || c.page_tokens > 256 || (c.page_tokens & (c.page_tokens - 1)))
+        fail("page_tokens must be 16, 32, 64, 128 or 256");
+    if (c.n_kv < 1 || c.n_kv > 4096) fail("n_kv must be 1 to 4096");
+    if (c.n_pages < 1 || c.n_slots < 1 || c.max_pages < 1) fail("n_pages, n_slots and max_pages must be positive");
+    if ((long long) c.max_pages * c.page_tokens > INT_MAX / 2) fail("max_pages x page_tokens is too large");
+    const long long page = 2ll * c.n_kv * c.page_tokens * c.head_dim;
+    if (c.page_stride < page || c.page_stride % 16) fail("page_stride must be a multiple of 16 and hold a page");
+    if (c.scale_stride < 2ll * c.n_kv * (c.page_tokens / 16)) fail("scale_stride must hold a page's scales");
+    if ((uintptr_t) c.pages % 16) fail("pages must be 16-byte aligned");
+    if ((uintptr_t) c.scales % 4 || (uintptr_t) c.page_table % 4 || (uintptr_t) c.status % 4)
+        fail("scales, page_table and status must be 4-byte aligned");
+    if (b.n_seq < 0 || b.n_tok < 0 || b.max_new < 0 || b.max_len < 0) fail("negative batch size");
+    if (b.n_seq > 0 && (!b.q_start || !b.kv_len)) fail("null q_start or kv_len");
+    if (!b.slots && b.n_seq > c.n_slots) fail("more sequences than page table rows and no slots");
+    if (b.max_len > (long long) c.max_pages * c.page_tokens) fail("max_len is more than a page table row holds");
+    if (b.max_new > (1 << 24) || b.n_seq > (1 << 24)) fail("max_new and n_seq must be at most 2^24");
+    Kv kv;
+    kv.pages = static_cast<uint8_t *>(c.pages);
+    kv.scales = c.scales;
+    kv.table = c.page_table;
+    kv.status = c.status;
+    kv.page_stride = c.page_stride;
+    kv.scale_stride = c.scale_stride;
+    kv.n_pages = c.n_pages;
+    kv.n_slots = c.n_slots;
+    kv.max_pages = c.max_pages;
+    kv.page_tokens = c.page_tokens;
+    kv.page_shift = __builtin_ctz((unsigned) c.page_tokens);
+    kv.n_kv = c.n_kv;
+    kv.q_start = b.q_start;
+    kv.kv_len = b.kv_len;
+    kv.slots = b.slots;
+    kv.n_seq = b.n_seq;
+    kv.n_tok = b.n_tok;
+    kv.max_new = b.max_new;
+    kv.max_len = b.max_len;
+    return kv;
+}
+
+// checks a row tensor and says whether groups of `n` elements of it are aligned to their size
+bool check_rows(const bzb_kv8_rows & r, const char * name, int heads, int hd, bool f32_allowed, int n, int n_tok) {
+    const std::string nm(name);
+    if (r.type != BZB_F16 && r.type != BZB_BF16 && !(f32_allowed && r.type == BZB_F32))
+        fail(nm + (f32_allowed ? ": type must be f32, f16 or bf16" : ": type must be f16 or bf16"));
+    if (r.n_head != heads) fail(nm + ": must have " + std::to_string(heads) + " heads");
+    if (n_tok > 0 && !r.data) fail(nm + ": null data");
+    if (r.row_stride < 0 || r.head_stride < 0 || (heads > 1 && r.head_stride < hd) || r.row_stride > (1ll << 40) ||
+        r.head_stride > (1ll << 40))
+        fail(nm + ": strides must be non-negative and heads may not overlap");
+    const int size = r.type == BZB_F32 ? 4 : 2;
+    if ((uintptr_t) r.data % size) fail(nm + ": data is not aligned to its type");
+    return (uintptr_t) r.data % (size * n) == 0 && r.row_stride % n == 0 && r.head_stride % n == 0;
+}
+// of an output: no two rows may share elements
+void check_distinct(const bzb_kv8_rows & r, const char * name, int hd, int n_tok) {
+    const long long span = (r.n_head - 1) * r.head_stride + hd;
+    const bool by_row = r.row_stride >= span, by_head = r.row_stride >= hd && r.head_stride >= (n_tok - 1) * r.row_stride + hd;
+    if (n_tok > 1 && !by_row && !by_head) fail(std::string(name) + ": rows overlap");
+}
+
+unsigned grid_of(long long tasks, int per_cta) {
+    const long long n = (tasks + per_cta - 1) / per_cta;
+    if (n > INT_MAX) fail("the batch is too large for one call");
+    return (unsigned) n;
+}
+
+template <int HD, int TYPE>
+void run_append(const AppendArgs & a, bool vec, cudaStream_t s) {
+    const unsigned grid = grid_of((long long) a.kv.n_seq * a.n_blk * (a.n_head + 2 * a.kv.n_kv), kRowWarps);
+    if (vec) kv8_append_kernel<HD, TYPE, true><<<grid, 32 * kRowWarps, 0, s>>>(a);
+    else kv8_append_kernel<HD, TYPE, false><<<grid, 32 * kRowWarps, 0, s>>>(a);
+    check_cuda(cudaGetLastError(), "launch");
+}
+
+// How the rows and the cache of a call are cut up.
+struct Plan {
+    int nt = 1, row_tiles = 1, chunks = 1, chunk_blocks = 1;
+};
+constexpr int kSmallWarps = 4;
+
+Plan plan_of(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int causal, int window) {
+    Plan p;
+    const int group = n_head / c.n_kv;
+    const long long rows = (long long) b.max_new * group;
+    const int most = c.head_dim == 64 ? 4 : 2;
+    while (p.nt < most && rows > 8 * p.nt) p.nt *= 2;
+    const long long tiles = std::max<long long>(1, (rows + 8 * p.nt - 1) / (8 * p.nt));
+    if (tiles > INT_MAX) fail("max_new x heads per kv head is too large");
+    p.row_tiles = (int) tiles;
+    long long keys = b.max_len;
+    if (causal && window > 0) keys = std::min<long long>(keys, (long long) window + (8 * p.nt + group - 1) / group + 1 + 15);
+    const int blocks = (int) std::max<long long>(1, (keys + 15) / 16 + (window > 0 ? 1 : 0));
+    // ranges: enough CTAs for two waves of four per SM, at least eight blocks (two a warp) in each
+    const long long units = std::max<long long>(1, (long long) b.n_seq * c.n_kv * p.row_tiles);
+    const long long want = std::max<long long>(1, 148 * 8 / units);
+    p.chunk_blocks = (int) std::max<long long>(8, (blocks + want - 1) / want);
+    p.chunks = (blocks + p.chunk_blocks - 1) / p.chunk_blocks;
+    return p;
+}
+
+long long counter_bytes(long long units) { return (units * 4 + 15) / 16 * 16; }
+
+template <int HD, int NT>
+void run_small(const AttnArgs & a, cudaStream_t s) {
+    const unsigned grid = grid_of((long long) a.kv.n_seq * a.row_tiles * a.chunks * a.kv.n_kv, 1);
+    kv8_attn_small_kernel<HD, NT, kSmallWarps><<<grid, 32 * kSmallWarps, 0, s>>>(a);
+    check_cuda(cudaGetLastError(), "launch");
+}
+
+void check_attention(const bzb_kv8_cache & c, int n_head, int causal, int window) {
+    if (n_head < 1 || n_head % c.n_kv) fail("the query heads must be a multiple of n_kv");
+    if (n_head > (1 << 16)) fail("too many query heads");
+    if (window < 0) fail("window must not be negative");
+    if (window > 0 && !causal) fail("a window needs causal attention");
+}
+
+}  // namespace
+
+void kv8_append(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_kv8_rows * q, const bzb_kv8_rows & k,
+                const bzb_kv8_rows & v, const bzb_kv8_rows * q_out, const float * q_norm, const float * k_norm, float eps,
+                const float * rope, int rope_len, cudaStream_t s) {
+    AppendArgs a;
+    a.kv = view(c, b);
+    if (!q != !q_out) fail("q and q_out come together");
+    if (k.type != v.type || (q && q->type != k.type)) fail("q, k and v must be of one type");
+    bool vec = check_rows(k, "k", c.n_kv, c.head_dim, true, 4, b.n_tok);
+    vec &= check_rows(v, "v", c.n_kv, c.head_dim, true, 4, b.n_tok);
+    a.n_head = 0;
+    a.q = a.q_out = Rows{ nullptr, 0, 0 };
+    a.q_out_type = BZB_F16;
+    a.q_out_vec = false;
+    if (q) {
+        a.n_head = q->n_head;
+        if (q->n_head < 1 || q->n_head > (1 << 16)) fail("q: between 1 and 65536 heads");
+        vec &= check_rows(*q, "q", q->n_head, c.head_dim, true, 4, b.n_tok);
+        a.q_out_vec = check_rows(*q_out, "q_out", q->n_head, c.head_dim, false, 4, b.n_tok);
+        check_distinct(*q_out, "q_out", c.head_dim, b.n_tok);
+        a.q = Rows{ q->data, q->row_stride, q->head_stride };
+        a.q_out = Rows{ q_out->data, q_out->row_stride, q_out->head_stride };
+        a.q_out_type = q_out->type;
+    }
+    if (!(eps >= 0.0f)) fail("eps must not be negative");
+    if ((uintptr_t) q_norm % 4 || (uintptr_t) k_norm % 4 || (uintptr_t) rope % 8) fail("q_norm, k_norm or rope is misaligned");
+    if (rope && rope_len < b.max_len) fail("rope has fewer positions than max_len");
+    if (b.n_seq == 0 || b.n_tok == 0 || b.max_new == 0 || b.max_len == 0) return;
+    a.k = Rows{ k.data, k.row_stride, k.head_stride };
+    a.v = Rows{ v.data, v.row_stride, v.head_stride };
+    a.q_norm = q_norm;
+    a.k_norm = k_norm;
+    a.rope = reinterpret_cast<const float2 *>(rope);
+    a.rope_len = rope_len;
+    a.eps = eps;
+    a.n_blk = (b.max_new + 30) / 16;  // blocks that max_new positions can touch
+    if (c.head_dim == 64) {
+        if (k.type == BZB_F32) run_append<64, BZB_F32>(a, vec, s);
+        else if (k.type == BZB_F16) run_append<64, BZB_F16>(a, vec, s);
+        else run_append<64, BZB_BF16>(a, vec, s);
+    } else {
+        if (k.type == BZB_F32) run_append<128, BZB_F32>(a, vec, s);
+        else if (k.type == BZB_F16) run_append<128, BZB_F16>(a, vec, s);
+        else run_append<128, BZB_BF16>(a, vec, s);
+    }
+}
+
+void kv8_read(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_kv8_rows & k_out, const bzb_kv8_rows & v_out,
+              cudaStream_t s) {
+    ReadArgs a;
+    a.kv = view(c, b);
+    a.vec = check_rows(k_out, "k_out", c.n_kv, c.head_dim, true, 4, b.n_tok);
+    a.vec &= check_rows(v_out, "v_out", c.n_kv, c.head_dim, true, 4, b.n_tok);
+    check_distinct(k_out, "k_out", c.head_dim, b.n_tok);
+    check_distinct(v_out, "v_out", c.head_dim, b.n_tok);
+    if (k_out.type != v_out.type) fail("k_out and v_out must be of one type");
+    if (b.n_seq == 0 || b.n_tok == 0 || b.max_new == 0) return;
+    a.k = Rows{ k_out.data, k_out.row_stride, k_out.head_stride };
+    a.v = Rows{ v_out.data, v_out.row_stride, v_out.head_stride };
+    a.type = k_out.type;
+    a.n_blk = (b.max_new + 30) / 16;
+    const unsigned grid = grid_of((long long) b.n_seq * a.n_blk * 2 * c.n_kv, kRowWarps);
+    if (c.head_dim == 64) kv8_read_kernel<64><<<grid, 32 * kRowWarps, 0, s>>>(a);
+    else kv8_read_kernel<128><<<grid, 32 * kRowWarps, 0, s>>>(a);
+    check_cuda(cudaGetLastError(), "launch");
+}
+
+long long kv8_attention_workspace(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int causal, int window) {
+    view(c, b);
+    check_attention(c, n_head, causal, window);
+    if (b.n_seq == 0 || b.n_tok == 0 || b.max_new == 0) return 0;
+    const Plan p = plan_of(c, b, n_head, causal, window);
+    if (p.chunks == 1) return 0;
+    const long long units = (long long) b.n_seq * p.row_tiles * c.n_kv;
+    return counter_bytes(units) + units * p.chunks * (8 * p.nt) * (c.head_dim + 2) * 4;
+}
+
+void kv8_attention(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_kv8_rows & q, const bzb_kv8_rows & out,
+                   float * lse, float scale, int causal, int window, void * workspace, long long workspace_bytes,
+                   cudaStream_t s) {
+    AttnArgs a;
+    a.kv = view(c, b);
+    if (q.n_head != out.n_head) fail("q and out must have the same heads");
+    check_attention(c, q.n_head, causal, window);
+    if (q.type != out.type) fail("q and out must be of one type");
+    a.q_vec = check_rows(q, "q", q.n_head, c.head_dim, false, 8, b.n_tok);
+    a.out_vec = check_rows(out, "out", q.n_head, c.head_dim, false, 4, b.n_tok);
+    check_distinct(out, "out", c.head_dim, b.n_tok);
+    if ((uintptr_t) lse % 4) fail("lse is misaligned");
+    const long long need = kv8_attention_workspace(c, b, q.n_head, causal, window);
+    if (need > 0 && (!workspace || workspace_bytes < need))
+        fail("workspace of " + std::to_string(need) + " bytes needed, " + std::to_string(workspace ? workspace_bytes : 0) + " given");
+    if (need > 0 && (uintptr_t) workspace % 16) fail("workspace must be 16-byte aligned");
+    if (b.n_seq == 0 || b.n_tok == 0 || b.max_new == 0) return;
+    const Plan p = plan_of(c, b, q.n_head, causal, window);
+    a.q = Rows{ q.data, q.row_stride, q.head_stride };
+    a.out = Rows{ out.data, out.row_stride, out.head_stride };
+    a.lse = lse;
+    a.scale2 = scale * kLog2e;
+    a.n_head = q.n_head;
+    a.group = q.n_head / c.n_kv;
+    a.causal = causal != 0;
+    a.window = window;
+    a.type = q.type;
+    a.row_tiles = p.row_tiles;
+    a.chunks = p.chunks;
+    a.chunk_blocks = p.chunk_blocks;
+    a.counters = static_cast<int *>(workspace);
+    a.part = need > 0 ? reinterpret_cast<float *>(static_cast<char *>(workspace) +
+                                                  counter_bytes((long long) b.n_seq * p.row_tiles * c.n_kv)) : nullptr;
+    if (c.head_dim == 64) {
+        if (p.nt == 1) run_small<64, 1>(a, s);
+        else if (p.nt == 2) run_small<64, 2>(a, s);
+        else run_small<64, 4>(a, s);
+    } else {
+        if (p.nt == 1) run_small<128, 1>(a, s);
+        else run_small<128, 2>(a, s);
+    }
+}
+
+}  // namespace bzb

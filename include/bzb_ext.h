@@ -126,6 +126,87 @@ BREEZE_API int bzb_generator_debug_sample(breeze_generator * gen, const float * 
                                           int * out_picks);
 BREEZE_API int bzb_debug_mbar_timeout(int device, long long polls);
 
+/* ---- 8-bit paged key/value cache (no counterpart in the reference, whose cache is f32) ----
+ * Keys and values in 8 bits (e4m3) with one scale for each block of 16 positions and head: half the
+ * bytes of the generator's f16 pages, for callers that run their own attention layers beside it. All
+ * buffers are the caller's and on one device; the calls only enqueue work on `stream` (NULL: the
+ * default stream), allocate nothing and can be captured in a CUDA graph.
+ *
+ * Layout. A page holds page_tokens positions (16, 32, 64, 128 or 256) of every head as bytes
+ * [K|V][n_kv][page_tokens][head_dim], head_dim 64 or 128; its scales are floats
+ * [K|V][n_kv][page_tokens / 16]. page_stride (bytes, a multiple of 16) and scale_stride (floats) lead
+ * from one page to the next, so a page may hold several layers with one descriptor for each. A scale is
+ * a power of two 2^e, e the smallest integer in [-24, 40] with 448 2^e >= the largest finite magnitude
+ * in the block (larger values saturate). A block of keys is 16 rows of head_dim bytes; a block of
+ * values is 4 x 4 patches [head_dim / 4][4 position groups][4 of head_dim][4 positions], the order in
+ * which the attention kernels' matrix operands want it. page_table[slot][i] is the page of positions
+ * [i page_tokens, (i + 1) page_tokens).
+ *
+ * Batches. Sequence b has the packed rows [q_start[b], q_start[b + 1]) of the row tensors and kv_len[b]
+ * cached positions, these rows' own included: its row t stands for position
+ * kv_len[b] - n_b + t, n_b its number of rows. Rows of a negative position are padding: append skips
+ * them, attention and read give zeros (kv_len[b] = 0 makes a whole sequence padding). slots[b]
+ * is its row of page_table (NULL: b). q_start, kv_len and slots are read on the device when the work
+ * runs; max_new >= every n_b and max_len >= every kv_len[b] are bounds that the host knows.
+ *
+ * What only the device can see -- a page or slot out of range, a sequence that breaks its bounds -- is
+ * not followed: `status` (one int on the device, may be NULL) is set to 1 and the sequence is skipped
+ * (its outputs are not written) or the page read as page 0, never written. The caller clears it. */
+enum { BZB_F32 = 0, BZB_F16 = 1, BZB_BF16 = 2 };
+typedef struct bzb_kv8_cache {
+    void * pages;
+    float * scales;
+    const int * page_table;  /* [n_slots][max_pages] */
+    int * status;
+    long long page_stride, scale_stride;
+    int n_pages, n_slots, max_pages, page_tokens, n_kv, head_dim;
+    int device;              /* the device of all buffers */
+} bzb_kv8_cache;
+typedef struct bzb_kv8_batch {
+    const int * q_start;     /* [n_seq + 1] */
+    const int * kv_len;      /* [n_seq] */
+    const int * slots;       /* [n_seq] or NULL */
+    int n_seq, n_tok, max_new, max_len;
+} bzb_kv8_batch;
+/* n_tok rows of n_head heads of head_dim elements of `type` (contiguous within a head), strides in elements */
+typedef struct bzb_kv8_rows {
+    void * data;
+    long long row_stride, head_stride;
+    int n_head, type;
+} bzb_kv8_rows;
+
+/* Norms and rotates every new row's queries and keys and appends its keys and values, in one launch:
+ *   q_out = rot(x w_q / sqrt(mean(x^2) + eps)), the same with w_k for the keys, values unchanged;
+ *   rot turns the pairs (i, i + head_dim / 2) by the row's position: rope [rope_len][head_dim / 2][2]
+ *   holds (cos, sin).
+ * q_norm / k_norm [head_dim] or NULL (no norm), rope or NULL (no rotation); q and q_out both NULL
+ * when only keys and values are wanted. q, k, v of one type (f32, f16 or bf16), q_out f16 or bf16; q_out
+ * may not overlap q. A block that already holds earlier positions of its sequence takes the larger of
+ * its scale and the new values' one; the earlier values are then rescaled (exactly, except where they
+ * fall below the smallest e4m3). Infinities and NaN are stored as NaN and do not count for the scale.
+ * Positions of a written block past kv_len become zero. Two sequences of one call may not share a
+ * page they append to. Returns 0, or -1 with breeze_last_error(). */
+BREEZE_API int bzb_kv8_append(const bzb_kv8_cache * cache, const bzb_kv8_batch * batch, const bzb_kv8_rows * q,
+                              const bzb_kv8_rows * k, const bzb_kv8_rows * v, const bzb_kv8_rows * q_out,
+                              const float * q_norm, const float * k_norm, float eps, const float * rope, int rope_len,
+                              void * stream);
+/* Reads the batch's positions back: k_out, v_out rows of f32, f16 or bf16. 0, or -1 with breeze_last_error(). */
+BREEZE_API int bzb_kv8_read(const bzb_kv8_cache * cache, const bzb_kv8_batch * batch, const bzb_kv8_rows * k_out,
+                            const bzb_kv8_rows * v_out, void * stream);
+/* Attention of the batch's rows over their sequences' cached positions:
+ *   out[row][h] = sum_j p_j v_j, p = softmax_j(scale q[row][h] . k_j), kv head h / (n_head / n_kv);
+ * causal != 0: the keys up to the row's own position, and with window > 0 only the last `window` of them;
+ * causal == 0 (window 0): all kv_len keys. A row without any key gives zeros. lse, when not NULL, gets
+ * log(sum_j exp(scale q . k_j)) as [n_tok][n_head] (-inf without keys), for merging with attention over
+ * other keys. q and out of one type, f16 or bf16. `workspace`: bzb_kv8_attention_workspace() bytes
+ * (0: none needed) on the device, 16-byte aligned, zeroed once by the caller before its first use and left fit for
+ * the next call by every call; calls that may overlap need one each. 0, or -1 with breeze_last_error(). */
+BREEZE_API long long bzb_kv8_attention_workspace(const bzb_kv8_cache * cache, const bzb_kv8_batch * batch, int n_head,
+                                                 int causal, int window);
+BREEZE_API int bzb_kv8_attention(const bzb_kv8_cache * cache, const bzb_kv8_batch * batch, const bzb_kv8_rows * q,
+                                 const bzb_kv8_rows * out, float * lse, float scale, int causal, int window,
+                                 void * workspace, long long workspace_bytes, void * stream);
+
 /* average microseconds of back-to-back launches of one dequant-GEMM of a named Q8_0 tensor on
    `rows` activation rows (epilogue 0 store, 1 residual add, 2 SwiGLU, 3 GeGLU), or -1 */
 BREEZE_API double bzb_generator_bench_gemv(breeze_generator * gen, const char * tensor, int sub, int rows, int iters,
