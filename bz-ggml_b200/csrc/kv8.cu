@@ -1,173 +1,18 @@
 // Kernels of the 8-bit paged key/value cache (include/bzb_ext.h, bzb_kv8_*): appending with the q/k
-// norms and the rotation in the same pass, reading back, and attention over the cache.
-//
-// Numbers. A cached value is an e4m3 byte times its block's scale 2^e (16 positions of one head). e4m3
-// converts to f16 exactly, so the attention kernels multiply the bytes as f16 and bring the scales in
-// where they are one number for a whole block: 2^e of the keys multiplies the scores, 2^e of the
-// values goes into the exponent of the weights (see attention below). A power of two costs e4m3 no
-// precision, since its relative spacing is the same at every magnitude, and lets an append
-// rescale a block's earlier values without rounding them again (except below the smallest normal).
-#include "kv8.h"
-#include "tc_ptx.cuh"
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
+// norms and the rotation in the same pass, reading back, and attention of few rows (a step of each
+// sequence, a few guessed tokens); attention of many rows is in kv8_tile.cu.
+#include "kv8_dev.cuh"
 
 #include <algorithm>
 #include <climits>
 #include <cmath>
-#include <cstdint>
 #include <stdexcept>
 #include <string>
-#include <utility>
 
 namespace bzb {
 namespace {
 
-constexpr int kExpMin = -24, kExpMax = 40;
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-
-void check_cuda(cudaError_t e, const char * what) {
-    if (e != cudaSuccess) throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(e));
-}
-
-// what every kernel needs of the cache and the batch
-struct Kv {
-    uint8_t * pages;
-    float * scales;
-    const int * table;
-    int * status;
-    long long page_stride, scale_stride;
-    int n_pages, n_slots, max_pages, page_tokens, page_shift, n_kv;
-    const int * q_start, * kv_len, * slots;
-    int n_seq, n_tok, max_new, max_len;
-};
-
-struct Rows {
-    void * p;
-    long long row, head;  // strides in elements
-};
-
-struct Seq {
-    int row0, n, len, slot;  // first packed row, rows, cached positions, page table row (-1: skip the sequence)
-};
-
-__device__ __forceinline__ void complain(const Kv & kv) {
-    if (kv.status) atomicExch(kv.status, 1);
-}
-
-__device__ __forceinline__ Seq load_seq(const Kv & kv, int b) {
-    Seq s;
-    s.row0 = kv.q_start[b];
-    const int end = kv.q_start[b + 1];
-    s.n = end - s.row0;
-    s.len = kv.kv_len[b];
-    s.slot = kv.slots ? kv.slots[b] : b;
-    // (end and row0 are compared before their difference is used: it may overflow)
-    if (s.row0 < 0 || end < s.row0 || end > kv.n_tok || s.n > kv.max_new || s.len < 0 || s.len > kv.max_len || s.slot < 0 ||
-        s.slot >= kv.n_slots) {
-        complain(kv);
-        s.slot = -1;
-    }
-    return s;
-}
-
-// the page of block `blk` (16 positions) of a sequence, or -1
-__device__ __forceinline__ int page_of(const Kv & kv, int slot, int blk) {
-    const int pg = __ldg(kv.table + (size_t) slot * kv.max_pages + (blk >> (kv.page_shift - 4)));
-    if ((unsigned) pg >= (unsigned) kv.n_pages) {
-        complain(kv);
-        return -1;
-    }
-    return pg;
-}
-__device__ __forceinline__ uint8_t * block_ptr(const Kv & kv, int pg, int blk, int plane, int head, int hd) {
-    const int at = (blk << 4) & (kv.page_tokens - 1);
-    return kv.pages + pg * kv.page_stride + ((size_t) (plane * kv.n_kv + head) * kv.page_tokens + at) * hd;
-}
-__device__ __forceinline__ float * scale_ptr(const Kv & kv, int pg, int blk, int plane, int head) {
-    const int per = kv.page_tokens >> 4;
-    return kv.scales + pg * kv.scale_stride + (plane * kv.n_kv + head) * per + (blk & (per - 1));
-}
-
-__device__ __forceinline__ float pow2f(int e) { return __int_as_float((e + 127) << 23); }
-__device__ __forceinline__ int exponent_of(float pow2) { return (__float_as_int(pow2) >> 23) - 127; }
-// smallest e with 448 2^e >= x (448 = 1.75 2^8), clamped; x >= 0 and finite
-__device__ __forceinline__ int block_exponent(float x) {
-    const int bits = __float_as_int(x);
-    const int e = (bits >> 23) - 127 - 8 + ((bits & 0x7fffff) > 0x600000);
-    return max(kExpMin, min(kExpMax, e));  // (subnormals and zero have exponent field 0: clamped)
-}
-
-// four floats -> four e4m3 bytes, nearest with ties to even; NaN stays NaN
-__device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d) {
-    uint16_t lo, hi;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
-    return (uint32_t) lo | ((uint32_t) hi << 16);
-}
-__device__ __forceinline__ uint32_t e4m3x2_to_h2(uint16_t v) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
-    return r;
-}
-__device__ __forceinline__ float4 e4m3x4_to_f4(uint32_t w) {
-    const uint32_t lo = e4m3x2_to_h2((uint16_t) w), hi = e4m3x2_to_h2((uint16_t) (w >> 16));
-    const float2 a = __half22float2(*reinterpret_cast<const half2 *>(&lo));
-    const float2 b = __half22float2(*reinterpret_cast<const half2 *>(&hi));
-    return make_float4(a.x, a.y, b.x, b.y);
-}
-
-// ---- four consecutive elements of a row, by type; VEC: they are aligned to their size ----
-template <int TYPE, bool VEC>
-__device__ __forceinline__ float4 load4(const void * p, long long i) {
-    if constexpr (TYPE == BZB_F32) {
-        const float * f = static_cast<const float *>(p) + i;
-        if constexpr (VEC) return __ldg(reinterpret_cast<const float4 *>(f));
-        return make_float4(f[0], f[1], f[2], f[3]);
-    } else if constexpr (TYPE == BZB_F16) {
-        const half * h = static_cast<const half *>(p) + i;
-        if constexpr (VEC) {
-            const uint2 u = __ldg(reinterpret_cast<const uint2 *>(h));
-            const float2 a = __half22float2(*reinterpret_cast<const half2 *>(&u.x));
-            const float2 b = __half22float2(*reinterpret_cast<const half2 *>(&u.y));
-            return make_float4(a.x, a.y, b.x, b.y);
-        }
-        return make_float4(__half2float(h[0]), __half2float(h[1]), __half2float(h[2]), __half2float(h[3]));
-    } else {
-        const __nv_bfloat16 * h = static_cast<const __nv_bfloat16 *>(p) + i;
-        if constexpr (VEC) {
-            const uint2 u = __ldg(reinterpret_cast<const uint2 *>(h));
-            return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
-                               __uint_as_float(u.y & 0xffff0000u));
-        }
-        return make_float4(__bfloat162float(h[0]), __bfloat162float(h[1]), __bfloat162float(h[2]), __bfloat162float(h[3]));
-    }
-}
-__device__ __forceinline__ uint32_t pack_half(float a, float b) {
-    const half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ void store4(int type, bool vec, void * p, long long i, float4 x) {
-    if (type == BZB_F32) {
-        float * f = static_cast<float *>(p) + i;
-        if (vec) *reinterpret_cast<float4 *>(f) = x;
-        else f[0] = x.x, f[1] = x.y, f[2] = x.z, f[3] = x.w;
-    } else {
-        const uint2 u = type == BZB_F16 ? make_uint2(pack_half(x.x, x.y), pack_half(x.z, x.w))
-                                        : make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
-        uint16_t * h = static_cast<uint16_t *>(p) + i;
-        if (vec) *reinterpret_cast<uint2 *>(h) = u;
-        else {
-            h[0] = (uint16_t) u.x, h[1] = (uint16_t) (u.x >> 16);
-            h[2] = (uint16_t) u.y, h[3] = (uint16_t) (u.y >> 16);
-        }
-    }
-}
+using namespace kv8;
 
 // ---- append and read: one warp per (sequence, block of 16 positions, head of q, k or v) ----
 //
@@ -406,28 +251,6 @@ __global__ void __launch_bounds__(32 * kRowWarps) kv8_read_kernel(const ReadArgs
     }
 }
 
-// ---- attention ----
-//
-// For a row with scores s_j (in powers of two: scale log2(e) q.k_j) and values 2^{e_j} v_j, the weights
-// are kept relative to M = max_j (s_j + e_j):
-//   w_j = 2^(s_j + e_j - M) <= 1,  O = sum_j w_j v_j,  l = sum_j w_j 2^-e_j,  out = O / l,
-//   log-sum-exp = ln 2 (M + log2 l),
-// so the f16 weights of the second product carry the values' block scales, and the sum undoes them
-// in f32 (|e| <= 40: no weight that matters underflows). M, l and O are f32 and updated
-// block by block.
-struct AttnArgs {
-    Kv kv;
-    Rows q, out;
-    float * lse;
-    float scale2;  // scale log2(e)
-    int n_head, group, causal, window;
-    int type;      // of q and out
-    bool q_vec, out_vec;
-    int row_tiles, chunks, chunk_blocks;
-    float * part;
-    int * counters;
-};
-
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -439,20 +262,12 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ uint4 load_stream(const void * p) {
     uint4 v;
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
-// bytes of w that are e4m3 NaN (0x7f or 0xff) become 0xff, the others 0
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
-
 // 16 elements of a query row from element i as f16 pairs: f16 rows as they are, bf16 rows times f (and
 // their largest magnitude into amax)
 __device__ __forceinline__ void load_q16(const AttnArgs & a, long long i, float f, uint32_t (&o)[8], float * amax) {
@@ -501,7 +316,7 @@ __device__ __forceinline__ void load_q16(const AttnArgs & a, long long i, float 
 // transposition but the 8x8 one of the weights; per lane 4 loads of 16 bytes a block for head_dim 64.
 template <int HD, int NT, int WARPS>
 struct SmallTile {
-    static constexpr int ROWS = 8 * NT, KS = HD / 64, VS = HD / 32, MT = HD / 16, PL = HD + 2;
+    static constexpr int ROWS = 8 * NT, KS = HD / 64, VS = HD / 32, MT = HD / 16, PL = HD + 4;
 };
 
 template <int HD, int NT, int WARPS>
@@ -811,6 +626,10 @@ __global__ void __launch_bounds__(32 * WARPS) kv8_attn_small_kernel(const AttnAr
 
 // ---- host side ----
 
+void check_cuda(cudaError_t e, const char * what) {
+    if (e != cudaSuccess) throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(e));
+}
+
 void fail(const std::string & what) { throw std::runtime_error(what); }
 
 Kv view(const bzb_kv8_cache & c, const bzb_kv8_batch & b) {
@@ -892,26 +711,39 @@ void run_append(const AppendArgs & a, bool vec, cudaStream_t s) {
 
 // How the rows and the cache of a call are cut up.
 struct Plan {
-    int nt = 1, row_tiles = 1, chunks = 1, chunk_blocks = 1;
+    bool tile = false;      // kv8_tile.cu's kernel
+    int nt = 1;             // else: tiles of 8 rows that a CTA of the few-row kernel holds
+    int rows = 8;           // rows of a CTA
+    int row_tiles = 1, chunks = 1, chunk_blocks = 1;
 };
 constexpr int kSmallWarps = 4;
+constexpr int kFewRows = 64;
 
 Plan plan_of(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int causal, int window) {
     Plan p;
     const int group = n_head / c.n_kv;
     const long long rows = (long long) b.max_new * group;
-    const int most = c.head_dim == 64 ? 4 : 2;
-    while (p.nt < most && rows > 8 * p.nt) p.nt *= 2;
-    const long long tiles = std::max<long long>(1, (rows + 8 * p.nt - 1) / (8 * p.nt));
+    p.tile = rows > kFewRows;
+    if (p.tile) {
+        p.rows = kTileRows;
+    } else {
+        const int most = c.head_dim == 64 ? 4 : 2;
+        while (p.nt < most && rows > 8 * p.nt) p.nt *= 2;
+        p.rows = 8 * p.nt;
+    }
+    const long long tiles = std::max<long long>(1, (rows + p.rows - 1) / p.rows);
     if (tiles > INT_MAX) fail("max_new x heads per kv head is too large");
     p.row_tiles = (int) tiles;
+    // blocks that one CTA's rows look at: its tokens' windows, at any offset within a block
     long long keys = b.max_len;
-    if (causal && window > 0) keys = std::min<long long>(keys, (long long) window + (8 * p.nt + group - 1) / group + 1 + 15);
+    if (causal && window > 0) keys = std::min<long long>(keys, (long long) window + (p.rows + group - 1) / group + 1 + 15);
     const int blocks = (int) std::max<long long>(1, (keys + 15) / 16 + (window > 0 ? 1 : 0));
-    // ranges: enough CTAs for two waves of four per SM, at least eight blocks (two a warp) in each
     const long long units = std::max<long long>(1, (long long) b.n_seq * c.n_kv * p.row_tiles);
-    const long long want = std::max<long long>(1, 148 * 8 / units);
-    p.chunk_blocks = (int) std::max<long long>(8, (blocks + want - 1) / want);
+    // few-row kernel: enough CTAs for two waves of four per SM, at least eight blocks (two a warp) in each range;
+    // tile kernel: one CTA per SM, at least two tiles of 128 keys in each range
+    const long long want = std::max<long long>(1, (p.tile ? 148 : 148 * 8) / units);
+    p.chunk_blocks = (int) std::max<long long>(p.tile ? 16 : 8, (blocks + want - 1) / want);
+    if (p.tile) p.chunk_blocks = (p.chunk_blocks + 7) / 8 * 8;
     p.chunks = (blocks + p.chunk_blocks - 1) / p.chunk_blocks;
     return p;
 }
@@ -1007,7 +839,7 @@ long long kv8_attention_workspace(const bzb_kv8_cache & c, const bzb_kv8_batch &
     const Plan p = plan_of(c, b, n_head, causal, window);
     if (p.chunks == 1) return 0;
     const long long units = (long long) b.n_seq * p.row_tiles * c.n_kv;
-    return counter_bytes(units) + units * p.chunks * (8 * p.nt) * (c.head_dim + 2) * 4;
+    return counter_bytes(units) + units * p.chunks * p.rows * (c.head_dim + 4) * 4;
 }
 
 void kv8_attention(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_kv8_rows & q, const bzb_kv8_rows & out,
@@ -1043,7 +875,9 @@ void kv8_attention(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_k
     a.counters = static_cast<int *>(workspace);
     a.part = need > 0 ? reinterpret_cast<float *>(static_cast<char *>(workspace) +
                                                   counter_bytes((long long) b.n_seq * p.row_tiles * c.n_kv)) : nullptr;
-    if (c.head_dim == 64) {
+    if (p.tile) {
+        launch_attn_tile(a, c.head_dim, s);
+    } else if (c.head_dim == 64) {
         if (p.nt == 1) run_small<64, 1>(a, s);
         else if (p.nt == 2) run_small<64, 2>(a, s);
         else run_small<64, 4>(a, s);
