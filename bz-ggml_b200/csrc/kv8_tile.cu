@@ -3,14 +3,15 @@
 //
 // One CTA takes up to 256 rows of one kv head -- (token, head of the group) pairs, so the group shares
 // the cache's tiles -- as two M = 128 tiles, and walks its keys 128 at a time:
-//   producers (4 warps)  bytes of 128 keys and values from global memory to registers, one tile ahead;
+//   producers (4 + 4 warps)  bytes of 128 keys and values from global memory to registers, one tile ahead;
 //                        converted to f16 into shared memory in the MMAs' swizzled layout (two stages),
 //                        the blocks' scales beside them;
-//   MMA (1 thread)       S_i = Q_i K^T into tensor memory, O_i += W_i V with the weights W_i read from
-//                        tensor memory;
+//   MMA (4 warps)        S_i = Q_i K^T into tensor memory, O_i += W_i V with the weights W_i read from
+//                        tensor memory, in steps of 64 keys: two buffers of scores a tile fit beside the
+//                        outputs, so the scores of the next step are there when a softmax ends. Each of the
+//                        four chains has a warp of its own, so that one's waits are under another's MMAs;
 //   softmax (4 warps a tile, one row a thread)  S_i from tensor memory, the running maximum and sum,
-//                        the weights back to tensor memory as f16.
-// While one tile's rows are in the softmax, the other's products run. The exponentials bound it: 16 a
+//                        the weights back to tensor memory as f16. The exponentials bound it: 16 a
 // clock and SM against 4096 multiply-adds, so for head_dim 64 a tile of 128 x 128 scores costs 1024 clocks there
 // and 512 in the MMAs; no key is converted more than once for 256 rows.
 // O is rescaled only when a row's maximum has grown by more than 2^8 since the last time (the
@@ -29,10 +30,14 @@ namespace {
 
 using namespace tc;
 
-constexpr int kKeys = 128;                 // keys of a tile
-constexpr int kProducers = 4, kSoftmax = 8;
-constexpr int kMmaWarp = kSoftmax + kProducers;
-constexpr int kTileThreads = 32 * (kMmaWarp + 1);
+constexpr int kKeys = 128, kStep = 64;     // keys of a stage in shared memory; of a step of the softmax
+constexpr int kProducers = 4, kSoftmax = 8;  // warps: of keys and of values each; of both tiles' softmax
+constexpr int kMmaWarp = kSoftmax + 2 * kProducers;
+constexpr int kTileThreads = 32 * (kMmaWarp + 4);
+// registers a thread: at launch, and after the softmax warps have taken what the others give back
+constexpr int kLaunchRegs = 96, kSoftmaxRegs = 144, kOtherRegs = 64;
+static_assert(32 * kSoftmax * kSoftmaxRegs + (kTileThreads - 32 * kSoftmax) * kOtherRegs <= kTileThreads * kLaunchRegs,
+              "the warps' registers must fit those of the launch");
 constexpr float kSlack = 8.0f;             // how far (powers of two) weights may exceed 1 before O is rescaled
 
 template <int HD>
@@ -41,21 +46,20 @@ struct Smem {
     static constexpr int kQ = 128 * HD * 2, kK = kKeys * HD * 2, kV = kKeys * HD * 2;
     static constexpr int oQ = 0, oK = 2 * kQ, oV = oK + 2 * kK, oEnd = oV + 2 * kV;
     static constexpr size_t kBytes = 1024 + oEnd;
-    // tensor memory columns: scores of the two tiles, outputs; the weights of head_dim 64 have
-    // columns of their own, those of head_dim 128 lie over the scores they came from
-    static constexpr int cO = 2 * kKeys, cW = HD == 64 ? cO + 2 * HD : 0;
-    static constexpr int kWStride = HD == 64 ? kKeys / 2 : kKeys;
-    static constexpr bool kOver = HD != 64;
+    // tensor memory columns: two buffers of scores for each tile, then the tiles' outputs. A step's weights
+    // (f16, 32 columns) lie over its scores
+    static constexpr int cO = 4 * kStep;
 };
 
 struct Shared {
-    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], w_full[2], o_full[2], pv_done[2], drain;
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], o_full[2], drain[4];
+    uint64_t s_full[2][2], w_full[2][2], pv_done[2][2];  // [tile][step & 1]
     uint64_t c_full[4], n_full[4];  // scale[] and nan_v[] of a tile (rings of four: see the producers)
     uint32_t tmem;
     int err;
     int last;
     int nan_v[4][kProducers];   // a producer warp found NaN values in this tile (only where it looked)
-    float scale[4][8][4];       // per block of 16 keys: scale of the keys, exponent of the values' scale, 2^-it
+    float4 scale[4][8];         // per block of 16 keys: scale of the keys, exponent of the values' scale, 2^-it
     float unit[2][128];         // power of two taken out of each query row
 };
 
@@ -69,7 +73,28 @@ __device__ __forceinline__ void ld32(uint32_t addr, uint32_t (&r)[32]) {
           "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
 }
+// two f32 operations an instruction
+__device__ __forceinline__ float2 pair(uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); }
+__device__ __forceinline__ float2 fma2(float2 a, float b, float c) { return __ffma2_rn(a, make_float2(b, b), make_float2(c, c)); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+// scores of 16 keys from key0: those outside [lo, hi) become -inf
+__device__ __forceinline__ void mask(float2 (&s)[8], int key0, int lo, int hi) {
+#pragma unroll
+    for (int t = 0; t < 8; t++) {
+        const int key = key0 + 2 * t;
+        if (key < lo || key >= hi) s[t].x = -INFINITY;
+        if (key + 1 < lo || key + 1 >= hi) s[t].y = -INFINITY;
+    }
+}
+
 __device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&r)[16]) { tmem_st16(addr, r); }
+
+// one lane of a converged warp, the same one every time
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
 
 // a whole warp's bounded wait: all lanes succeed, or all take it as failed
 __device__ __forceinline__ bool warp_wait(uint64_t * bar, uint32_t parity, int * err) {
@@ -115,24 +140,14 @@ __device__ __forceinline__ bool find_work(const AttnArgs & a, Work & w) {
     return true;
 }
 
-// 8 consecutive query elements as f16 pairs times f (f16 rows: unchanged)
-__device__ __forceinline__ uint4 load_q8(const AttnArgs & a, long long i, float (&x)[8]) {
+// 8 consecutive query elements, as they are
+__device__ __forceinline__ uint4 load_q8(const AttnArgs & a, long long i) {
     const uint16_t * p = static_cast<const uint16_t *>(a.q.p) + i;
-    uint4 u;
-    if (a.q_vec) {
-        u = *reinterpret_cast<const uint4 *>(p);
-    } else {
-        uint32_t w[4];
+    if (a.q_vec) return *reinterpret_cast<const uint4 *>(p);
+    uint32_t w[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) w[j] = (uint32_t) p[2 * j] | ((uint32_t) p[2 * j + 1] << 16);
-        u = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    if (a.type == BZB_BF16) {
-        const uint32_t w[4] = { u.x, u.y, u.z, u.w };
-#pragma unroll
-        for (int j = 0; j < 4; j++) x[2 * j] = __uint_as_float(w[j] << 16), x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-    }
-    return u;
+    for (int j = 0; j < 4; j++) w[j] = (uint32_t) p[2 * j] | ((uint32_t) p[2 * j + 1] << 16);
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // a softmax warp's 32 query rows into the swizzled tile; rows that do not exist become zero
@@ -140,16 +155,25 @@ template <int HD>
 __device__ __forceinline__ void load_queries(const AttnArgs & a, const Work & w, Shared & sh, uint8_t * sq, int tile, int quarter, int lane) {
     constexpr int LPR = HD / 8, RPP = 32 / LPR;  // lanes of a row, rows of a pass
     const int c = lane % LPR;
+    uint4 u[LPR];
+    // (all of them under way before the first is used)
+#pragma unroll
     for (int p = 0; p < LPR; p++) {
-        const int r = quarter * 32 + p * RPP + lane / LPR, rr = w.row0 + tile * 128 + r;
-        uint4 u = make_uint4(0, 0, 0, 0);
-        float unit = 1.0f;
-        float x[8] = {};
+        const int rr = w.row0 + tile * 128 + quarter * 32 + p * RPP + lane / LPR;
+        u[p] = make_uint4(0, 0, 0, 0);
         if (rr < w.rows)
-            u = load_q8(a, (long long) (w.s.row0 + rr / a.group) * a.q.row + (w.h * a.group + rr % a.group) * a.q.head + 8 * c, x);
+            u[p] = load_q8(a, (long long) (w.s.row0 + rr / a.group) * a.q.row + (w.h * a.group + rr % a.group) * a.q.head + 8 * c);
+    }
+#pragma unroll
+    for (int p = 0; p < LPR; p++) {
+        const int r = quarter * 32 + p * RPP + lane / LPR;
+        float unit = 1.0f;
         if (a.type == BZB_BF16) {
             // bf16 may lie outside f16: the row is brought to about [1, 2) by a power of two
-            float amax = 0.0f;
+            const uint32_t v[4] = { u[p].x, u[p].y, u[p].z, u[p].w };
+            float x[8], amax = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[2 * j] = __uint_as_float(v[j] << 16), x[2 * j + 1] = __uint_as_float(v[j] & 0xffff0000u);
 #pragma unroll
             for (int j = 0; j < 8; j++) amax = fmaxf(amax, fabsf(x[j]));
 #pragma unroll
@@ -157,115 +181,119 @@ __device__ __forceinline__ void load_queries(const AttnArgs & a, const Work & w,
             const int e = amax < INFINITY && amax > 0.0f ? min(126, max(-125, (__float_as_int(amax) >> 23) - 127)) : 0;
             unit = pow2f(e);
             const float f = pow2f(-e);
-            u = make_uint4(pack_half(x[0] * f, x[1] * f), pack_half(x[2] * f, x[3] * f), pack_half(x[4] * f, x[5] * f),
-                           pack_half(x[6] * f, x[7] * f));
+            u[p] = make_uint4(pack_half(x[0] * f, x[1] * f), pack_half(x[2] * f, x[3] * f), pack_half(x[4] * f, x[5] * f),
+                              pack_half(x[6] * f, x[7] * f));
         }
-        *reinterpret_cast<uint4 *>(sq + (c / 8) * Smem<HD>::kHalf + r * 128 + (((c % 8) ^ (r & 7)) << 4)) = u;
+        *reinterpret_cast<uint4 *>(sq + (c / 8) * Smem<HD>::kHalf + r * 128 + (((c % 8) ^ (r & 7)) << 4)) = u[p];
         if (c == 0) sh.unit[tile][r] = unit;
     }
 }
 
-// ---- producers: tile after tile of keys and values, bytes to swizzled f16 ----
-template <int HD>
-struct Producer {
-    static constexpr int NK = HD / 16;  // 16-byte pieces of keys a thread takes of a tile (128 threads)
-    static constexpr int NV = HD / 32;  // 32-byte pieces (two patches) of values
-    uint4 k[NK], v[NV][2];
-    const AttnArgs & a;
-    const Work & w;
-    int tid, lane;
+// ---- producers: tile after tile, bytes in registers to swizzled f16 ----
+//
+// Four warps bring the keys, four the values. A thread's pieces of a tile lie at the same place of
+// successive blocks, so their addresses differ by the blocks' alone.
+__device__ __forceinline__ const uint8_t * shfl_ptr(const uint8_t * p, int lane) {
+    return reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(p), lane));
+}
 
-    // (page of each block, one block per lane 0..7; -1 past the last)
-    __device__ int pages(int j) const {
-        const int blk = w.blk0 + 8 * j + (lane & 7);
-        if (j >= w.n_tiles || blk >= w.blk_hi) return -1;
-        return max(page_of(a.kv, w.s.slot, blk), 0);
+// block b (0..7) of tile j, one block per lane (lane & 7): its page, or -1 past the last
+__device__ __forceinline__ int tile_page(const AttnArgs & a, const Work & w, int j, int lane) {
+    const int blk = w.blk0 + 8 * j + (lane & 7);
+    return j < w.n_tiles && blk < w.blk_hi ? max(page_of(a.kv, w.s.slot, blk), 0) : -1;
+}
+
+template <int HD>
+struct Keys {
+    static constexpr int N = HD / 16;  // 16-byte pieces of a tile for each of 128 threads
+    uint4 x[N];
+    int in_block, dst, first, step;    // bytes into a block; bytes into the tile; block of piece 0, blocks between pieces
+
+    __device__ explicit Keys(int tid) {
+        // row of the block and 16 bytes of the row, so that the lanes of a store fall on different banks
+        const int row = HD == 64 ? tid >> 2 : ((tid >> 2) & 1) | (tid >> 4) << 1;
+        const int c = HD == 64 ? tid & 3 : (tid & 3) | ((tid >> 3) & 1) << 2;
+        in_block = (row & 15) * HD + 16 * c;
+        first = row >> 4;
+        step = HD == 64 ? 2 : 1;
+        dst = (c >> 2) * Smem<HD>::kHalf + row * 128 + ((((c & 3) * 2) ^ (row & 7)) << 4);
     }
-    // row of the tile and 16-byte piece of the row: lanes of a store phase fall on different banks
-    __device__ static void key_piece(int i, int & row, int & c) {
-        if (HD == 64) {
-            row = i >> 2, c = i & 3;
-        } else {
-            c = (i & 3) | ((i >> 3) & 1) << 2;
-            row = ((i >> 2) & 1) | (i >> 4) << 1;
+    __device__ void load(const uint8_t * block) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const uint8_t * p = shfl_ptr(block, first + step * i);
+            x[i] = make_uint4(0, 0, 0, 0);
+            if (p) x[i] = __ldg(reinterpret_cast<const uint4 *>(p + in_block));
         }
     }
-    // block of the tile, group of 4 elements, pair of position groups
-    __device__ static void value_piece(int i, int & kb, int & q, int & u) {
-        u = i & 1;
-        q = (i >> 3) & (HD / 4 - 1);
-        kb = ((i >> 1) & 3) | (i / (HD / 4 * 8)) << 2;
-    }
-    __device__ void load_k(int j, int pg) {
+    __device__ void store(uint8_t * tile) const {
 #pragma unroll
-        for (int i = 0; i < NK; i++) {
-            int row, c;
-            key_piece(i * 128 + tid, row, c);
-            const int p = __shfl_sync(0xffffffffu, pg, row >> 4);
-            k[i] = make_uint4(0, 0, 0, 0);
-            if (p >= 0) {
-                const uint8_t * src = block_ptr(a.kv, p, w.blk0 + 8 * j + (row >> 4), 0, w.h, HD) + (row & 15) * HD + 16 * c;
-                k[i] = __ldg(reinterpret_cast<const uint4 *>(src));
-            }
-        }
-    }
-    __device__ void load_v(int j, int pg) {
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-            int kb, q, u;
-            value_piece(i * 128 + tid, kb, q, u);
-            const int p = __shfl_sync(0xffffffffu, pg, kb);
-            v[i][0] = v[i][1] = make_uint4(0, 0, 0, 0);
-            if (p >= 0) {
-                const uint4 * src = reinterpret_cast<const uint4 *>(block_ptr(a.kv, p, w.blk0 + 8 * j + kb, 1, w.h, HD) + q * 64 + u * 32);
-                v[i][0] = __ldg(src);
-                v[i][1] = __ldg(src + 1);
-            }
-        }
-    }
-    __device__ void store_k(uint8_t * dst) const {
-#pragma unroll
-        for (int i = 0; i < NK; i++) {
-            int row, c;
-            key_piece(i * 128 + tid, row, c);
-            const uint32_t x[4] = { k[i].x, k[i].y, k[i].z, k[i].w };
+        for (int i = 0; i < N; i++) {
+            const uint32_t v[4] = { x[i].x, x[i].y, x[i].z, x[i].w };
             uint32_t y[8];
 #pragma unroll
-            for (int m = 0; m < 4; m++) y[2 * m] = e4m3x2_to_h2((uint16_t) x[m]), y[2 * m + 1] = e4m3x2_to_h2((uint16_t) (x[m] >> 16));
-            uint8_t * r = dst + (c >> 2) * Smem<HD>::kHalf + row * 128;
-            const int c0 = (c & 3) * 2;
-            *reinterpret_cast<uint4 *>(r + ((c0 ^ (row & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
-            *reinterpret_cast<uint4 *>(r + (((c0 + 1) ^ (row & 7)) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
+            for (int m = 0; m < 4; m++) y[2 * m] = e4m3x2_to_h2((uint16_t) v[m]), y[2 * m + 1] = e4m3x2_to_h2((uint16_t) (v[m] >> 16));
+            uint8_t * at = tile + dst + i * step * 16 * 128;
+            *reinterpret_cast<uint4 *>(at) = make_uint4(y[0], y[1], y[2], y[3]);
+            // (the second half is the next 16-byte chunk before the swizzle: chunk number ^ 1)
+            *reinterpret_cast<uint4 *>(tile + ((dst + i * step * 16 * 128) ^ 16)) = make_uint4(y[4], y[5], y[6], y[7]);
         }
     }
-    // NaNs of a tile that some row does not see in whole are stored as zero; says whether there were any
+};
+
+template <int HD>
+struct Values {
+    static constexpr int N = HD / 32;  // 32-byte pieces (two patches: 4 elements x 8 positions) for each of 128 threads
+    uint4 x[N][2];
+    int in_block, first, tid;
+
+    __device__ explicit Values(int t) : tid(t) {
+        in_block = ((t >> 3) & 15) * 64 + (t & 1) * 32;
+        first = (t >> 1) & 3;
+    }
+    // piece i: blocks first + 4 (i of the tile's halves), element quads of the low or high half
+    static __device__ constexpr int half_of(int i) { return HD == 64 ? i : i >> 1; }
+    static __device__ constexpr int quads_of(int i) { return HD == 64 ? 0 : (i & 1) * 16; }
+    __device__ void load(const uint8_t * block) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const uint8_t * p = shfl_ptr(block, first + 4 * half_of(i));
+            x[i][0] = x[i][1] = make_uint4(0, 0, 0, 0);
+            if (p) {
+                const uint4 * src = reinterpret_cast<const uint4 *>(p + in_block + quads_of(i) * 64);
+                x[i][0] = __ldg(src);
+                x[i][1] = __ldg(src + 1);
+            }
+        }
+    }
+    // NaNs become zero; says whether there were any
     __device__ bool clear_nan() {
         uint32_t any = 0;
 #pragma unroll
-        for (int i = 0; i < NV; i++)
+        for (int i = 0; i < N; i++)
 #pragma unroll
             for (int m = 0; m < 2; m++) {
-                uint4 & x = v[i][m];
-                const uint4 n = make_uint4(nan_bytes(x.x), nan_bytes(x.y), nan_bytes(x.z), nan_bytes(x.w));
+                uint4 & v = x[i][m];
+                const uint4 n = make_uint4(nan_bytes(v.x), nan_bytes(v.y), nan_bytes(v.z), nan_bytes(v.w));
                 any |= n.x | n.y | n.z | n.w;
-                x = make_uint4(x.x & ~n.x, x.y & ~n.y, x.z & ~n.z, x.w & ~n.w);
+                v = make_uint4(v.x & ~n.x, v.y & ~n.y, v.z & ~n.z, v.w & ~n.w);
             }
         return any != 0;
     }
-    __device__ void store_v(uint8_t * dst) const {
+    __device__ void store(uint8_t * tile) const {
+        const int q = (tid >> 3) & 15, chunk = first * 2 + (tid & 1);
+        uint8_t * row = tile + q * 4 * 128;
+        int at[4];
 #pragma unroll
-        for (int i = 0; i < NV; i++) {
-            int kb, q, u;
-            value_piece(i * 128 + tid, kb, q, u);
-            const uint32_t x[4] = { v[i][0].x, v[i][0].y, v[i][0].z, v[i][0].w }, y[4] = { v[i][1].x, v[i][1].y, v[i][1].z, v[i][1].w };
-            const int chunk = (kb & 3) * 2 + u;
+        for (int m = 0; m < 4; m++) at[m] = m * 128 + ((chunk ^ ((4 * q + m) & 7)) << 4);
 #pragma unroll
-            for (int m = 0; m < 4; m++) {
-                const int d = 4 * q + m;
-                *reinterpret_cast<uint4 *>(dst + (kb >> 2) * (HD * 128) + d * 128 + ((chunk ^ (d & 7)) << 4)) =
-                    make_uint4(e4m3x2_to_h2((uint16_t) x[m]), e4m3x2_to_h2((uint16_t) (x[m] >> 16)),
+        for (int i = 0; i < N; i++) {
+            const uint32_t v[4] = { x[i][0].x, x[i][0].y, x[i][0].z, x[i][0].w }, y[4] = { x[i][1].x, x[i][1].y, x[i][1].z, x[i][1].w };
+#pragma unroll
+            for (int m = 0; m < 4; m++)
+                *reinterpret_cast<uint4 *>(row + half_of(i) * (HD * 128) + quads_of(i) * 512 + at[m]) =
+                    make_uint4(e4m3x2_to_h2((uint16_t) v[m]), e4m3x2_to_h2((uint16_t) (v[m] >> 16)),
                                e4m3x2_to_h2((uint16_t) y[m]), e4m3x2_to_h2((uint16_t) (y[m] >> 16)));
-            }
         }
     }
 };
@@ -284,18 +312,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
         for (int i = 0; i < 2; i++) {
             mbar_init(&sh.k_full[i], kProducers);
             mbar_init(&sh.v_full[i], kProducers);
-            mbar_init(&sh.k_empty[i], 1);
-            mbar_init(&sh.v_empty[i], 1);
-            mbar_init(&sh.s_full[i], 1);
-            mbar_init(&sh.w_full[i], 4);
+            mbar_init(&sh.k_empty[i], tiles);
+            mbar_init(&sh.v_empty[i], tiles);
             mbar_init(&sh.o_full[i], 1);
-            mbar_init(&sh.pv_done[i], 1);
+            for (int b = 0; b < 2; b++) {
+                mbar_init(&sh.s_full[i][b], 1);
+                mbar_init(&sh.w_full[i][b], 4);
+                mbar_init(&sh.pv_done[i][b], 1);
+            }
         }
         for (int i = 0; i < 4; i++) {
             mbar_init(&sh.c_full[i], 1);
             mbar_init(&sh.n_full[i], kProducers);
+            mbar_init(&sh.drain[i], 1);
         }
-        mbar_init(&sh.drain, 1);
         sh.err = 0;
         fence_mbar_init();
     }
@@ -308,7 +338,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
-    const int n = w.n_tiles;
+    const int n = w.n_tiles, steps = max(0, (w.blk_hi - w.blk0 + 3) / 4);
     int * err = &sh.err;
     constexpr int PL = HD + 4;
     const size_t unit = ((size_t) w.b * a.row_tiles + w.tile) * a.kv.n_kv + w.h;
@@ -328,10 +358,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
     };
 
     if (warp < kSoftmax) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         const int i = warp >> 2, r = threadIdx.x & 127, rr = w.row0 + 128 * i + r;
         if (i < tiles) {
             const uint32_t lanes = (uint32_t) (warp & 3) << 21;  // tensor memory lanes 32 (warp % 4) ..
-            const uint32_t ts = tmem + lanes + i * kKeys, tw = tmem + lanes + M::cW + i * M::kWStride, to = tmem + lanes + M::cO + i * HD;
+            const uint32_t ts = tmem + lanes + i * 2 * kStep, to = tmem + lanes + M::cO + i * HD;
             const bool real = rr < w.rows;
             const int pos = w.first + rr / a.group;
             const int hi = !real ? INT_MAX : a.causal ? pos + 1 : w.s.len, lo = real && a.window > 0 ? pos - a.window + 1 : INT_MIN;
@@ -340,91 +371,86 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
             float m = -INFINITY, l = 0.0f;
             uint32_t nan_d[HD / 32] = {};
             bool ok = true;
-            for (int j = 0; j < n; j++) {
-                const int key0 = (w.blk0 + 8 * j) << 4;
-                ok = warp_wait(&sh.c_full[j & 3], (j >> 2) & 1, err) && warp_wait(&sh.s_full[i], j & 1, err);
+            for (int u = 0; u < steps; u++) {
+                const int j = u >> 1, key0 = (w.blk0 << 4) + kStep * u;
+                ok = warp_wait(&sh.c_full[j & 3], (j >> 2) & 1, err) && warp_wait(&sh.s_full[i][u & 1], j & 1, err);
                 if (!ok) break;
                 tc_fence_after();
-                const bool whole = key0 >= warp_lo && key0 + kKeys <= warp_hi;
+                const bool whole = key0 >= warp_lo && key0 + kStep <= warp_hi;
+                const uint32_t at = ts + (u & 1) * kStep;
+                uint32_t x[2][32];
+                ld32(at, x[0]);
+                ld32(at + 32, x[1]);
+                const float4 * scale = sh.scale[j & 3] + 4 * (u & 1);
+                float4 c[4];  // of 16 keys: keys' scale and the row's factor, values' exponent, its inverse
+#pragma unroll
+                for (int g = 0; g < 4; g++) c[g] = scale[g], c[g].x *= coef;
+                tmem_wait_ld();
+                float2 s[4][8];
                 float top = -INFINITY;
-#pragma unroll 1
-                for (int c = 0; c < 4; c++) {
-                    uint32_t x[32];
-                    ld32(ts + 32 * c, x);
-                    tmem_wait_ld();
 #pragma unroll
-                    for (int g = 0; g < 2; g++) {
-                        const float ks = sh.scale[j & 3][2 * c + g][0] * coef, ev = sh.scale[j & 3][2 * c + g][1];
+                for (int g = 0; g < 4; g++) {
 #pragma unroll
-                        for (int t = 0; t < 16; t++) {
-                            float s = fmaf(__uint_as_float(x[16 * g + t]), ks, ev);
-                            if (!whole) {
-                                const int key = key0 + 32 * c + 16 * g + t;
-                                if (key < lo || key >= hi) s = -INFINITY;
-                            }
-                            top = fmaxf(top, s);
-                        }
-                    }
+                    for (int t = 0; t < 8; t++) s[g][t] = fma2(pair(x[g >> 1][16 * (g & 1) + 2 * t], x[g >> 1][16 * (g & 1) + 2 * t + 1]), c[g].x, c[g].y);
+                    if (!whole) mask(s[g], key0 + 16 * g, lo, hi);
+#pragma unroll
+                    for (int t = 0; t < 8; t++) top = fmaxf(fmaxf(top, s[g][t].x), s[g][t].y);
                 }
                 // (the first maximum is taken as it is; -inf while a row has seen no key)
-                const bool grow = top > m + kSlack || (m == -INFINITY && top > m);
+                const bool grow = top > m + kSlack;
                 if (__any_sync(0xffffffffu, grow)) {
                     const float f = grow ? exp2_approx(m - top) : 1.0f;
                     if (grow) m = top;
                     l *= f;
-                    if (j > 0) {
+                    if (u > 0) {
+                        // the last product into these outputs must be in before they are scaled
+                        ok = warp_wait(&sh.pv_done[i][(u - 1) & 1], ((u - 1) >> 1) & 1, err);
+                        if (!ok) break;
+                        tc_fence_after();
 #pragma unroll 1
-                        for (int c = 0; c < HD / 16; c++) {
+                        for (int d = 0; d < HD; d += 16) {
                             float y[16];
-                            tmem_ld16(to + 16 * c, y);
+                            tmem_ld16(to + d, y);
                             tmem_wait_ld();
                             uint32_t z[16];
 #pragma unroll
                             for (int t = 0; t < 16; t++) z[t] = __float_as_uint(y[t] * f);
-                            st16(to + 16 * c, z);
+                            st16(to + d, z);
                         }
                     }
                 }
-                const float ref = m == -INFINITY ? 0.0f : m;
-#pragma unroll 1
-                for (int c = 0; c < 4; c++) {
-                    uint32_t x[32], p[16];
-                    ld32(ts + 32 * c, x);
-                    tmem_wait_ld();
+                const float2 ref = make_float2(m == -INFINITY ? 0.0f : -m, m == -INFINITY ? 0.0f : -m);
 #pragma unroll
-                    for (int g = 0; g < 2; g++) {
-                        const float ks = sh.scale[j & 3][2 * c + g][0] * coef, ev = sh.scale[j & 3][2 * c + g][1] - ref;
-                        const float inv = sh.scale[j & 3][2 * c + g][2];
-                        float sum = 0.0f;
+                for (int g = 0; g < 4; g += 2) {
+                    uint32_t p[16];
 #pragma unroll
-                        for (int t = 0; t < 16; t += 2) {
-                            float s0 = fmaf(__uint_as_float(x[16 * g + t]), ks, ev), s1 = fmaf(__uint_as_float(x[16 * g + t + 1]), ks, ev);
-                            if (!whole) {
-                                const int key = key0 + 32 * c + 16 * g + t;
-                                if (key < lo || key >= hi) s0 = -INFINITY;
-                                if (key + 1 < lo || key + 1 >= hi) s1 = -INFINITY;
-                            }
-                            s0 = exp2_approx(s0), s1 = exp2_approx(s1);
-                            sum += s0 + s1;
-                            p[8 * g + t / 2] = pack_half(s0, s1);
+                    for (int k = 0; k < 2; k++) {
+                        float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+                        for (int t = 0; t < 8; t++) {
+                            const float2 v = add2(s[g + k][t], ref);
+                            const float2 e = make_float2(exp2_approx(v.x), exp2_approx(v.y));
+                            sum = add2(sum, e);
+                            p[8 * k + t] = pack_half(e.x, e.y);
                         }
-                        l = fmaf(sum, inv, l);
+                        l = fmaf(sum.x + sum.y, c[g + k].z, l);
                     }
-                    st16(tw + 16 * c, p);
+                    st16(at + 8 * g, p);
                 }
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.w_full[i]);
-                // NaN values in a tile that some row of the CTA does not see in whole: the producers left them
+                if (lane == 0) mbar_arrive(&sh.w_full[i][u & 1]);
+                // NaN values in a stage that some row of the CTA does not see in whole: the producers left them
                 // out; the rows that see one get it at the end
-                if (key0 < w.full_lo || key0 + kKeys > w.full_hi) {
+                const int stage0 = (w.blk0 + 8 * j) << 4;
+                if (stage0 < w.full_lo || stage0 + kKeys > w.full_hi) {
                     ok = warp_wait(&sh.n_full[j & 3], (j >> 2) & 1, err);
                     if (!ok) break;
                     bool any = false;
                     for (int q = 0; q < kProducers; q++) any |= sh.nan_v[j & 3][q] != 0;
                     if (any && real)
-                        for (int key = max(lo, key0); key < min(hi, key0 + kKeys) && (key >> 4) < w.blk_hi; key++) {
+                        for (int key = max(lo, key0); key < min(hi, key0 + kStep) && (key >> 4) < w.blk_hi; key++) {
                             const int pg = max(page_of(a.kv, w.s.slot, key >> 4), 0);
                             const uint8_t * src = block_ptr(a.kv, pg, key >> 4, 1, w.h, HD) + ((key >> 2) & 3) * 16 + (key & 3);
 #pragma unroll
@@ -470,97 +496,118 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
             }
             tc_fence_before();
         }
-    } else if (warp < kMmaWarp) {
-        Producer<HD> p = { {}, {}, a, w, (int) threadIdx.x - 32 * kSoftmax, lane };
+    } else if (warp < kSoftmax + kProducers) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        Keys<HD> k((int) threadIdx.x - 32 * kSoftmax);
         const int pw = warp - kSoftmax;
-        int pg = p.pages(0), next = p.pages(1);
-        if (n > 0) p.load_k(0, pg), p.load_v(0, pg);
+        auto block = [&](int pg, int j) -> const uint8_t * {
+            return pg < 0 ? nullptr : block_ptr(a.kv, pg, w.blk0 + 8 * j + (lane & 7), 0, w.h, HD);
+        };
+        int pg = tile_page(a, w, 0, lane), next = tile_page(a, w, 1, lane);
+        k.load(block(pg, 0));
         for (int j = 0; j < n; j++) {
-            const int st = j & 1, key0 = (w.blk0 + 8 * j) << 4;
+            const int st = j & 1;
+            float ks = 0.0f, vs = 1.0f;
+            if (pw == 0 && lane < 8 && pg >= 0) {
+                ks = __ldg(scale_ptr(a.kv, pg, w.blk0 + 8 * j + lane, 0, w.h));
+                vs = __ldg(scale_ptr(a.kv, pg, w.blk0 + 8 * j + lane, 1, w.h));
+            }
             if (!warp_wait(&sh.k_empty[st], ((j >> 1) & 1) ^ 1, err)) break;
-            p.store_k(base + M::oK + st * M::kK);
+            k.store(base + M::oK + st * M::kK);
             if (pw == 0 && lane < 8) {
-                const bool there = pg >= 0;
-                const int blk = w.blk0 + 8 * j + lane;
-                const float vs = there ? __ldg(scale_ptr(a.kv, pg, blk, 1, w.h)) : 1.0f;
-                sh.scale[j & 3][lane][0] = there ? __ldg(scale_ptr(a.kv, pg, blk, 0, w.h)) : 0.0f;
-                sh.scale[j & 3][lane][1] = (float) exponent_of(vs);
-                sh.scale[j & 3][lane][2] = 1.0f / vs;
+                sh.scale[j & 3][lane] = make_float4(ks, (float) exponent_of(vs), 1.0f / vs, 0.0f);
             }
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(&sh.k_full[st]);
                 // scale[] and nan_v[] are rings of four: tile j + 4 is stored when the products of tile j + 2
-                // are done, which every softmax warp's weights of tile j + 1 come before
+                // have been issued, which every softmax warp's weights of tile j + 1 come before
                 if (pw == 0) mbar_arrive(&sh.c_full[j & 3]);
             }
-            if (j + 1 < n) p.load_k(j + 1, next);
-            if (!warp_wait(&sh.v_empty[st], ((j >> 1) & 1) ^ 1, err)) break;
+            pg = next;
+            k.load(block(pg, j + 1));
+            next = tile_page(a, w, j + 2, lane);
+        }
+    } else if (warp < kMmaWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        Values<HD> v((int) threadIdx.x - 32 * (kSoftmax + kProducers));
+        const int pw = warp - kSoftmax - kProducers;
+        auto block = [&](int pg, int j) -> const uint8_t * {
+            return pg < 0 ? nullptr : block_ptr(a.kv, pg, w.blk0 + 8 * j + (lane & 7), 1, w.h, HD);
+        };
+        int next = tile_page(a, w, 1, lane);
+        v.load(block(tile_page(a, w, 0, lane), 0));
+        for (int j = 0; j < n; j++) {
+            const int st = j & 1, key0 = (w.blk0 + 8 * j) << 4;
             bool bad = false;
-            if (key0 < w.full_lo || key0 + kKeys > w.full_hi) bad = p.clear_nan();
+            if (key0 < w.full_lo || key0 + kKeys > w.full_hi) bad = v.clear_nan();
             bad = __any_sync(0xffffffffu, bad);
+            if (!warp_wait(&sh.v_empty[st], ((j >> 1) & 1) ^ 1, err)) break;
+            v.store(base + M::oV + st * M::kV);
             if (lane == 0) sh.nan_v[j & 3][pw] = bad;
-            p.store_v(base + M::oV + st * M::kV);
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.v_full[st]), mbar_arrive(&sh.n_full[j & 3]);
-            if (j + 1 < n) p.load_v(j + 1, next);
-            pg = next;
-            next = p.pages(j + 2);
+            v.load(block(next, j + 1));
+            next = tile_page(a, w, j + 2, lane);
         }
-    } else if (lane == 0 && n > 0) {
-        constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t) (kKeys >> 3) << 17) | (8u << 24);
-        constexpr uint32_t idesc_o = (1u << 4) | ((uint32_t) (HD >> 3) << 17) | (8u << 24);
-        const uint32_t q0 = smem_u32(base + M::oQ), k0 = smem_u32(base + M::oK), v0 = smem_u32(base + M::oV);
-        auto scores = [&](int i, int j) {
-#pragma unroll
-            for (int kk = 0; kk < HD / 16; kk++) {
-                const uint32_t at = (kk / 4) * M::kHalf + (kk % 4) * 32;
-                umma_f16(tmem + i * kKeys, sw128_desc(q0 + i * M::kQ + at), sw128_desc(k0 + (j & 1) * M::kK + at), idesc_s, kk > 0);
-            }
-            umma_commit(&sh.s_full[i]);
-        };
-        bool ok = mbar_wait(&sh.k_full[0], 0, err);
-        tc_fence_after();
-        if (ok) {
-            for (int i = 0; i < tiles; i++) scores(i, 0);
-            umma_commit(&sh.k_empty[0]);
-        }
-        for (int j = 0; ok && j < n; j++) {
-            for (int i = 0; ok && i < tiles; i++) {
-                ok = mbar_wait(&sh.w_full[i], j & 1, err);
-                if (ok && i == 0) ok = mbar_wait(&sh.v_full[j & 1], (j >> 1) & 1, err);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    }
+    const int mma = warp - kMmaWarp, mt = mma & 1;
+    if (mma >= 0 && mt < tiles && n > 0) {
+        // (offsets are added to the descriptors' 16-byte address field, which no tile here carries out of)
+        const uint32_t sc = tmem + mt * 2 * kStep;
+        bool ok = true;
+        if (mma < 2) {
+            constexpr uint32_t idesc = (1u << 4) | ((uint32_t) (kStep >> 3) << 17) | (8u << 24);
+            const uint64_t q = sw128_desc(smem_u32(base + M::oQ + mt * M::kQ)), k0 = sw128_desc(smem_u32(base + M::oK));
+            for (int u = 0; u < steps; u++) {
+                const int st = (u >> 1) & 1;
+                // the buffer's last weights have been read (MMAs of different accumulators have no guaranteed
+                // order, so that product is waited for; the other buffer's scores keep the softmax busy)
+                if (u >= 2) ok = warp_wait(&sh.pv_done[mt][u & 1], ((u - 2) >> 1) & 1, err);
+                if (ok && !(u & 1)) ok = warp_wait(&sh.k_full[st], (u >> 2) & 1, err);
                 if (!ok) break;
                 tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t k = k0 + ((st * M::kK + (u & 1) * kStep * 128) >> 4);
 #pragma unroll
-                for (int kk = 0; kk < kKeys / 16; kk++)
-                    umma_f16_tmem_a(tmem + M::cO + i * HD, tmem + M::cW + i * M::kWStride + kk * 8,
-                                    sw128_desc(v0 + (j & 1) * M::kV + (kk / 4) * (HD * 128) + (kk % 4) * 32), idesc_o, j > 0 || kk > 0);
-                if (j + 1 == n) {
-                    umma_commit(&sh.o_full[i]);
-                } else {
-                    if (i == 0) ok = mbar_wait(&sh.k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, err);
-                    if (ok && M::kOver) {
-                        // the next scores overwrite the weights: MMAs of different accumulators have no
-                        // guaranteed order, so the product that reads them is waited for (the other tile's
-                        // softmax covers it)
-                        umma_commit(&sh.pv_done[i]);
-                        ok = mbar_wait(&sh.pv_done[i], j & 1, err);
+                    for (int kk = 0; kk < HD / 16; kk++) {
+                        const uint32_t at = ((kk / 4) * M::kHalf + (kk % 4) * 32) >> 4;
+                        umma_f16(sc + (u & 1) * kStep, q + at, k + at, idesc, kk > 0);
                     }
-                    if (!ok) break;
-                    tc_fence_after();
-                    scores(i, j + 1);
+                    umma_commit(&sh.s_full[mt][u & 1]);
+                    if (u & 1) umma_commit(&sh.k_empty[st]);
                 }
+                __syncwarp();
             }
-            if (!ok) break;
-            umma_commit(&sh.v_empty[j & 1]);
-            if (j + 1 < n) umma_commit(&sh.k_empty[(j + 1) & 1]);
+        } else {
+            constexpr uint32_t idesc = (1u << 4) | ((uint32_t) (HD >> 3) << 17) | (8u << 24);
+            const uint64_t v0 = sw128_desc(smem_u32(base + M::oV));
+            for (int u = 0; u < steps; u++) {
+                const int st = (u >> 1) & 1;
+                if (!(u & 1)) ok = warp_wait(&sh.v_full[st], (u >> 2) & 1, err);
+                if (ok) ok = warp_wait(&sh.w_full[mt][u & 1], (u >> 1) & 1, err);
+                if (!ok) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t v = v0 + ((st * M::kV + (u & 1) * HD * 128) >> 4);
+#pragma unroll
+                    for (int kk = 0; kk < kStep / 16; kk++)
+                        umma_f16_tmem_a(tmem + M::cO + mt * HD, sc + (u & 1) * kStep + kk * 8, v + (kk * 32 >> 4), idesc, u > 0 || kk > 0);
+                    umma_commit(u + 1 == steps ? &sh.o_full[mt] : &sh.pv_done[mt][u & 1]);
+                    if (u & 1) umma_commit(&sh.v_empty[st]);
+                }
+                __syncwarp();
+            }
         }
         if (!ok) {
             // what was issued lands before shared and tensor memory are given up
-            umma_commit(&sh.drain);
-            mbar_drain(&sh.drain, 0, err);
+            if (elect_one()) umma_commit(&sh.drain[mma]);
+            __syncwarp();
+            mbar_drain(&sh.drain[mma], 0, err);
         }
     }
     __syncwarp();
@@ -605,6 +652,11 @@ template <int HD>
 void launch(const AttnArgs & a, cudaStream_t s) {
     const long long grid = (long long) a.kv.n_seq * a.row_tiles * a.chunks * a.kv.n_kv;
     if (grid > INT_MAX) throw std::runtime_error("the batch is too large for one call");
+    // the register split adds up only for the launch it was made for: a build that gives the kernel
+    // another count must not reach the GPU, where it would wait for registers that never come free
+    cudaFuncAttributes at;
+    if (cudaFuncGetAttributes(&at, kv8_attn_tile_kernel<HD>) != cudaSuccess || at.numRegs != kLaunchRegs)
+        throw std::runtime_error("kv8_attn_tile_kernel: built with another register count than its split needs");
     // (set on every call: the attribute belongs to the current device)
     cudaError_t e = cudaFuncSetAttribute(kv8_attn_tile_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) Smem<HD>::kBytes);
     if (e == cudaSuccess) {
