@@ -849,6 +849,7 @@ void kv8_attention(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_k
     a.kv = view(c, b);
     if (q.n_head != out.n_head) fail("q and out must have the same heads");
     check_attention(c, q.n_head, causal, window);
+    if (!std::isfinite(scale * kLog2e)) fail("scale must be finite");
     if (q.type != out.type) fail("q and out must be of one type");
     a.q_vec = check_rows(q, "q", q.n_head, c.head_dim, false, 8, b.n_tok);
     a.out_vec = check_rows(out, "out", q.n_head, c.head_dim, false, 4, b.n_tok);

@@ -3,7 +3,7 @@
 //
 // One CTA takes up to 256 rows of one kv head -- (token, head of the group) pairs, so the group shares
 // the cache's tiles -- as two M = 128 tiles, and walks its keys 128 at a time:
-//   producers (4 + 4 warps)  bytes of 128 keys and values from global memory to registers, one tile ahead;
+//   producers (4 warps)  bytes of 128 keys and values from global memory to registers, one tile ahead;
 //                        converted to f16 into shared memory in the MMAs' swizzled layout (two stages),
 //                        the blocks' scales beside them;
 //   MMA (4 warps)        S_i = Q_i K^T into tensor memory, O_i += W_i V with the weights W_i read from
@@ -31,11 +31,11 @@ namespace {
 using namespace tc;
 
 constexpr int kKeys = 128, kStep = 64;     // keys of a stage in shared memory; of a step of the softmax
-constexpr int kProducers = 4, kSoftmax = 8;  // warps: of keys and of values each; of both tiles' softmax
-constexpr int kMmaWarp = kSoftmax + 2 * kProducers;
+constexpr int kProducers = 4, kSoftmax = 8;  // warps
+constexpr int kMmaWarp = kSoftmax + kProducers;
 constexpr int kTileThreads = 32 * (kMmaWarp + 4);
 // registers a thread: at launch, and after the softmax warps have taken what the others give back
-constexpr int kLaunchRegs = 96, kSoftmaxRegs = 144, kOtherRegs = 64;
+constexpr int kLaunchRegs = 128, kSoftmaxRegs = 152, kOtherRegs = 104;
 static_assert(32 * kSoftmax * kSoftmaxRegs + (kTileThreads - 32 * kSoftmax) * kOtherRegs <= kTileThreads * kLaunchRegs,
               "the warps' registers must fit those of the launch");
 constexpr float kSlack = 8.0f;             // how far (powers of two) weights may exceed 1 before O is rescaled
@@ -59,7 +59,7 @@ struct Shared {
     int err;
     int last;
     int nan_v[4][kProducers];   // a producer warp found NaN values in this tile (only where it looked)
-    float4 scale[4][8];         // per block of 16 keys: scale of the keys, exponent of the values' scale, 2^-it
+    float4 scale[4];            // of a stage: the keys' scale, the values' exponent, 2^-it
     float unit[2][128];         // power of two taken out of each query row
 };
 
@@ -77,10 +77,10 @@ __device__ __forceinline__ void ld32(uint32_t addr, uint32_t (&r)[32]) {
 __device__ __forceinline__ float2 pair(uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); }
 __device__ __forceinline__ float2 fma2(float2 a, float b, float c) { return __ffma2_rn(a, make_float2(b, b), make_float2(c, c)); }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
-// scores of 16 keys from key0: those outside [lo, hi) become -inf
-__device__ __forceinline__ void mask(float2 (&s)[8], int key0, int lo, int hi) {
+// scores of 64 keys from key0: those outside [lo, hi) become -inf
+__device__ __forceinline__ void mask(float2 (&s)[32], int key0, int lo, int hi) {
 #pragma unroll
-    for (int t = 0; t < 8; t++) {
+    for (int t = 0; t < 32; t++) {
         const int key = key0 + 2 * t;
         if (key < lo || key >= hi) s[t].x = -INFINITY;
         if (key + 1 < lo || key + 1 >= hi) s[t].y = -INFINITY;
@@ -168,6 +168,7 @@ __device__ __forceinline__ void load_queries(const AttnArgs & a, const Work & w,
     for (int p = 0; p < LPR; p++) {
         const int r = quarter * 32 + p * RPP + lane / LPR;
         float unit = 1.0f;
+        if (a.scale2 < 0.0f) u[p] = make_uint4(u[p].x ^ 0x80008000u, u[p].y ^ 0x80008000u, u[p].z ^ 0x80008000u, u[p].w ^ 0x80008000u);
         if (a.type == BZB_BF16) {
             // bf16 may lie outside f16: the row is brought to about [1, 2) by a power of two
             const uint32_t v[4] = { u[p].x, u[p].y, u[p].z, u[p].w };
@@ -191,7 +192,7 @@ __device__ __forceinline__ void load_queries(const AttnArgs & a, const Work & w,
 
 // ---- producers: tile after tile, bytes in registers to swizzled f16 ----
 //
-// Four warps bring the keys, four the values. A thread's pieces of a tile lie at the same place of
+// A thread's pieces of a tile lie at the same place of
 // successive blocks, so their addresses differ by the blocks' alone.
 __device__ __forceinline__ const uint8_t * shfl_ptr(const uint8_t * p, int lane) {
     return reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(p), lane));
@@ -201,6 +202,27 @@ __device__ __forceinline__ const uint8_t * shfl_ptr(const uint8_t * p, int lane)
 __device__ __forceinline__ int tile_page(const AttnArgs & a, const Work & w, int j, int lane) {
     const int blk = w.blk0 + 8 * j + (lane & 7);
     return j < w.n_tiles && blk < w.blk_hi ? max(page_of(a.kv, w.s.slot, blk), 0) : -1;
+}
+
+// The blocks' scales are brought to the largest of the stage, 2^E, by multiplying the f16 values with 2^(e - E):
+// exact, but for bits below 2^-24 of that scale. One factor then serves 128 keys in the softmax.
+struct StageScale {
+    int top;         // E
+    uint32_t mine;   // lane & 7's block: 2^(e - E) twice, as f16
+};
+__device__ __forceinline__ StageScale stage_scale(float scale, bool there) {
+    const int e = there ? exponent_of(scale) : -1000;
+    int top = e;
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const int d = e - top;  // f16: 2^d has exponent field d + 15, or is subnormal from -15 to -24
+    const uint32_t h = d >= -14 ? (uint32_t) (d + 15) << 10 : d >= -24 ? 1u << (d + 24) : 0u;
+    return { top, h | h << 16 };
+}
+__device__ __forceinline__ uint32_t scaled(uint16_t e4m3x2, uint32_t f) {
+    const uint32_t h = e4m3x2_to_h2(e4m3x2);
+    const half2 r = __hmul2(*reinterpret_cast<const half2 *>(&h), *reinterpret_cast<const half2 *>(&f));
+    return *reinterpret_cast<const uint32_t *>(&r);
 }
 
 template <int HD>
@@ -226,13 +248,14 @@ struct Keys {
             if (p) x[i] = __ldg(reinterpret_cast<const uint4 *>(p + in_block));
         }
     }
-    __device__ void store(uint8_t * tile) const {
+    __device__ void store(uint8_t * tile, uint32_t factor) const {
 #pragma unroll
         for (int i = 0; i < N; i++) {
+            const uint32_t f = __shfl_sync(0xffffffffu, factor, first + step * i);
             const uint32_t v[4] = { x[i].x, x[i].y, x[i].z, x[i].w };
             uint32_t y[8];
 #pragma unroll
-            for (int m = 0; m < 4; m++) y[2 * m] = e4m3x2_to_h2((uint16_t) v[m]), y[2 * m + 1] = e4m3x2_to_h2((uint16_t) (v[m] >> 16));
+            for (int m = 0; m < 4; m++) y[2 * m] = scaled((uint16_t) v[m], f), y[2 * m + 1] = scaled((uint16_t) (v[m] >> 16), f);
             uint8_t * at = tile + dst + i * step * 16 * 128;
             *reinterpret_cast<uint4 *>(at) = make_uint4(y[0], y[1], y[2], y[3]);
             // (the second half is the next 16-byte chunk before the swizzle: chunk number ^ 1)
@@ -280,7 +303,7 @@ struct Values {
             }
         return any != 0;
     }
-    __device__ void store(uint8_t * tile) const {
+    __device__ void store(uint8_t * tile, uint32_t factor) const {
         const int q = (tid >> 3) & 15, chunk = first * 2 + (tid & 1);
         uint8_t * row = tile + q * 4 * 128;
         int at[4];
@@ -288,12 +311,13 @@ struct Values {
         for (int m = 0; m < 4; m++) at[m] = m * 128 + ((chunk ^ ((4 * q + m) & 7)) << 4);
 #pragma unroll
         for (int i = 0; i < N; i++) {
+            const uint32_t f = __shfl_sync(0xffffffffu, factor, first + 4 * half_of(i));
             const uint32_t v[4] = { x[i][0].x, x[i][0].y, x[i][0].z, x[i][0].w }, y[4] = { x[i][1].x, x[i][1].y, x[i][1].z, x[i][1].w };
 #pragma unroll
             for (int m = 0; m < 4; m++)
                 *reinterpret_cast<uint4 *>(row + half_of(i) * (HD * 128) + quads_of(i) * 512 + at[m]) =
-                    make_uint4(e4m3x2_to_h2((uint16_t) v[m]), e4m3x2_to_h2((uint16_t) (v[m] >> 16)),
-                               e4m3x2_to_h2((uint16_t) y[m]), e4m3x2_to_h2((uint16_t) (y[m] >> 16)));
+                    make_uint4(scaled((uint16_t) v[m], f), scaled((uint16_t) (v[m] >> 16), f), scaled((uint16_t) y[m], f),
+                               scaled((uint16_t) (y[m] >> 16), f));
         }
     }
 };
@@ -367,13 +391,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
             const int pos = w.first + rr / a.group;
             const int hi = !real ? INT_MAX : a.causal ? pos + 1 : w.s.len, lo = real && a.window > 0 ? pos - a.window + 1 : INT_MIN;
             const int warp_hi = __reduce_min_sync(0xffffffffu, hi), warp_lo = __reduce_max_sync(0xffffffffu, lo);
-            const float coef = a.scale2 * sh.unit[i][r];
+            // (a negative scale's sign is in the queries; never zero, which times -inf would be NaN)
+            const float row_coef = fmaxf(fabsf(a.scale2) * sh.unit[i][r], 1e-37f);
             float m = -INFINITY, l = 0.0f;
             uint32_t nan_d[HD / 32] = {};
             bool ok = true;
+            float4 c = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // the stage's keys' scale times the row's factor, values' exponent, 2^-it
             for (int u = 0; u < steps; u++) {
                 const int j = u >> 1, key0 = (w.blk0 << 4) + kStep * u;
-                ok = warp_wait(&sh.c_full[j & 3], (j >> 2) & 1, err) && warp_wait(&sh.s_full[i][u & 1], j & 1, err);
+                if (!(u & 1)) {
+                    ok = warp_wait(&sh.c_full[j & 3], (j >> 2) & 1, err);
+                    if (!ok) break;
+                    c = sh.scale[j & 3];
+                    c.x *= row_coef;
+                }
+                ok = warp_wait(&sh.s_full[i][u & 1], j & 1, err);
                 if (!ok) break;
                 tc_fence_after();
                 const bool whole = key0 >= warp_lo && key0 + kStep <= warp_hi;
@@ -381,21 +413,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
                 uint32_t x[2][32];
                 ld32(at, x[0]);
                 ld32(at + 32, x[1]);
-                const float4 * scale = sh.scale[j & 3] + 4 * (u & 1);
-                float4 c[4];  // of 16 keys: keys' scale and the row's factor, values' exponent, its inverse
-#pragma unroll
-                for (int g = 0; g < 4; g++) c[g] = scale[g], c[g].x *= coef;
                 tmem_wait_ld();
-                float2 s[4][8];
-                float top = -INFINITY;
+                float2 s[32];
 #pragma unroll
-                for (int g = 0; g < 4; g++) {
+                for (int t = 0; t < 32; t++) s[t] = pair(x[t / 16][2 * (t % 16)], x[t / 16][2 * (t % 16) + 1]);
+                if (!whole) mask(s, key0, lo, hi);
+                float tops[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
 #pragma unroll
-                    for (int t = 0; t < 8; t++) s[g][t] = fma2(pair(x[g >> 1][16 * (g & 1) + 2 * t], x[g >> 1][16 * (g & 1) + 2 * t + 1]), c[g].x, c[g].y);
-                    if (!whole) mask(s[g], key0 + 16 * g, lo, hi);
-#pragma unroll
-                    for (int t = 0; t < 8; t++) top = fmaxf(fmaxf(top, s[g][t].x), s[g][t].y);
-                }
+                for (int t = 0; t < 32; t++) tops[t & 3] = fmaxf(fmaxf(tops[t & 3], s[t].x), s[t].y);
+                const float top = fmaf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), c.x, c.y);
                 // (the first maximum is taken as it is; -inf while a row has seen no key)
                 const bool grow = top > m + kSlack;
                 if (__any_sync(0xffffffffu, grow)) {
@@ -419,24 +445,22 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
                         }
                     }
                 }
-                const float2 ref = make_float2(m == -INFINITY ? 0.0f : -m, m == -INFINITY ? 0.0f : -m);
+                const float ref = c.y - (m == -INFINITY ? 0.0f : m);
+                float2 sum[2] = { { 0.0f, 0.0f }, { 0.0f, 0.0f } };
 #pragma unroll
-                for (int g = 0; g < 4; g += 2) {
+                for (int g = 0; g < 2; g++) {
                     uint32_t p[16];
 #pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        float2 sum = make_float2(0.0f, 0.0f);
-#pragma unroll
-                        for (int t = 0; t < 8; t++) {
-                            const float2 v = add2(s[g + k][t], ref);
-                            const float2 e = make_float2(exp2_approx(v.x), exp2_approx(v.y));
-                            sum = add2(sum, e);
-                            p[8 * k + t] = pack_half(e.x, e.y);
-                        }
-                        l = fmaf(sum.x + sum.y, c[g + k].z, l);
+                    for (int t = 0; t < 16; t++) {
+                        const float2 v = fma2(s[16 * g + t], c.x, ref);
+                        const float2 e = make_float2(exp2_approx(v.x), exp2_approx(v.y));
+                        sum[t & 1] = add2(sum[t & 1], e);
+                        p[t] = pack_half(e.x, e.y);
                     }
-                    st16(at + 8 * g, p);
+                    st16(at + 16 * g, p);
                 }
+                sum[0] = add2(sum[0], sum[1]);
+                l = fmaf(sum[0].x + sum[0].y, c.z, l);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -496,27 +520,30 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
             }
             tc_fence_before();
         }
-    } else if (warp < kSoftmax + kProducers) {
+    } else if (warp < kMmaWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-        Keys<HD> k((int) threadIdx.x - 32 * kSoftmax);
-        const int pw = warp - kSoftmax;
-        auto block = [&](int pg, int j) -> const uint8_t * {
-            return pg < 0 ? nullptr : block_ptr(a.kv, pg, w.blk0 + 8 * j + (lane & 7), 0, w.h, HD);
+        const int pw = warp - kSoftmax, tid = (int) threadIdx.x - 32 * kSoftmax;
+        Keys<HD> k(tid);
+        Values<HD> v(tid);
+        auto block = [&](int pg, int j, int plane) -> const uint8_t * {
+            return pg < 0 ? nullptr : block_ptr(a.kv, pg, w.blk0 + 8 * j + (lane & 7), plane, w.h, HD);
         };
         int pg = tile_page(a, w, 0, lane), next = tile_page(a, w, 1, lane);
-        k.load(block(pg, 0));
+        float ks = 0.0f, vs = 0.0f;
+        auto load_scales = [&](int j) {
+            if (pg < 0) return;
+            ks = __ldg(scale_ptr(a.kv, pg, w.blk0 + 8 * j + (lane & 7), 0, w.h));
+            vs = __ldg(scale_ptr(a.kv, pg, w.blk0 + 8 * j + (lane & 7), 1, w.h));
+        };
+        k.load(block(pg, 0, 0));
+        v.load(block(pg, 0, 1));
+        load_scales(0);
         for (int j = 0; j < n; j++) {
-            const int st = j & 1;
-            float ks = 0.0f, vs = 1.0f;
-            if (pw == 0 && lane < 8 && pg >= 0) {
-                ks = __ldg(scale_ptr(a.kv, pg, w.blk0 + 8 * j + lane, 0, w.h));
-                vs = __ldg(scale_ptr(a.kv, pg, w.blk0 + 8 * j + lane, 1, w.h));
-            }
+            const int st = j & 1, key0 = (w.blk0 + 8 * j) << 4;
+            const StageScale sk = stage_scale(ks, pg >= 0), sv = stage_scale(vs, pg >= 0);
             if (!warp_wait(&sh.k_empty[st], ((j >> 1) & 1) ^ 1, err)) break;
-            k.store(base + M::oK + st * M::kK);
-            if (pw == 0 && lane < 8) {
-                sh.scale[j & 3][lane] = make_float4(ks, (float) exponent_of(vs), 1.0f / vs, 0.0f);
-            }
+            k.store(base + M::oK + st * M::kK, sk.mine);
+            if (pw == 0 && lane == 0) sh.scale[j & 3] = make_float4(pow2f(sk.top), (float) sv.top, pow2f(-sv.top), 0.0f);
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) {
@@ -526,31 +553,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
                 if (pw == 0) mbar_arrive(&sh.c_full[j & 3]);
             }
             pg = next;
-            k.load(block(pg, j + 1));
             next = tile_page(a, w, j + 2, lane);
-        }
-    } else if (warp < kMmaWarp) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-        Values<HD> v((int) threadIdx.x - 32 * (kSoftmax + kProducers));
-        const int pw = warp - kSoftmax - kProducers;
-        auto block = [&](int pg, int j) -> const uint8_t * {
-            return pg < 0 ? nullptr : block_ptr(a.kv, pg, w.blk0 + 8 * j + (lane & 7), 1, w.h, HD);
-        };
-        int next = tile_page(a, w, 1, lane);
-        v.load(block(tile_page(a, w, 0, lane), 0));
-        for (int j = 0; j < n; j++) {
-            const int st = j & 1, key0 = (w.blk0 + 8 * j) << 4;
+            k.load(block(pg, j + 1, 0));
+            load_scales(j + 1);
             bool bad = false;
             if (key0 < w.full_lo || key0 + kKeys > w.full_hi) bad = v.clear_nan();
             bad = __any_sync(0xffffffffu, bad);
             if (!warp_wait(&sh.v_empty[st], ((j >> 1) & 1) ^ 1, err)) break;
-            v.store(base + M::oV + st * M::kV);
+            v.store(base + M::oV + st * M::kV, sv.mine);
             if (lane == 0) sh.nan_v[j & 3][pw] = bad;
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.v_full[st]), mbar_arrive(&sh.n_full[j & 3]);
-            v.load(block(next, j + 1));
-            next = tile_page(a, w, j + 2, lane);
+            v.load(block(pg, j + 1, 1));
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
@@ -568,6 +583,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
                 // the buffer's last weights have been read (MMAs of different accumulators have no guaranteed
                 // order, so that product is waited for; the other buffer's scores keep the softmax busy)
                 if (u >= 2) ok = warp_wait(&sh.pv_done[mt][u & 1], ((u - 2) >> 1) & 1, err);
+                // the second tile starts when the first has done its first step: the two softmaxes then take the
+                // exponential units in turn instead of both at once and both not at all
+                else if (u == 0 && mt == 1) ok = warp_wait(&sh.w_full[0][0], 0, err);
                 if (ok && !(u & 1)) ok = warp_wait(&sh.k_full[st], (u >> 2) & 1, err);
                 if (!ok) break;
                 tc_fence_after();
