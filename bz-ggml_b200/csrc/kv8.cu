@@ -14,240 +14,255 @@ namespace {
 
 using namespace kv8;
 
-// ---- append and read: one warp per (sequence, block of 16 positions, head of q, k or v) ----
+// ---- append and read ----
 //
-// A lane holds, of each of its rows, the four elements from 4c and the four from hd/2 + 4c, c its
-// column of hd/8: the two members of four rotated pairs, so the rotation needs no exchange and
-// each (cos, sin) is read by one lane. Its rows are consecutive positions (4 of 16 for head_dim 64, 8 of 16 for 128), so that of
-// the values it holds whole 4 x 4 patches and stores them as 16 bytes. All rows' loads are issued
-// before the first is used. The maximum of a block is one warp reduction, and no other warp
-// touches the block: no atomics, and the same bytes whatever the launch's shape.
+// A CTA takes one block of 16 positions of a sequence and a few heads of q, k or v: a warp holds 16 rows of
+// a head of 64, or 8 of one of 128 (two warps share a block, and its maximum through shared memory). A lane
+// holds, of each of four consecutive rows, the four elements from 4c and the four from hd/2 + 4c, c its
+// column of hd/8: the two members of four rotated pairs, so the rotation needs no exchange and each
+// (cos, sin) is read by one lane, and of the values whole 4 x 4 patches, stored as 16 bytes. All rows' loads are
+// issued before the first is used; what an append needs of the page (its scale, earlier bytes) is
+// on the way while the norm and the rotation run. No other CTA touches the block: no atomics, and the
+// same bytes whatever the launch's shape.
+constexpr int kRowWarps = 4;
+template <int HD>
+struct RowMap {
+    static constexpr int LPR = HD / 8;              // lanes of a row
+    static constexpr int WPB = HD / 64;             // warps of a block
+    static constexpr int HEADS = kRowWarps / WPB;   // heads of a CTA
+};
+
 struct AppendArgs {
     Kv kv;
     Rows q, k, v, q_out;
     const float * q_norm, * k_norm;
     const float2 * rope;
     float eps;
-    int n_head, n_blk, q_out_type, rope_len;
-    bool q_out_vec;
+    int n_head, n_blk, units, q_out_type;           // units: CTAs of a block of positions
+    bool q_out_vec, norm_vec;
 };
 
-constexpr int kRowWarps = 4;
-
 template <int HD, int TYPE, bool VEC>
-__global__ void __launch_bounds__(32 * kRowWarps) kv8_append_kernel(const AppendArgs a) {
-    constexpr int LPR = HD / 8, RPL = HD / 16;  // lanes per row, rows per lane
+__global__ void __launch_bounds__(32 * kRowWarps, 6) kv8_append_kernel(const AppendArgs a) {
+    using R = RowMap<HD>;
+    __shared__ float tops[kRowWarps];
     const Kv & kv = a.kv;
-    const int tasks = a.n_head + 2 * kv.n_kv;
-    const int lane = threadIdx.x & 31, c = lane % LPR, r0 = lane / LPR * RPL;
-    const long long task = (long long) blockIdx.x * kRowWarps + (threadIdx.x >> 5);
-    const int unit = (int) (task % tasks);
-    const long long sb = task / tasks;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane % R::LPR;
+    const int r0 = warp % R::WPB * (16 / R::WPB) + lane / R::LPR * 4;  // the lane's first row of the block
+    const int unit = (int) (blockIdx.x % a.units);
+    const unsigned sb = blockIdx.x / a.units;
     const int b = (int) (sb / a.n_blk);
-    if (b >= kv.n_seq) return;
     const Seq s = load_seq(kv, b);
     if (s.slot < 0) return;
     const int first = s.len - s.n;  // position of the sequence's first row (negative: padding rows)
     const int blk = (max(first, 0) >> 4) + (int) (sb % a.n_blk), p0 = blk << 4;
-    if (p0 >= s.len || s.n == 0) return;
-    const int kind = unit < a.n_head ? 0 : unit < a.n_head + kv.n_kv ? 1 : 2;
-    const int head = kind == 0 ? unit : kind == 1 ? unit - a.n_head : unit - a.n_head - kv.n_kv;
+    if (p0 >= s.len || s.n == 0) return;  // (the whole CTA, as above)
+    const int any = unit * R::HEADS + warp / R::WPB;
+    const int kind = any < a.n_head ? 0 : any < a.n_head + kv.n_kv ? 1 : any < a.n_head + 2 * kv.n_kv ? 2 : 3;
+    const int head = kind == 0 ? any : kind == 1 ? any - a.n_head : any - a.n_head - kv.n_kv;
     const Rows src = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
+    const int live_lo = kind < 3 ? max(first - p0, 0) : 16, live_hi = min(16, s.len - p0);  // the block's new rows
 
-    float4 lo[RPL], hi[RPL];
+    float4 lo[4], hi[4];
 #pragma unroll
-    for (int i = 0; i < RPL; i++) {
-        const int pos = p0 + r0 + i;
+    for (int i = 0; i < 4; i++) {
         lo[i] = hi[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (pos >= first && pos < s.len) {
-            const long long at = (long long) (s.row0 + pos - first) * src.row + head * src.head + 4 * c;
+        if (r0 + i >= live_lo && r0 + i < live_hi) {
+            const long long at = (long long) (s.row0 + p0 + r0 + i - first) * src.row + head * src.head + 4 * c;
             lo[i] = load4<TYPE, VEC>(src.p, at);
             hi[i] = load4<TYPE, VEC>(src.p, at + HD / 2);
         }
     }
+    const bool cached = kind == 1 || kind == 2, older = cached && p0 < first;  // older: the block holds earlier positions
+    const int pg = cached ? page_of(kv, s.slot, blk) : -1;
+    uint8_t * dst = pg < 0 ? nullptr : block_ptr(kv, pg, blk, kind - 1, head, HD);
+    float * sp = pg < 0 ? nullptr : scale_ptr(kv, pg, blk, kind - 1, head);
+    float was = 1.0f;
+    uint32_t old[8];  // keys: a row's words c and c + hd/8, row after row; values: the patch of quad c, then of c + hd/8
+#pragma unroll
+    for (int i = 0; i < 8; i++) old[i] = 0;
+    if (older && pg >= 0) {
+        was = *sp;
+        if (p0 + r0 < first) {
+            if (kind == 1) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t * row = reinterpret_cast<const uint32_t *>(dst + (r0 + i) * HD);
+                    old[2 * i] = row[c];
+                    old[2 * i + 1] = row[c + HD / 8];
+                }
+            } else {
+                const uint4 * pl = reinterpret_cast<const uint4 *>(dst + c * 64 + r0 * 4), x = pl[0], y = pl[HD / 8 * 4];
+                old[0] = x.x, old[1] = x.y, old[2] = x.z, old[3] = x.w, old[4] = y.x, old[5] = y.y, old[6] = y.z, old[7] = y.w;
+            }
+        }
+    }
     const float * w = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
     if (w) {
-        // (the weights' pointers are only 4-byte aligned)
-        const float4 wl = load4<BZB_F32, false>(w, 4 * c), wh = load4<BZB_F32, false>(w, HD / 2 + 4 * c);
+        const float4 wl = a.norm_vec ? load4<BZB_F32, true>(w, 4 * c) : load4<BZB_F32, false>(w, 4 * c);
+        const float4 wh = a.norm_vec ? load4<BZB_F32, true>(w, HD / 2 + 4 * c) : load4<BZB_F32, false>(w, HD / 2 + 4 * c);
 #pragma unroll
-        for (int i = 0; i < RPL; i++) {
+        for (int i = 0; i < 4; i++) {
             float4 & x = lo[i], & y = hi[i];
             float ss = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w + y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w;
 #pragma unroll
-            for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            const float r = 1.0f / sqrtf(ss * (1.0f / HD) + a.eps);
+            for (int o = R::LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            const float r = rsqrtf(ss * (1.0f / HD) + a.eps);
             x = make_float4(x.x * r * wl.x, x.y * r * wl.y, x.z * r * wl.z, x.w * r * wl.w);
             y = make_float4(y.x * r * wh.x, y.y * r * wh.y, y.z * r * wh.z, y.w * r * wh.w);
         }
     }
     if (kind < 2 && a.rope) {
 #pragma unroll
-        for (int i = 0; i < RPL; i++) {
-            const int pos = p0 + r0 + i;
-            if (pos < first || pos >= s.len) continue;
-            const float2 * t = a.rope + (size_t) pos * (HD / 2) + 4 * c;
-            const float2 t0 = __ldg(t), t1 = __ldg(t + 1), t2 = __ldg(t + 2), t3 = __ldg(t + 3);
+        for (int i = 0; i < 4; i++) {
+            if (r0 + i < live_lo || r0 + i >= live_hi) continue;
+            const float4 * t = reinterpret_cast<const float4 *>(a.rope + (size_t) (p0 + r0 + i) * (HD / 2) + 4 * c);
+            const float4 t0 = __ldg(t), t1 = __ldg(t + 1);  // (cos, sin) of pairs 4c, 4c + 1 and of 4c + 2, 4c + 3
             const float4 x = lo[i], y = hi[i];
-            lo[i] = make_float4(x.x * t0.x - y.x * t0.y, x.y * t1.x - y.y * t1.y, x.z * t2.x - y.z * t2.y, x.w * t3.x - y.w * t3.y);
-            hi[i] = make_float4(x.x * t0.y + y.x * t0.x, x.y * t1.y + y.y * t1.x, x.z * t2.y + y.z * t2.x, x.w * t3.y + y.w * t3.x);
+            lo[i] = make_float4(x.x * t0.x - y.x * t0.y, x.y * t0.z - y.y * t0.w, x.z * t1.x - y.z * t1.y, x.w * t1.z - y.w * t1.w);
+            hi[i] = make_float4(x.x * t0.y + y.x * t0.x, x.y * t0.w + y.y * t0.z, x.z * t1.y + y.z * t1.x, x.w * t1.w + y.w * t1.z);
         }
     }
     if (kind == 0) {
 #pragma unroll
-        for (int i = 0; i < RPL; i++) {
-            const int pos = p0 + r0 + i;
-            if (pos < first || pos >= s.len) continue;
-            const long long at = (long long) (s.row0 + pos - first) * a.q_out.row + head * a.q_out.head + 4 * c;
+        for (int i = 0; i < 4; i++) {
+            if (r0 + i < live_lo || r0 + i >= live_hi) continue;
+            const long long at = (long long) (s.row0 + p0 + r0 + i - first) * a.q_out.row + head * a.q_out.head + 4 * c;
             store4(a.q_out_type, a.q_out_vec, a.q_out.p, at, lo[i]);
             store4(a.q_out_type, a.q_out_vec, a.q_out.p, at + HD / 2, hi[i]);
         }
-        return;
     }
 
-    const int pg = page_of(kv, s.slot, blk);
-    if (pg < 0) return;
-    uint8_t * dst = block_ptr(kv, pg, blk, kind - 1, head, HD);
-    float * sp = scale_ptr(kv, pg, blk, kind - 1, head);
-    const bool older = p0 < first;  // the block holds earlier positions of this sequence
     // the block's largest finite magnitude; what is not finite becomes NaN
     float top = 0.0f;
-    auto finite = [&](float & x) {
-        const float m = fabsf(x);
-        if (m < INFINITY) top = fmaxf(top, m);
-        else x = __int_as_float(0x7fffffff);
-    };
+    if (cached) {
+        auto finite = [&](float & x) {
+            const float m = fabsf(x);
+            if (m < INFINITY) top = fmaxf(top, m);
+            else x = __int_as_float(0x7fffffff);
+        };
 #pragma unroll
-    for (int i = 0; i < RPL; i++) {
-        finite(lo[i].x), finite(lo[i].y), finite(lo[i].z), finite(lo[i].w);
-        finite(hi[i].x), finite(hi[i].y), finite(hi[i].z), finite(hi[i].w);
+        for (int i = 0; i < 4; i++) {
+            finite(lo[i].x), finite(lo[i].y), finite(lo[i].z), finite(lo[i].w);
+            finite(hi[i].x), finite(hi[i].y), finite(hi[i].z), finite(hi[i].w);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (R::WPB > 1) {
+        if (lane == 0) tops[warp] = top;
+        __syncthreads();  // (also: both warps of a block have read its old scale before one writes the new)
+        top = fmaxf(top, tops[warp ^ 1]);
+    } else {
+        __syncwarp();
+    }
+    if (pg < 0) return;
     int e = block_exponent(top);
     float keep = 1.0f;  // factor of the earlier values' bytes
     if (older) {
-        const int e_old = min(kExpMax, max(kExpMin, exponent_of(*sp)));
+        const int e_old = min(kExpMax, max(kExpMin, exponent_of(was)));
         e = max(e, e_old);
         keep = pow2f(e_old - e);
     }
     const float inv = pow2f(-e);
-    uint32_t wl[RPL], wh[RPL];
+    auto kept = [&](uint32_t w) {
+        const float4 f = e4m3x4_to_f4(w);
+        return to_e4m3x4(f.x * keep, f.y * keep, f.z * keep, f.w * keep);
+    };
     if (kind == 1) {
 #pragma unroll
-        for (int i = 0; i < RPL; i++) {
+        for (int i = 0; i < 4; i++) {
             uint32_t * row = reinterpret_cast<uint32_t *>(dst + (r0 + i) * HD);
-            wl[i] = to_e4m3x4(lo[i].x * inv, lo[i].y * inv, lo[i].z * inv, lo[i].w * inv);
-            wh[i] = to_e4m3x4(hi[i].x * inv, hi[i].y * inv, hi[i].z * inv, hi[i].w * inv);
-            if (older && p0 + r0 + i < first) {
-                const float4 x = e4m3x4_to_f4(row[c]), y = e4m3x4_to_f4(row[c + HD / 8]);
-                wl[i] = to_e4m3x4(x.x * keep, x.y * keep, x.z * keep, x.w * keep);
-                wh[i] = to_e4m3x4(y.x * keep, y.y * keep, y.z * keep, y.w * keep);
-            }
-            row[c] = wl[i];
-            row[c + HD / 8] = wh[i];
+            uint32_t wl = to_e4m3x4(lo[i].x * inv, lo[i].y * inv, lo[i].z * inv, lo[i].w * inv);
+            uint32_t wh = to_e4m3x4(hi[i].x * inv, hi[i].y * inv, hi[i].z * inv, hi[i].w * inv);
+            if (r0 + i < live_lo) wl = kept(old[2 * i]), wh = kept(old[2 * i + 1]);
+            row[c] = wl;
+            row[c + HD / 8] = wh;
         }
     } else {
-#pragma unroll
-        for (int g = 0; g < RPL; g += 4) {
-            // patch (element quad c or c + hd/8, position group): word j holds element j of the four positions
-            uint4 * pl = reinterpret_cast<uint4 *>(dst + c * 64 + (r0 + g) * 4), * ph = pl + HD / 8 * 4;
-            uint4 ol = make_uint4(0, 0, 0, 0), oh = ol;
-            if (older && p0 + r0 + g < first) ol = *pl, oh = *ph;
-            auto patch = [&](const float4 (&x)[RPL], uint4 old) {
-                const int kept = older ? min(4, max(0, first - (p0 + r0 + g))) : 0;
-                auto word = [&](float v0, float v1, float v2, float v3, uint32_t was) {
-                    uint32_t n = to_e4m3x4(v0 * inv, v1 * inv, v2 * inv, v3 * inv);
-                    if (kept > 0) {
-                        const float4 f = e4m3x4_to_f4(was);
-                        const uint32_t o = to_e4m3x4(f.x * keep, f.y * keep, f.z * keep, f.w * keep);
-                        const uint32_t m = kept == 4 ? 0xffffffffu : (1u << (8 * kept)) - 1;
-                        n = (o & m) | (n & ~m);
-                    }
-                    return n;
-                };
-                return make_uint4(word(x[g].x, x[g + 1].x, x[g + 2].x, x[g + 3].x, old.x),
-                                  word(x[g].y, x[g + 1].y, x[g + 2].y, x[g + 3].y, old.y),
-                                  word(x[g].z, x[g + 1].z, x[g + 2].z, x[g + 3].z, old.z),
-                                  word(x[g].w, x[g + 1].w, x[g + 2].w, x[g + 3].w, old.w));
-            };
-            *pl = patch(lo, ol);
-            *ph = patch(hi, oh);
-        }
+        // patch (quad c or c + hd/8, the lane's four rows): word j holds element j of the four positions
+        const int n_old = min(4, max(0, live_lo - r0));
+        const uint32_t m = n_old == 4 ? 0xffffffffu : (1u << (8 * n_old)) - 1;
+        auto word = [&](float v0, float v1, float v2, float v3, uint32_t o) {
+            const uint32_t n = to_e4m3x4(v0 * inv, v1 * inv, v2 * inv, v3 * inv);
+            return m ? (kept(o) & m) | (n & ~m) : n;
+        };
+        uint4 * pl = reinterpret_cast<uint4 *>(dst + c * 64 + r0 * 4);
+        pl[0] = make_uint4(word(lo[0].x, lo[1].x, lo[2].x, lo[3].x, old[0]), word(lo[0].y, lo[1].y, lo[2].y, lo[3].y, old[1]),
+                           word(lo[0].z, lo[1].z, lo[2].z, lo[3].z, old[2]), word(lo[0].w, lo[1].w, lo[2].w, lo[3].w, old[3]));
+        pl[HD / 8 * 4] = make_uint4(word(hi[0].x, hi[1].x, hi[2].x, hi[3].x, old[4]), word(hi[0].y, hi[1].y, hi[2].y, hi[3].y, old[5]),
+                                    word(hi[0].z, hi[1].z, hi[2].z, hi[3].z, old[6]), word(hi[0].w, hi[1].w, hi[2].w, hi[3].w, old[7]));
     }
-    // (a block's scale is read above by every lane of the one warp that owns it)
-    __syncwarp();
-    if (lane == 0) *sp = pow2f(e);
+    if (lane == 0 && warp % R::WPB == 0) *sp = pow2f(e);
 }
 
 struct ReadArgs {
     Kv kv;
     Rows k, v;
-    int n_blk, type;
+    int n_blk, units;
     bool vec;
 };
 
-template <int HD>
+template <int HD, int TYPE>
 __global__ void __launch_bounds__(32 * kRowWarps) kv8_read_kernel(const ReadArgs a) {
-    constexpr int LPR = HD / 8, RPL = HD / 16;
+    using R = RowMap<HD>;
     const Kv & kv = a.kv;
-    const int lane = threadIdx.x & 31, c = lane % LPR, r0 = lane / LPR * RPL;
-    const long long task = (long long) blockIdx.x * kRowWarps + (threadIdx.x >> 5);
-    const int unit = (int) (task % (2 * kv.n_kv));
-    const long long sb = task / (2 * kv.n_kv);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane % R::LPR;
+    const int r0 = warp % R::WPB * (16 / R::WPB) + lane / R::LPR * 4;
+    const int unit = (int) (blockIdx.x % a.units);
+    const unsigned sb = blockIdx.x / a.units;
     const int b = (int) (sb / a.n_blk);
-    if (b >= kv.n_seq) return;
     const Seq s = load_seq(kv, b);
     if (s.slot < 0 || s.n == 0) return;
     // blocks count from the first row's position; `first` may be negative (padding rows, read as zeros)
     const int first = s.len - s.n, blk = (first >> 4) + (int) (sb % a.n_blk), p0 = blk << 4;
-    if (p0 >= s.len) return;
-    const int plane = unit >= kv.n_kv, head = unit - plane * kv.n_kv;
-    float4 lo[RPL], hi[RPL];
+    const int any = unit * R::HEADS + warp / R::WPB;
+    if (p0 >= s.len || any >= 2 * kv.n_kv) return;
+    const int plane = any >= kv.n_kv, head = any - plane * kv.n_kv;
+    float4 lo[4], hi[4];
 #pragma unroll
-    for (int i = 0; i < RPL; i++) lo[i] = hi[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i = 0; i < 4; i++) lo[i] = hi[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (blk >= 0) {
         const int pg = max(page_of(kv, s.slot, blk), 0);
         const uint8_t * src = block_ptr(kv, pg, blk, plane, head, HD);
-        const float scale = *scale_ptr(kv, pg, blk, plane, head);
+        const float scale = __ldg(scale_ptr(kv, pg, blk, plane, head));
+        uint32_t w[8];
         if (plane == 0) {
-            uint32_t wl[RPL], wh[RPL];
 #pragma unroll
-            for (int i = 0; i < RPL; i++) {
+            for (int i = 0; i < 4; i++) {
                 const uint32_t * row = reinterpret_cast<const uint32_t *>(src + (r0 + i) * HD);
-                wl[i] = row[c];
-                wh[i] = row[c + HD / 8];
+                w[2 * i] = __ldg(row + c);
+                w[2 * i + 1] = __ldg(row + c + HD / 8);
             }
 #pragma unroll
-            for (int i = 0; i < RPL; i++) lo[i] = e4m3x4_to_f4(wl[i]), hi[i] = e4m3x4_to_f4(wh[i]);
+            for (int i = 0; i < 4; i++) lo[i] = e4m3x4_to_f4(w[2 * i]), hi[i] = e4m3x4_to_f4(w[2 * i + 1]);
         } else {
-#pragma unroll
-            for (int g = 0; g < RPL; g += 4) {
-                const uint4 * pl = reinterpret_cast<const uint4 *>(src + c * 64 + (r0 + g) * 4);
-                auto patch = [&](float4 (&x)[RPL], uint4 w) {
-                    const float4 e0 = e4m3x4_to_f4(w.x), e1 = e4m3x4_to_f4(w.y), e2 = e4m3x4_to_f4(w.z), e3 = e4m3x4_to_f4(w.w);
-                    x[g] = make_float4(e0.x, e1.x, e2.x, e3.x);
-                    x[g + 1] = make_float4(e0.y, e1.y, e2.y, e3.y);
-                    x[g + 2] = make_float4(e0.z, e1.z, e2.z, e3.z);
-                    x[g + 3] = make_float4(e0.w, e1.w, e2.w, e3.w);
-                };
-                patch(lo, pl[0]);
-                patch(hi, pl[HD / 8 * 4]);
-            }
+            const uint4 * pl = reinterpret_cast<const uint4 *>(src + c * 64 + r0 * 4);
+            const uint4 x = __ldg(pl), y = __ldg(pl + HD / 8 * 4);
+            auto patch = [&](float4 (&o)[4], uint4 w) {
+                const float4 e0 = e4m3x4_to_f4(w.x), e1 = e4m3x4_to_f4(w.y), e2 = e4m3x4_to_f4(w.z), e3 = e4m3x4_to_f4(w.w);
+                o[0] = make_float4(e0.x, e1.x, e2.x, e3.x);
+                o[1] = make_float4(e0.y, e1.y, e2.y, e3.y);
+                o[2] = make_float4(e0.z, e1.z, e2.z, e3.z);
+                o[3] = make_float4(e0.w, e1.w, e2.w, e3.w);
+            };
+            patch(lo, x);
+            patch(hi, y);
         }
 #pragma unroll
-        for (int i = 0; i < RPL; i++) {
+        for (int i = 0; i < 4; i++) {
             lo[i] = make_float4(lo[i].x * scale, lo[i].y * scale, lo[i].z * scale, lo[i].w * scale);
             hi[i] = make_float4(hi[i].x * scale, hi[i].y * scale, hi[i].z * scale, hi[i].w * scale);
         }
     }
     const Rows dst = plane ? a.v : a.k;
 #pragma unroll
-    for (int i = 0; i < RPL; i++) {
+    for (int i = 0; i < 4; i++) {
         const int pos = p0 + r0 + i;
         if (pos < first || pos >= s.len) continue;
         const long long at = (long long) (s.row0 + pos - first) * dst.row + head * dst.head + 4 * c;
-        store4(a.type, a.vec, dst.p, at, lo[i]);
-        store4(a.type, a.vec, dst.p, at + HD / 2, hi[i]);
+        store4(TYPE, a.vec, dst.p, at, lo[i]);
+        store4(TYPE, a.vec, dst.p, at + HD / 2, hi[i]);
     }
 }
 
@@ -702,10 +717,19 @@ unsigned grid_of(long long tasks, int per_cta) {
 }
 
 template <int HD, int TYPE>
-void run_append(const AppendArgs & a, bool vec, cudaStream_t s) {
-    const unsigned grid = grid_of((long long) a.kv.n_seq * a.n_blk * (a.n_head + 2 * a.kv.n_kv), kRowWarps);
+void run_append(AppendArgs a, bool vec, cudaStream_t s) {
+    a.units = (a.n_head + 2 * a.kv.n_kv + RowMap<HD>::HEADS - 1) / RowMap<HD>::HEADS;
+    const unsigned grid = grid_of((long long) a.kv.n_seq * a.n_blk * a.units, 1);
     if (vec) kv8_append_kernel<HD, TYPE, true><<<grid, 32 * kRowWarps, 0, s>>>(a);
     else kv8_append_kernel<HD, TYPE, false><<<grid, 32 * kRowWarps, 0, s>>>(a);
+    check_cuda(cudaGetLastError(), "launch");
+}
+
+template <int HD, int TYPE>
+void run_read(ReadArgs a, cudaStream_t s) {
+    a.units = (2 * a.kv.n_kv + RowMap<HD>::HEADS - 1) / RowMap<HD>::HEADS;
+    const unsigned grid = grid_of((long long) a.kv.n_seq * a.n_blk * a.units, 1);
+    kv8_read_kernel<HD, TYPE><<<grid, 32 * kRowWarps, 0, s>>>(a);
     check_cuda(cudaGetLastError(), "launch");
 }
 
@@ -790,7 +814,8 @@ void kv8_append(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_kv8_
         a.q_out_type = q_out->type;
     }
     if (!(eps >= 0.0f)) fail("eps must not be negative");
-    if ((uintptr_t) q_norm % 4 || (uintptr_t) k_norm % 4 || (uintptr_t) rope % 8) fail("q_norm, k_norm or rope is misaligned");
+    if ((uintptr_t) q_norm % 4 || (uintptr_t) k_norm % 4) fail("q_norm and k_norm must be 4-byte aligned");
+    if ((uintptr_t) rope % 16) fail("rope must be 16-byte aligned");
     if (rope && rope_len < b.max_len) fail("rope has fewer positions than max_len");
     if (b.n_seq == 0 || b.n_tok == 0 || b.max_new == 0 || b.max_len == 0) return;
     a.k = Rows{ k.data, k.row_stride, k.head_stride };
@@ -798,7 +823,7 @@ void kv8_append(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_kv8_
     a.q_norm = q_norm;
     a.k_norm = k_norm;
     a.rope = reinterpret_cast<const float2 *>(rope);
-    a.rope_len = rope_len;
+    a.norm_vec = (uintptr_t) q_norm % 16 == 0 && (uintptr_t) k_norm % 16 == 0;
     a.eps = eps;
     a.n_blk = (b.max_new + 30) / 16;  // blocks that max_new positions can touch
     if (c.head_dim == 64) {
@@ -824,12 +849,16 @@ void kv8_read(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_kv8_ro
     if (b.n_seq == 0 || b.n_tok == 0 || b.max_new == 0) return;
     a.k = Rows{ k_out.data, k_out.row_stride, k_out.head_stride };
     a.v = Rows{ v_out.data, v_out.row_stride, v_out.head_stride };
-    a.type = k_out.type;
     a.n_blk = (b.max_new + 30) / 16;
-    const unsigned grid = grid_of((long long) b.n_seq * a.n_blk * 2 * c.n_kv, kRowWarps);
-    if (c.head_dim == 64) kv8_read_kernel<64><<<grid, 32 * kRowWarps, 0, s>>>(a);
-    else kv8_read_kernel<128><<<grid, 32 * kRowWarps, 0, s>>>(a);
-    check_cuda(cudaGetLastError(), "launch");
+    if (c.head_dim == 64) {
+        if (k_out.type == BZB_F32) run_read<64, BZB_F32>(a, s);
+        else if (k_out.type == BZB_F16) run_read<64, BZB_F16>(a, s);
+        else run_read<64, BZB_BF16>(a, s);
+    } else {
+        if (k_out.type == BZB_F32) run_read<128, BZB_F32>(a, s);
+        else if (k_out.type == BZB_F16) run_read<128, BZB_F16>(a, s);
+        else run_read<128, BZB_BF16>(a, s);
+    }
 }
 
 long long kv8_attention_workspace(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int causal, int window) {

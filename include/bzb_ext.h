@@ -178,7 +178,7 @@ typedef struct bzb_kv8_rows {
 /* Norms and rotates every new row's queries and keys and appends its keys and values, in one launch:
  *   q_out = rot(x w_q / sqrt(mean(x^2) + eps)), the same with w_k for the keys, values unchanged;
  *   rot turns the pairs (i, i + head_dim / 2) by the row's position: rope [rope_len][head_dim / 2][2]
- *   holds (cos, sin).
+ *   (16-byte aligned) holds (cos, sin).
  * q_norm / k_norm [head_dim] or NULL (no norm), rope or NULL (no rotation); q and q_out both NULL
  * when only keys and values are wanted. q, k, v of one type (f32, f16 or bf16), q_out f16 or bf16; q_out
  * may not overlap q. A block that already holds earlier positions of its sequence takes the larger of
