@@ -32,46 +32,95 @@ struct RowMap {
     static constexpr int HEADS = kRowWarps / WPB;   // heads of a CTA
 };
 
+// four consecutive elements as loaded: what is in flight takes half the registers for 16-bit types
+template <int TYPE>
+struct Raw4 {
+    uint2 u;
+    __device__ float4 value() const {
+        if constexpr (TYPE == BZB_F16) {
+            const float2 a = __half22float2(*reinterpret_cast<const half2 *>(&u.x)), b = __half22float2(*reinterpret_cast<const half2 *>(&u.y));
+            return make_float4(a.x, a.y, b.x, b.y);
+        } else {
+            return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                               __uint_as_float(u.y & 0xffff0000u));
+        }
+    }
+};
+template <>
+struct Raw4<BZB_F32> {
+    float4 u;
+    __device__ float4 value() const { return u; }
+};
+template <int TYPE, bool VEC>
+__device__ __forceinline__ Raw4<TYPE> raw4(const void * p, long long i) {
+    Raw4<TYPE> r;
+    if constexpr (TYPE == BZB_F32) {
+        r.u = load4<BZB_F32, VEC>(p, i);
+    } else {
+        const uint16_t * h = static_cast<const uint16_t *>(p) + i;
+        if constexpr (VEC) r.u = __ldg(reinterpret_cast<const uint2 *>(h));
+        else r.u = make_uint2((uint32_t) h[0] | (uint32_t) h[1] << 16, (uint32_t) h[2] | (uint32_t) h[3] << 16);
+    }
+    return r;
+}
+
 struct AppendArgs {
     Kv kv;
     Rows q, k, v, q_out;
     const float * q_norm, * k_norm;
     const float2 * rope;
     float eps;
-    int n_head, n_blk, units, q_out_type;           // units: CTAs of a block of positions
+    int n_head, q_out_type;
     bool q_out_vec, norm_vec;
 };
 
 template <int HD, int TYPE, bool VEC>
-__global__ void __launch_bounds__(32 * kRowWarps, 6) kv8_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(32 * kRowWarps, 5) kv8_append_kernel(const AppendArgs a) {
     using R = RowMap<HD>;
     __shared__ float tops[kRowWarps];
     const Kv & kv = a.kv;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane % R::LPR;
     const int r0 = warp % R::WPB * (16 / R::WPB) + lane / R::LPR * 4;  // the lane's first row of the block
-    const int unit = (int) (blockIdx.x % a.units);
-    const unsigned sb = blockIdx.x / a.units;
-    const int b = (int) (sb / a.n_blk);
-    const Seq s = load_seq(kv, b);
+    const Seq s = load_seq(kv, (int) blockIdx.z);
     if (s.slot < 0) return;
     const int first = s.len - s.n;  // position of the sequence's first row (negative: padding rows)
-    const int blk = (max(first, 0) >> 4) + (int) (sb % a.n_blk), p0 = blk << 4;
+    const int blk = (max(first, 0) >> 4) + (int) blockIdx.y, p0 = blk << 4;
     if (p0 >= s.len || s.n == 0) return;  // (the whole CTA, as above)
-    const int any = unit * R::HEADS + warp / R::WPB;
-    const int kind = any < a.n_head ? 0 : any < a.n_head + kv.n_kv ? 1 : any < a.n_head + 2 * kv.n_kv ? 2 : 3;
-    const int head = kind == 0 ? any : kind == 1 ? any - a.n_head : any - a.n_head - kv.n_kv;
+    const int nq = a.n_head, nkv = kv.n_kv;
+    const int any = (int) blockIdx.x * R::HEADS + warp / R::WPB;
+    const int kind = any < nq ? 0 : any < nq + nkv ? 1 : any < nq + 2 * nkv ? 2 : 3;
+    const int head = kind == 0 ? any : kind == 1 ? any - nq : any - nq - nkv;
     const Rows src = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-    const int live_lo = kind < 3 ? max(first - p0, 0) : 16, live_hi = min(16, s.len - p0);  // the block's new rows
+    const int live_lo = max(first - p0, 0), live_hi = min(16, s.len - p0);  // the block's new rows
+    bool live[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) live[i] = kind < 3 && r0 + i >= live_lo && r0 + i < live_hi;
+    const long long row = s.row0 + p0 + r0 - first;  // packed row of the lane's first position
 
-    float4 lo[4], hi[4];
+    // rows, (cos, sin) and weights on the way together
+    Raw4<TYPE> lo_raw[4] = {}, hi_raw[4] = {};
+    float4 turn[4][2];  // of pairs 4c, 4c + 1 and of 4c + 2, 4c + 3
+    long long at = row * src.row + head * src.head + 4 * c;
+    const bool turned = kind < 2 && a.rope;
+#pragma unroll
+    for (int i = 0; i < 4; i++, at += src.row) {
+        if (!live[i]) continue;
+        lo_raw[i] = raw4<TYPE, VEC>(src.p, at);
+        hi_raw[i] = raw4<TYPE, VEC>(src.p, at + HD / 2);
+    }
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        lo[i] = hi[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (r0 + i >= live_lo && r0 + i < live_hi) {
-            const long long at = (long long) (s.row0 + p0 + r0 + i - first) * src.row + head * src.head + 4 * c;
-            lo[i] = load4<TYPE, VEC>(src.p, at);
-            hi[i] = load4<TYPE, VEC>(src.p, at + HD / 2);
-        }
+        turn[i][0] = turn[i][1] = make_float4(1.0f, 0.0f, 1.0f, 0.0f);
+        if (!live[i] || !turned) continue;
+        const float4 * t = reinterpret_cast<const float4 *>(a.rope + (size_t) (p0 + r0 + i) * (HD / 2) + 4 * c);
+        turn[i][0] = __ldg(t);
+        turn[i][1] = __ldg(t + 1);
+    }
+    const float * w = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
+    float4 wl = make_float4(0.0f, 0.0f, 0.0f, 0.0f), wh = wl;
+    if (w) {
+        wl = a.norm_vec ? load4<BZB_F32, true>(w, 4 * c) : load4<BZB_F32, false>(w, 4 * c);
+        wh = a.norm_vec ? load4<BZB_F32, true>(w, HD / 2 + 4 * c) : load4<BZB_F32, false>(w, HD / 2 + 4 * c);
     }
     const bool cached = kind == 1 || kind == 2, older = cached && p0 < first;  // older: the block holds earlier positions
     const int pg = cached ? page_of(kv, s.slot, blk) : -1;
@@ -97,37 +146,43 @@ __global__ void __launch_bounds__(32 * kRowWarps, 6) kv8_append_kernel(const App
             }
         }
     }
-    const float * w = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
+    float4 lo[4], hi[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) lo[i] = lo_raw[i].value(), hi[i] = hi_raw[i].value();
     if (w) {
-        const float4 wl = a.norm_vec ? load4<BZB_F32, true>(w, 4 * c) : load4<BZB_F32, false>(w, 4 * c);
-        const float4 wh = a.norm_vec ? load4<BZB_F32, true>(w, HD / 2 + 4 * c) : load4<BZB_F32, false>(w, HD / 2 + 4 * c);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             float4 & x = lo[i], & y = hi[i];
-            float ss = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w + y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w;
+            float2 sq = __fmul2_rn(make_float2(x.x, x.y), make_float2(x.x, x.y));
+            sq = __ffma2_rn(make_float2(x.z, x.w), make_float2(x.z, x.w), sq);
+            sq = __ffma2_rn(make_float2(y.x, y.y), make_float2(y.x, y.y), sq);
+            sq = __ffma2_rn(make_float2(y.z, y.w), make_float2(y.z, y.w), sq);
+            float ss = sq.x + sq.y;
 #pragma unroll
             for (int o = R::LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
             const float r = rsqrtf(ss * (1.0f / HD) + a.eps);
-            x = make_float4(x.x * r * wl.x, x.y * r * wl.y, x.z * r * wl.z, x.w * r * wl.w);
-            y = make_float4(y.x * r * wh.x, y.y * r * wh.y, y.z * r * wh.z, y.w * r * wh.w);
+            auto scale = [&](float4 & v, const float4 & w) {
+                const float2 p = __fmul2_rn(__fmul2_rn(make_float2(v.x, v.y), make_float2(r, r)), make_float2(w.x, w.y));
+                const float2 q = __fmul2_rn(__fmul2_rn(make_float2(v.z, v.w), make_float2(r, r)), make_float2(w.z, w.w));
+                v = make_float4(p.x, p.y, q.x, q.y);
+            };
+            scale(x, wl);
+            scale(y, wh);
         }
     }
-    if (kind < 2 && a.rope) {
+    if (turned) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            if (r0 + i < live_lo || r0 + i >= live_hi) continue;
-            const float4 * t = reinterpret_cast<const float4 *>(a.rope + (size_t) (p0 + r0 + i) * (HD / 2) + 4 * c);
-            const float4 t0 = __ldg(t), t1 = __ldg(t + 1);  // (cos, sin) of pairs 4c, 4c + 1 and of 4c + 2, 4c + 3
-            const float4 x = lo[i], y = hi[i];
+            const float4 t0 = turn[i][0], t1 = turn[i][1], x = lo[i], y = hi[i];
             lo[i] = make_float4(x.x * t0.x - y.x * t0.y, x.y * t0.z - y.y * t0.w, x.z * t1.x - y.z * t1.y, x.w * t1.z - y.w * t1.w);
             hi[i] = make_float4(x.x * t0.y + y.x * t0.x, x.y * t0.w + y.y * t0.z, x.z * t1.y + y.z * t1.x, x.w * t1.w + y.w * t1.z);
         }
     }
     if (kind == 0) {
+        long long at = row * a.q_out.row + head * a.q_out.head + 4 * c;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (r0 + i < live_lo || r0 + i >= live_hi) continue;
-            const long long at = (long long) (s.row0 + p0 + r0 + i - first) * a.q_out.row + head * a.q_out.head + 4 * c;
+        for (int i = 0; i < 4; i++, at += a.q_out.row) {
+            if (!live[i]) continue;
             store4(a.q_out_type, a.q_out_vec, a.q_out.p, at, lo[i]);
             store4(a.q_out_type, a.q_out_vec, a.q_out.p, at + HD / 2, hi[i]);
         }
@@ -199,7 +254,6 @@ __global__ void __launch_bounds__(32 * kRowWarps, 6) kv8_append_kernel(const App
 struct ReadArgs {
     Kv kv;
     Rows k, v;
-    int n_blk, units;
     bool vec;
 };
 
@@ -209,14 +263,11 @@ __global__ void __launch_bounds__(32 * kRowWarps) kv8_read_kernel(const ReadArgs
     const Kv & kv = a.kv;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane % R::LPR;
     const int r0 = warp % R::WPB * (16 / R::WPB) + lane / R::LPR * 4;
-    const int unit = (int) (blockIdx.x % a.units);
-    const unsigned sb = blockIdx.x / a.units;
-    const int b = (int) (sb / a.n_blk);
-    const Seq s = load_seq(kv, b);
+    const Seq s = load_seq(kv, (int) blockIdx.z);
     if (s.slot < 0 || s.n == 0) return;
     // blocks count from the first row's position; `first` may be negative (padding rows, read as zeros)
-    const int first = s.len - s.n, blk = (first >> 4) + (int) (sb % a.n_blk), p0 = blk << 4;
-    const int any = unit * R::HEADS + warp / R::WPB;
+    const int first = s.len - s.n, blk = (first >> 4) + (int) blockIdx.y, p0 = blk << 4;
+    const int any = (int) blockIdx.x * R::HEADS + warp / R::WPB;
     if (p0 >= s.len || any >= 2 * kv.n_kv) return;
     const int plane = any >= kv.n_kv, head = any - plane * kv.n_kv;
     float4 lo[4], hi[4];
@@ -256,11 +307,11 @@ __global__ void __launch_bounds__(32 * kRowWarps) kv8_read_kernel(const ReadArgs
         }
     }
     const Rows dst = plane ? a.v : a.k;
+    long long at = (long long) (s.row0 + p0 + r0 - first) * dst.row + head * dst.head + 4 * c;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < 4; i++, at += dst.row) {
         const int pos = p0 + r0 + i;
         if (pos < first || pos >= s.len) continue;
-        const long long at = (long long) (s.row0 + pos - first) * dst.row + head * dst.head + 4 * c;
         store4(TYPE, a.vec, dst.p, at, lo[i]);
         store4(TYPE, a.vec, dst.p, at + HD / 2, hi[i]);
     }
@@ -716,19 +767,24 @@ unsigned grid_of(long long tasks, int per_cta) {
     return (unsigned) n;
 }
 
+// append and read: (heads, blocks of 16 positions that max_new rows can touch, sequences)
+dim3 row_grid(const Kv & kv, int heads, int per_cta) {
+    const int blocks = (kv.max_new + 30) / 16;
+    if (blocks > 65535 || kv.n_seq > 65535) fail("at most 65535 sequences and 2^20 - 31 rows of each in one call");
+    return dim3((heads + per_cta - 1) / per_cta, blocks, kv.n_seq);
+}
+
 template <int HD, int TYPE>
-void run_append(AppendArgs a, bool vec, cudaStream_t s) {
-    a.units = (a.n_head + 2 * a.kv.n_kv + RowMap<HD>::HEADS - 1) / RowMap<HD>::HEADS;
-    const unsigned grid = grid_of((long long) a.kv.n_seq * a.n_blk * a.units, 1);
+void run_append(const AppendArgs & a, bool vec, cudaStream_t s) {
+    const dim3 grid = row_grid(a.kv, a.n_head + 2 * a.kv.n_kv, RowMap<HD>::HEADS);
     if (vec) kv8_append_kernel<HD, TYPE, true><<<grid, 32 * kRowWarps, 0, s>>>(a);
     else kv8_append_kernel<HD, TYPE, false><<<grid, 32 * kRowWarps, 0, s>>>(a);
     check_cuda(cudaGetLastError(), "launch");
 }
 
 template <int HD, int TYPE>
-void run_read(ReadArgs a, cudaStream_t s) {
-    a.units = (2 * a.kv.n_kv + RowMap<HD>::HEADS - 1) / RowMap<HD>::HEADS;
-    const unsigned grid = grid_of((long long) a.kv.n_seq * a.n_blk * a.units, 1);
+void run_read(const ReadArgs & a, cudaStream_t s) {
+    const dim3 grid = row_grid(a.kv, 2 * a.kv.n_kv, RowMap<HD>::HEADS);
     kv8_read_kernel<HD, TYPE><<<grid, 32 * kRowWarps, 0, s>>>(a);
     check_cuda(cudaGetLastError(), "launch");
 }
@@ -825,7 +881,6 @@ void kv8_append(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_kv8_
     a.rope = reinterpret_cast<const float2 *>(rope);
     a.norm_vec = (uintptr_t) q_norm % 16 == 0 && (uintptr_t) k_norm % 16 == 0;
     a.eps = eps;
-    a.n_blk = (b.max_new + 30) / 16;  // blocks that max_new positions can touch
     if (c.head_dim == 64) {
         if (k.type == BZB_F32) run_append<64, BZB_F32>(a, vec, s);
         else if (k.type == BZB_F16) run_append<64, BZB_F16>(a, vec, s);
@@ -849,7 +904,6 @@ void kv8_read(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_kv8_ro
     if (b.n_seq == 0 || b.n_tok == 0 || b.max_new == 0) return;
     a.k = Rows{ k_out.data, k_out.row_stride, k_out.head_stride };
     a.v = Rows{ v_out.data, v_out.row_stride, v_out.head_stride };
-    a.n_blk = (b.max_new + 30) / 16;
     if (c.head_dim == 64) {
         if (k_out.type == BZB_F32) run_read<64, BZB_F32>(a, s);
         else if (k_out.type == BZB_F16) run_read<64, BZB_F16>(a, s);
