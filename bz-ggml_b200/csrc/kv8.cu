@@ -328,12 +328,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ uint4 load_stream(const void * p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
 // 16 elements of a query row from element i as f16 pairs: f16 rows as they are, bf16 rows times f (and
 // their largest magnitude into amax)
 __device__ __forceinline__ void load_q16(const AttnArgs & a, long long i, float f, uint32_t (&o)[8], float * amax) {
@@ -371,24 +365,40 @@ __device__ __forceinline__ void load_q16(const AttnArgs & a, long long i, float 
 }
 
 // Few query rows (a step of each sequence, or a few guessed tokens): one CTA per (sequence, kv head, tile
-// of 8 NT query rows, range of the cache), its warps taking the range's blocks in turn. The rows of a
-// kv head are (token, head of the group) pairs, so a block read once serves the whole group.
+// of 8 NT query rows, range of the cache), its warps taking the range's blocks in turn, two at a time. The rows
+// of a kv head are (token, head of the group) pairs, so a block read once serves the whole group.
 //
 // The matrix products are m16n8k16 with the cache as the 16-row operand: S^T = K Q^T (16 positions x 8
 // rows) and O^T = V^T W^T (16 of head_dim x 8 rows): no half of a tile is empty when a group has at
-// most 8 rows. Both operands come straight from global memory into the MMA's register layout: a lane's 16
-// bytes of a key row are the four k-steps' values of head_dim for it (the queries are read in the same
-// order, so any order of the sum's terms will do), and the value patches are stored in operand order. No shared memory, no
-// transposition but the 8x8 one of the weights; per lane 4 loads of 16 bytes a block for head_dim 64.
+// most 8 rows. A lane's 16 bytes of a key row are the four k-steps' values of head_dim for it (the queries are
+// read in the same order, and any order of the sum's terms will do), and the value patches are stored in operand
+// order, so every lane copies exactly the bytes it multiplies: a ring of cp.async copies for each
+// warp, each lane reading back its own slots, without a barrier, a bank conflict or a transposition but the
+// 8x8 one of the weights.
 template <int HD, int NT, int WARPS>
 struct SmallTile {
     static constexpr int ROWS = 8 * NT, KS = HD / 64, VS = HD / 32, MT = HD / 16, PL = HD + 4;
+    static constexpr int PIECES = 2 * KS + VS;            // 16-byte pieces of a block for each lane
+    static constexpr int DEPTH = 4;                       // blocks of a warp's ring: two in use, two under way
+    static constexpr int RING = WARPS * DEPTH * PIECES * 512, MERGE = WARPS * ROWS * (HD + 4) * 4;
+    static constexpr int BYTES = RING > MERGE ? RING : MERGE;
 };
+constexpr int kSmallWarps = 4;
+constexpr int kSmallRange = 32 * kSmallWarps;  // blocks of a range at most: a lane holds one page id for its warp
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void * src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
 
 template <int HD, int NT, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS) kv8_attn_small_kernel(const AttnArgs a) {
     using T = SmallTile<HD, NT, WARPS>;
-    __shared__ float sm_o[WARPS][T::ROWS][HD + 4];
+    extern __shared__ __align__(16) uint8_t ring[];
     __shared__ float sm_ml[WARPS][T::ROWS][2];
     const Kv & kv = a.kv;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -414,6 +424,40 @@ __global__ void __launch_bounds__(32 * WARPS) kv8_attn_small_kernel(const AttnAr
     const int my_chunks = max(1, (blk_hi - blk_lo + a.chunk_blocks - 1) / a.chunk_blocks);
     if (chunk >= my_chunks) return;
     const int c_lo = blk_lo + chunk * a.chunk_blocks, c_hi = min(blk_hi, c_lo + a.chunk_blocks);
+
+    // pages and scales of this warp's blocks base, base + WARPS, ..., one block per lane
+    const int base = c_lo + warp, n = max(0, (c_hi - base + WARPS - 1) / WARPS);
+    int my_pg = 0;
+    float my_ks = 0.0f, my_vs = 1.0f;
+    if (lane < n) {
+        const int blk = base + lane * WARPS;
+        my_pg = max(page_of(kv, s.slot, blk), 0);
+        my_ks = __ldg(scale_ptr(kv, my_pg, blk, 0, h));
+        my_vs = __ldg(scale_ptr(kv, my_pg, blk, 1, h));
+    }
+    const int kpos = (g >> 1) * 4 + (g & 1);  // the lane's key rows: kpos and kpos + 2 (see the patches' position order)
+    const uint32_t mine = (uint32_t) __cvta_generic_to_shared(ring) + warp * (T::DEPTH * T::PIECES * 512) + lane * 16;
+    // blocks i, i + 1 of the warp into their slots; a block past the last is zeros
+    auto fetch = [&](int i) {
+#pragma unroll
+        for (int k2 = 0; k2 < 2; k2++) {
+            const bool there = i + k2 < n;
+            const int pg = __shfl_sync(0xffffffffu, my_pg, (i + k2) & 31), blk = there ? base + (i + k2) * WARPS : c_lo;
+            const uint8_t * kp = block_ptr(kv, pg, blk, 0, h, HD) + kpos * HD + 16 * t;
+            const uint8_t * vp = block_ptr(kv, pg, blk, 1, h, HD) + 16 * lane;
+            const uint32_t slot = mine + (i + k2) % T::DEPTH * (T::PIECES * 512);
+#pragma unroll
+            for (int k = 0; k < T::KS; k++) {
+                copy16(slot + (2 * k) * 512, kp + 64 * k, there);
+                copy16(slot + (2 * k + 1) * 512, kp + 2 * HD + 64 * k, there);
+            }
+#pragma unroll
+            for (int j = 0; j < T::VS; j++) copy16(slot + (2 * T::KS + j) * 512, vp + 512 * j, there);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < T::DEPTH - 2; i += 2) fetch(i);
 
     // queries as the 8-column operand: lane (g, t) holds row 8 nt + g, elements 64 k + 16 t ..+15
     uint32_t qf[NT][T::KS][8];
@@ -458,36 +502,23 @@ __global__ void __launch_bounds__(32 * WARPS) kv8_attn_small_kernel(const AttnAr
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) m[nt][0] = m[nt][1] = -INFINITY;
 
-    const int kpos = (g >> 1) * 4 + (g & 1);  // the lane's key rows: kpos and kpos + 2 (see the patches' position order)
-    for (int base = c_lo + warp; base < c_hi; base += 32 * WARPS) {
-        // pages and scales of this warp's next 32 blocks, one block per lane
-        int my_pg = 0;
-        float my_ks = 0.0f, my_vs = 1.0f;
-        if (base + lane * WARPS < c_hi) {
-            const int blk = base + lane * WARPS;
-            my_pg = max(page_of(kv, s.slot, blk), 0);
-            my_ks = __ldg(scale_ptr(kv, my_pg, blk, 0, h));
-            my_vs = __ldg(scale_ptr(kv, my_pg, blk, 1, h));
-        }
-        const int n = min(32, (c_hi - base + WARPS - 1) / WARPS);
-        uint4 kf[2][T::KS][2], vf[2][T::VS];
-        auto fetch = [&](int i, uint4 (&kk)[T::KS][2], uint4 (&vv)[T::VS]) {
-            const int pg = __shfl_sync(0xffffffffu, my_pg, i), blk = base + i * WARPS;
-            const uint8_t * kp = block_ptr(kv, pg, blk, 0, h, HD) + kpos * HD + 16 * t;
-            const uint8_t * vp = block_ptr(kv, pg, blk, 1, h, HD) + 16 * lane;
+    for (int i = 0; i < n; i += 2) {
+        // (always a group, empty past the end, so that the one waited for is the DEPTH / 2 - 1 st before)
+        if (i + T::DEPTH - 2 < n) fetch(i + T::DEPTH - 2);
+        else asm volatile("cp.async.commit_group;" ::: "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(T::DEPTH / 2 - 1) : "memory");
+        float x[2][NT][4];  // columns 2t, 2t+1 at key kpos, then at key kpos + 2
+        uint32_t seen[2][NT][2];  // (positions x rows) the rows that see each position, as f16 ones
+        bool whole[2];
+        float inv_vs[2];
 #pragma unroll
-            for (int k = 0; k < T::KS; k++) kk[k][0] = load_stream(kp + 64 * k), kk[k][1] = load_stream(kp + 2 * HD + 64 * k);
-#pragma unroll
-            for (int j = 0; j < T::VS; j++) vv[j] = load_stream(vp + 512 * j);
-        };
-        auto use = [&](int i, const uint4 (&kk)[T::KS][2], const uint4 (&vv)[T::VS]) {
-            const float ks = __shfl_sync(0xffffffffu, my_ks, i), vs = __shfl_sync(0xffffffffu, my_vs, i);
-            const int key0 = (base + i * WARPS) << 4;
+        for (int k2 = 0; k2 < 2; k2++) {
+            const uint32_t slot = mine + (i + k2) % T::DEPTH * (T::PIECES * 512);
             float sc[NT][4] = {};
 #pragma unroll
             for (int k = 0; k < T::KS; k++) {
-                const uint32_t w0[4] = { kk[k][0].x, kk[k][0].y, kk[k][0].z, kk[k][0].w };
-                const uint32_t w1[4] = { kk[k][1].x, kk[k][1].y, kk[k][1].z, kk[k][1].w };
+                const uint4 u0 = lds16(slot + (2 * k) * 512), u1 = lds16(slot + (2 * k + 1) * 512);
+                const uint32_t w0[4] = { u0.x, u0.y, u0.z, u0.w }, w1[4] = { u1.x, u1.y, u1.z, u1.w };
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const uint32_t a0 = e4m3x2_to_h2((uint16_t) w0[j]), a2 = e4m3x2_to_h2((uint16_t) (w0[j] >> 16));
@@ -496,93 +527,109 @@ __global__ void __launch_bounds__(32 * WARPS) kv8_attn_small_kernel(const AttnAr
                     for (int nt = 0; nt < NT; nt++) mma16816(sc[nt], a0, a1, a2, a3, qf[nt][k][2 * j], qf[nt][k][2 * j + 1]);
                 }
             }
-            const float ev = (float) exponent_of(vs), inv_vs = 1.0f / vs;
-            const bool whole = key0 >= full_lo && key0 + 16 <= full_hi;
-            uint32_t seen[NT][2];  // (positions x rows) the rows that see each position, as f16 ones
-            uint32_t wb[NT][2];
-            bool moved = false;
-            float corr[NT][2];
+            const float ks = __shfl_sync(0xffffffffu, my_ks, (i + k2) & 31), vs = __shfl_sync(0xffffffffu, my_vs, (i + k2) & 31);
+            const int key0 = (base + (i + k2) * WARPS) << 4;  // (past the range: past every row's limit or masked below)
+            const bool there = i + k2 < n;
+            const float ev = (float) exponent_of(vs);
+            inv_vs[k2] = pow2f(-exponent_of(vs));
+            whole[k2] = there && key0 >= full_lo && key0 + 16 <= full_hi;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                float x[4];  // columns 2t, 2t+1 at key kpos, then at key kpos + 2
+                const float c0 = coef[nt][0] * ks, c1 = coef[nt][1] * ks;
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    x[j] = fmaf(sc[nt][j], coef[nt][j & 1] * ks, ev);
-                    if (!whole) {
+                for (int j = 0; j < 4; j++) x[k2][nt][j] = fmaf(sc[nt][j], j & 1 ? c1 : c0, ev);
+                if (!whole[k2]) {
+                    uint32_t one[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
                         const int key = key0 + kpos + (j >> 1) * 2;
-                        if (key < lim_lo[nt][j & 1] || key >= lim_hi[nt][j & 1]) x[j] = -INFINITY;
+                        const bool in = there && key >= lim_lo[nt][j & 1] && key < lim_hi[nt][j & 1];
+                        if (!in) x[k2][nt][j] = -INFINITY;
+                        one[j] = in ? 0x3c00u : 0u;
                     }
+                    seen[k2][nt][0] = one[0] | (one[1] << 16);
+                    seen[k2][nt][1] = one[2] | (one[3] << 16);
                 }
-                if (!whole) {
-                    auto one = [&](int j) {
-                        const int key = key0 + kpos + (j >> 1) * 2;
-                        return key >= lim_lo[nt][j & 1] && key < lim_hi[nt][j & 1] ? 0x3c00u : 0u;
-                    };
-                    seen[nt][0] = one(0) | (one(1) << 16);
-                    seen[nt][1] = one(2) | (one(3) << 16);
-                }
-#pragma unroll
-                for (int i2 = 0; i2 < 2; i2++) {
-                    float mx = fmaxf(x[i2], x[i2 + 2]);
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                    const float to = fmaxf(m[nt][i2], mx), ref = to == -INFINITY ? 0.0f : to;
-                    corr[nt][i2] = exp2_approx(m[nt][i2] - ref);
-                    moved |= to != m[nt][i2];
-                    m[nt][i2] = to;
-                    x[i2] = exp2_approx(x[i2] - ref);
-                    x[i2 + 2] = exp2_approx(x[i2 + 2] - ref);
-                    l[nt][i2] = fmaf(l[nt][i2], corr[nt][i2], (x[i2] + x[i2 + 2]) * inv_vs);
-                }
-                wb[nt][0] = transpose8x8(pack_half(x[0], x[1]));
-                wb[nt][1] = transpose8x8(pack_half(x[2], x[3]));
             }
-            if (__any_sync(0xffffffffu, moved)) {
+        }
+        uint32_t wb[2][NT][2];
+        bool moved = false;
+        float corr[NT][2];
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
+        for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-                    for (int j = 0; j < T::MT; j++)
+            for (int i2 = 0; i2 < 2; i2++) {
+                float mx = fmaxf(fmaxf(x[0][nt][i2], x[0][nt][i2 + 2]), fmaxf(x[1][nt][i2], x[1][nt][i2 + 2]));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                const float to = fmaxf(m[nt][i2], mx), ref = to == -INFINITY ? 0.0f : to;
+                corr[nt][i2] = exp2_approx(m[nt][i2] - ref);
+                moved |= to != m[nt][i2];
+                m[nt][i2] = to;
+                float sum = 0.0f;
 #pragma unroll
-                        for (int i2 = 0; i2 < 4; i2++) o[nt][j][i2] *= corr[nt][i2 & 1];
+                for (int k2 = 0; k2 < 2; k2++) {
+                    x[k2][nt][i2] = exp2_approx(x[k2][nt][i2] - ref);
+                    x[k2][nt][i2 + 2] = exp2_approx(x[k2][nt][i2 + 2] - ref);
+                    sum = fmaf(x[k2][nt][i2] + x[k2][nt][i2 + 2], inv_vs[k2], sum);
+                }
+                l[nt][i2] = fmaf(l[nt][i2], corr[nt][i2], sum);
             }
+#pragma unroll
+            for (int k2 = 0; k2 < 2; k2++) {
+                wb[k2][nt][0] = transpose8x8(pack_half(x[k2][nt][0], x[k2][nt][1]));
+                wb[k2][nt][1] = transpose8x8(pack_half(x[k2][nt][2], x[k2][nt][3]));
+            }
+        }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int j = 0; j < T::MT; j++)
+#pragma unroll
+                    for (int i2 = 0; i2 < 4; i2++) o[nt][j][i2] *= corr[nt][i2 & 1];
+        }
+#pragma unroll
+        for (int k2 = 0; k2 < 2; k2++) {
+            const uint32_t slot = mine + (i + k2) % T::DEPTH * (T::PIECES * 512);
             uint4 vw[T::VS];
-            uint32_t bad = 0;
 #pragma unroll
-            for (int j = 0; j < T::VS; j++) {
-                vw[j] = vv[j];
-                if (!whole) bad |= nan_bytes(vv[j].x) | nan_bytes(vv[j].y) | nan_bytes(vv[j].z) | nan_bytes(vv[j].w);
-            }
-            // a NaN at a position that some row does not see must not reach that row (0 x NaN):
-            // NaNs are taken out of the product and given to the rows that see them
-            const bool poisoned = !whole && __any_sync(0xffffffffu, bad != 0);
-            if (poisoned) {
-                uint32_t sb0[NT], sb1[NT];
+            for (int j = 0; j < T::VS; j++) vw[j] = lds16(slot + (2 * T::KS + j) * 512);
+            if (!whole[k2]) {
+                // a NaN at a position that some row does not see must not reach that row (0 x NaN):
+                // NaNs are taken out of the product and given to the rows that see them
+                uint32_t bad = 0;
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) sb0[nt] = transpose8x8(seen[nt][0]), sb1[nt] = transpose8x8(seen[nt][1]);
+                for (int j = 0; j < T::VS; j++) bad |= nan_bytes(vw[j].x) | nan_bytes(vw[j].y) | nan_bytes(vw[j].z) | nan_bytes(vw[j].w);
+                if (__any_sync(0xffffffffu, bad != 0)) {
+                    uint32_t sb0[NT], sb1[NT];
 #pragma unroll
-                for (int j = 0; j < T::VS; j++) {
-                    uint32_t w[4] = { vw[j].x, vw[j].y, vw[j].z, vw[j].w };
+                    for (int nt = 0; nt < NT; nt++) sb0[nt] = transpose8x8(seen[k2][nt][0]), sb1[nt] = transpose8x8(seen[k2][nt][1]);
 #pragma unroll
-                    for (int half_ = 0; half_ < 2; half_++) {
-                        uint32_t f[4];  // f16 ones at NaNs
+                    for (int j = 0; j < T::VS; j++) {
+                        uint32_t w[4] = { vw[j].x, vw[j].y, vw[j].z, vw[j].w };
 #pragma unroll
-                        for (int i2 = 0; i2 < 2; i2++) {
-                            const uint32_t nb = nan_bytes(w[2 * half_ + i2]);
-                            f[i2] = ((nb & 1u) ? 0x3c00u : 0u) | ((nb & 0x100u) ? 0x3c000000u : 0u);
-                            f[2 + i2] = ((nb & 0x10000u) ? 0x3c00u : 0u) | ((nb & 0x1000000u) ? 0x3c000000u : 0u);
-                            w[2 * half_ + i2] &= ~nb;
+                        for (int half_ = 0; half_ < 2; half_++) {
+                            uint32_t f[4];  // f16 ones at NaNs
+#pragma unroll
+                            for (int i2 = 0; i2 < 2; i2++) {
+                                const uint32_t nb = nan_bytes(w[2 * half_ + i2]);
+                                f[i2] = ((nb & 1u) ? 0x3c00u : 0u) | ((nb & 0x100u) ? 0x3c000000u : 0u);
+                                f[2 + i2] = ((nb & 0x10000u) ? 0x3c00u : 0u) | ((nb & 0x1000000u) ? 0x3c000000u : 0u);
+                                w[2 * half_ + i2] &= ~nb;
+                            }
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) {
+                                float hit[4] = {};
+                                mma16816(hit, f[0], f[1], f[2], f[3], sb0[nt], sb1[nt]);
+#pragma unroll
+                                for (int i2 = 0; i2 < 4; i2++)
+                                    if (hit[i2] > 0.0f) o[nt][2 * j + half_][i2] = __int_as_float(0x7fffffff);
+                            }
                         }
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++) {
-                            float hit[4] = {};
-                            mma16816(hit, f[0], f[1], f[2], f[3], sb0[nt], sb1[nt]);
-#pragma unroll
-                            for (int i2 = 0; i2 < 4; i2++)
-                                if (hit[i2] > 0.0f) o[nt][2 * j + half_][i2] = __int_as_float(0x7fffffff);
-                        }
+                        vw[j] = make_uint4(w[0], w[1], w[2], w[3]);
                     }
-                    vw[j] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
 #pragma unroll
@@ -593,20 +640,14 @@ __global__ void __launch_bounds__(32 * WARPS) kv8_attn_small_kernel(const AttnAr
                     const uint32_t a0 = e4m3x2_to_h2((uint16_t) w[2 * half_]), a2 = e4m3x2_to_h2((uint16_t) (w[2 * half_] >> 16));
                     const uint32_t a1 = e4m3x2_to_h2((uint16_t) w[2 * half_ + 1]), a3 = e4m3x2_to_h2((uint16_t) (w[2 * half_ + 1] >> 16));
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) mma16816(o[nt][2 * j + half_], a0, a1, a2, a3, wb[nt][0], wb[nt][1]);
+                    for (int nt = 0; nt < NT; nt++) mma16816(o[nt][2 * j + half_], a0, a1, a2, a3, wb[k2][nt][0], wb[k2][nt][1]);
                 }
-            }
-        };
-        fetch(0, kf[0], vf[0]);
-        for (int i = 0; i < n; i += 2) {
-            if (i + 1 < n) fetch(i + 1, kf[1], vf[1]);
-            use(i, kf[0], vf[0]);
-            if (i + 1 < n) {
-                if (i + 2 < n) fetch(i + 2, kf[0], vf[0]);
-                use(i + 1, kf[1], vf[1]);
             }
         }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();  // the rings become the warps' outputs
+    float (*sm_o)[T::ROWS][HD + 4] = reinterpret_cast<float (*)[T::ROWS][HD + 4]>(ring);
 
     // the warps' states to shared memory: [row][element]; element of (mt, half, g): 32 (mt/2) + 4 g + 2 (mt%2) + half
 #pragma unroll
@@ -796,8 +837,7 @@ struct Plan {
     int rows = 8;           // rows of a CTA
     int row_tiles = 1, chunks = 1, chunk_blocks = 1;
 };
-constexpr int kSmallWarps = 4;
-constexpr int kFewRows = 64;
+constexpr int kFewRows = 32;
 
 Plan plan_of(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int causal, int window) {
     Plan p;
@@ -824,6 +864,7 @@ Plan plan_of(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int c
     const long long want = std::max<long long>(1, (p.tile ? 148 : 148 * 8) / units);
     p.chunk_blocks = (int) std::max<long long>(p.tile ? 16 : 8, (blocks + want - 1) / want);
     if (p.tile) p.chunk_blocks = (p.chunk_blocks + 7) / 8 * 8;
+    else p.chunk_blocks = std::min(p.chunk_blocks, kSmallRange);
     p.chunks = (blocks + p.chunk_blocks - 1) / p.chunk_blocks;
     return p;
 }
@@ -833,7 +874,10 @@ long long counter_bytes(long long units) { return (units * 4 + 15) / 16 * 16; }
 template <int HD, int NT>
 void run_small(const AttnArgs & a, cudaStream_t s) {
     const unsigned grid = grid_of((long long) a.kv.n_seq * a.row_tiles * a.chunks * a.kv.n_kv, 1);
-    kv8_attn_small_kernel<HD, NT, kSmallWarps><<<grid, 32 * kSmallWarps, 0, s>>>(a);
+    constexpr int bytes = SmallTile<HD, NT, kSmallWarps>::BYTES;
+    static std::atomic<uint64_t> ready{ 0 };
+    allow_shared_memory(kv8_attn_small_kernel<HD, NT, kSmallWarps>, bytes, ready);
+    kv8_attn_small_kernel<HD, NT, kSmallWarps><<<grid, 32 * kSmallWarps, bytes, s>>>(a);
     check_cuda(cudaGetLastError(), "launch");
 }
 

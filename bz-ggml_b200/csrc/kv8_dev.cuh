@@ -13,7 +13,10 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <cstdint>
+#include <stdexcept>
+#include <string>
 
 namespace bzb {
 namespace kv8 {
@@ -190,6 +193,18 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // bytes of w that are e4m3 NaN (0x7f or 0xff) become 0xff, the others 0
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu); }
 
+
+// a kernel's shared-memory limit, set once for each device (`ready`: one bit per device that has it)
+template <typename K>
+void allow_shared_memory(K kernel, int bytes, std::atomic<uint64_t> & ready) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (e == cudaSuccess && (ready.load(std::memory_order_acquire) & bit) && dev < 64) return;
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) throw std::runtime_error(std::string("shared memory: ") + cudaGetErrorString(e));
+    ready.fetch_or(bit, std::memory_order_release);
+}
 
 // the attention of many rows (kv8_tile.cu): rows of a kv head in tiles of kTileRows
 constexpr int kTileRows = 256;

@@ -670,17 +670,17 @@ template <int HD>
 void launch(const AttnArgs & a, cudaStream_t s) {
     const long long grid = (long long) a.kv.n_seq * a.row_tiles * a.chunks * a.kv.n_kv;
     if (grid > INT_MAX) throw std::runtime_error("the batch is too large for one call");
-    // the register split adds up only for the launch it was made for: a build that gives the kernel
-    // another count must not reach the GPU, where it would wait for registers that never come free
-    cudaFuncAttributes at;
-    if (cudaFuncGetAttributes(&at, kv8_attn_tile_kernel<HD>) != cudaSuccess || at.numRegs != kLaunchRegs)
-        throw std::runtime_error("kv8_attn_tile_kernel: built with another register count than its split needs");
-    // (set on every call: the attribute belongs to the current device)
-    cudaError_t e = cudaFuncSetAttribute(kv8_attn_tile_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) Smem<HD>::kBytes);
-    if (e == cudaSuccess) {
-        kv8_attn_tile_kernel<HD><<<(unsigned) grid, kTileThreads, Smem<HD>::kBytes, s>>>(a);
-        e = cudaGetLastError();
+    static std::atomic<uint64_t> ready{ 0 };
+    if (!ready.load(std::memory_order_acquire)) {
+        // the register split adds up only for the launch it was made for: a build that gives the kernel
+        // another count must not reach the GPU, where it would wait for registers that never come free
+        cudaFuncAttributes at;
+        if (cudaFuncGetAttributes(&at, kv8_attn_tile_kernel<HD>) != cudaSuccess || at.numRegs != kLaunchRegs)
+            throw std::runtime_error("kv8_attn_tile_kernel: built with another register count than its split needs");
     }
+    allow_shared_memory(kv8_attn_tile_kernel<HD>, (int) Smem<HD>::kBytes, ready);
+    kv8_attn_tile_kernel<HD><<<(unsigned) grid, kTileThreads, Smem<HD>::kBytes, s>>>(a);
+    const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) throw std::runtime_error(std::string("launch: ") + cudaGetErrorString(e));
 }
 
