@@ -372,19 +372,22 @@ __device__ __forceinline__ void load_q16(const AttnArgs & a, long long i, float 
 // rows) and O^T = V^T W^T (16 of head_dim x 8 rows): no half of a tile is empty when a group has at
 // most 8 rows. A lane's 16 bytes of a key row are the four k-steps' values of head_dim for it (the queries are
 // read in the same order, and any order of the sum's terms will do), and the value patches are stored in operand
-// order, so every lane copies exactly the bytes it multiplies: a ring of cp.async copies for each
-// warp, each lane reading back its own slots, without a barrier, a bank conflict or a transposition but the
-// 8x8 one of the weights.
+// order: no transposition but the 8x8 one of the weights. Each warp copies its blocks by itself, as they lie in
+// memory (cp.async), AHEAD pairs of blocks in advance: a pair's keys are copied as soon as the scores are
+// done with the pair before it in the ring, its values after the second product.
+// CTAs that an SM holds, by their registers
+constexpr int small_ctas(int hd, int nt) { return hd == 64 ? (nt == 1 ? 5 : nt == 2 ? 3 : 2) : (nt == 1 ? 4 : 2); }
+
 template <int HD, int NT, int WARPS>
 struct SmallTile {
     static constexpr int ROWS = 8 * NT, KS = HD / 64, VS = HD / 32, MT = HD / 16, PL = HD + 4;
     static constexpr int PIECES = 2 * KS + VS;            // 16-byte pieces of a block for each lane
-    static constexpr int DEPTH = 4;                       // blocks of a warp's ring: two in use, two under way
-    static constexpr int RING = WARPS * DEPTH * PIECES * 512, MERGE = WARPS * ROWS * (HD + 4) * 4;
+    static constexpr int AHEAD = HD == 64 ? 2 : 1;   // pairs of blocks that a warp's ring holds
+    static constexpr int RING = WARPS * AHEAD * 2 * PIECES * 512, MERGE = WARPS * ROWS * (HD + 4) * 4;
     static constexpr int BYTES = RING > MERGE ? RING : MERGE;
 };
-constexpr int kSmallWarps = 4;
-constexpr int kSmallRange = 32 * kSmallWarps;  // blocks of a range at most: a lane holds one page id for its warp
+constexpr int kSmallWarps = 4, kSmallBlocks = 128;
+constexpr int kSmallRange = kSmallBlocks * kSmallWarps;  // blocks of a range at most
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void * src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
@@ -396,19 +399,22 @@ __device__ __forceinline__ uint4 lds16(uint32_t a) {
 }
 
 template <int HD, int NT, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS) kv8_attn_small_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, NT)) kv8_attn_small_kernel(const AttnArgs a) {
     using T = SmallTile<HD, NT, WARPS>;
     extern __shared__ __align__(16) uint8_t ring[];
     __shared__ float sm_ml[WARPS][T::ROWS][2];
+    // the blocks of a warp's range: the head's keys (its values lie one plane on), the scales of both
+    __shared__ const uint8_t * block_at[WARPS][kSmallBlocks];
+    __shared__ float2 scales[WARPS][kSmallBlocks];
     const Kv & kv = a.kv;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     // (heads fastest: neighbouring CTAs read neighbouring bytes of the same pages)
-    long long id = blockIdx.x;
-    const int h = (int) (id % kv.n_kv);
-    id /= kv.n_kv;
-    const int chunk = (int) (id % a.chunks);
-    id /= a.chunks;
-    const int tile = (int) (id % a.row_tiles), b = (int) (id / a.row_tiles);
+    unsigned id = blockIdx.x;
+    const int h = (int) (id % (unsigned) kv.n_kv);
+    id /= (unsigned) kv.n_kv;
+    const int chunk = (int) (id % (unsigned) a.chunks);
+    id /= (unsigned) a.chunks;
+    const int tile = (int) (id % (unsigned) a.row_tiles), b = (int) (id / (unsigned) a.row_tiles);
     const Seq s = load_seq(kv, b);
     if (s.slot < 0) return;
     const int rows = s.n * a.group, row0 = tile * T::ROWS;
@@ -425,39 +431,59 @@ __global__ void __launch_bounds__(32 * WARPS) kv8_attn_small_kernel(const AttnAr
     if (chunk >= my_chunks) return;
     const int c_lo = blk_lo + chunk * a.chunk_blocks, c_hi = min(blk_hi, c_lo + a.chunk_blocks);
 
-    // pages and scales of this warp's blocks base, base + WARPS, ..., one block per lane
+    // this warp's blocks: base, base + WARPS, ...
     const int base = c_lo + warp, n = max(0, (c_hi - base + WARPS - 1) / WARPS);
-    int my_pg = 0;
-    float my_ks = 0.0f, my_vs = 1.0f;
+    auto look_up = [&](int i) {
+        if (i >= n) return;
+        const int blk = base + i * WARPS, pg = max(page_of(kv, s.slot, blk), 0);
+        block_at[warp][i] = block_ptr(kv, pg, blk, 0, h, HD);
+        scales[warp][i] = make_float2(__ldg(scale_ptr(kv, pg, blk, 0, h)), __ldg(scale_ptr(kv, pg, blk, 1, h)));
+    };
+    // (the first blocks' copies do not wait for their scales)
+    float2 sc0 = make_float2(0.0f, 0.0f);
     if (lane < n) {
-        const int blk = base + lane * WARPS;
-        my_pg = max(page_of(kv, s.slot, blk), 0);
-        my_ks = __ldg(scale_ptr(kv, my_pg, blk, 0, h));
-        my_vs = __ldg(scale_ptr(kv, my_pg, blk, 1, h));
+        const int blk = base + lane * WARPS, pg = max(page_of(kv, s.slot, blk), 0);
+        block_at[warp][lane] = block_ptr(kv, pg, blk, 0, h, HD);
+        sc0 = make_float2(__ldg(scale_ptr(kv, pg, blk, 0, h)), __ldg(scale_ptr(kv, pg, blk, 1, h)));
     }
+    __syncwarp();
     const int kpos = (g >> 1) * 4 + (g & 1);  // the lane's key rows: kpos and kpos + 2 (see the patches' position order)
-    const uint32_t mine = (uint32_t) __cvta_generic_to_shared(ring) + warp * (T::DEPTH * T::PIECES * 512) + lane * 16;
-    // blocks i, i + 1 of the warp into their slots; a block past the last is zeros
-    auto fetch = [&](int i) {
+    const long long v_at = (long long) kv.n_kv * kv.page_tokens * HD;
+    const uint32_t mine = (uint32_t) __cvta_generic_to_shared(ring) + warp * (T::AHEAD * 2 * T::PIECES * 512);
+    // where the lane's 16 bytes of 512 go: rows of 128 bytes have their halves swapped in every second row,
+    // which keeps the reading lanes on different banks
+    const int k_to = HD == 64 ? 16 * lane : (lane >> 3) * 128 + (((lane & 7) ^ ((lane >> 3 & 1) << 2)) << 4);
+    const int k_from = kpos * HD + 16 * t;
+    // keys, or values, of blocks i and i + 1 into the ring; a block past the last is zeros
+    auto fetch_k = [&](int i) {
 #pragma unroll
         for (int k2 = 0; k2 < 2; k2++) {
             const bool there = i + k2 < n;
-            const int pg = __shfl_sync(0xffffffffu, my_pg, (i + k2) & 31), blk = there ? base + (i + k2) * WARPS : c_lo;
-            const uint8_t * kp = block_ptr(kv, pg, blk, 0, h, HD) + kpos * HD + 16 * t;
-            const uint8_t * vp = block_ptr(kv, pg, blk, 1, h, HD) + 16 * lane;
-            const uint32_t slot = mine + (i + k2) % T::DEPTH * (T::PIECES * 512);
+            const uint8_t * p = block_at[warp][there ? i + k2 : 0] + 16 * lane;
+            const uint32_t slot = mine + (i / 2 % T::AHEAD * 2 + k2) * (T::PIECES * 512);
 #pragma unroll
-            for (int k = 0; k < T::KS; k++) {
-                copy16(slot + (2 * k) * 512, kp + 64 * k, there);
-                copy16(slot + (2 * k + 1) * 512, kp + 2 * HD + 64 * k, there);
-            }
-#pragma unroll
-            for (int j = 0; j < T::VS; j++) copy16(slot + (2 * T::KS + j) * 512, vp + 512 * j, there);
+            for (int k = 0; k < 2 * T::KS; k++) copy16(slot + 512 * k + k_to, p + 512 * k, there);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    auto fetch_v = [&](int i) {
 #pragma unroll
-    for (int i = 0; i < T::DEPTH - 2; i += 2) fetch(i);
+        for (int k2 = 0; k2 < 2; k2++) {
+            const bool there = i + k2 < n;
+            const uint8_t * p = block_at[warp][there ? i + k2 : 0] + v_at + 16 * lane;
+            const uint32_t slot = mine + (i / 2 % T::AHEAD * 2 + k2) * (T::PIECES * 512) + 2 * T::KS * 512 + 16 * lane;
+#pragma unroll
+            for (int j = 0; j < T::VS; j++) copy16(slot + 512 * j, p + 512 * j, there);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    if (n > 0) {
+#pragma unroll
+        for (int i = 0; i < T::AHEAD; i++) fetch_k(2 * i), fetch_v(2 * i);
+    }
+    if (lane < n) scales[warp][lane] = sc0;
+    for (int i = 32; i < n; i += 32) look_up(i + lane);
+    __syncwarp();
 
     // queries as the 8-column operand: lane (g, t) holds row 8 nt + g, elements 64 k + 16 t ..+15
     uint32_t qf[NT][T::KS][8];
@@ -503,33 +529,33 @@ __global__ void __launch_bounds__(32 * WARPS) kv8_attn_small_kernel(const AttnAr
     for (int nt = 0; nt < NT; nt++) m[nt][0] = m[nt][1] = -INFINITY;
 
     for (int i = 0; i < n; i += 2) {
-        // (always a group, empty past the end, so that the one waited for is the DEPTH / 2 - 1 st before)
-        if (i + T::DEPTH - 2 < n) fetch(i + T::DEPTH - 2);
-        else asm volatile("cp.async.commit_group;" ::: "memory");
-        asm volatile("cp.async.wait_group %0;" ::"n"(T::DEPTH / 2 - 1) : "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(2 * T::AHEAD - 1) : "memory");  // the keys
+        __syncwarp();
+        const uint32_t pair = mine + i / 2 % T::AHEAD * 2 * (T::PIECES * 512);
         float x[2][NT][4];  // columns 2t, 2t+1 at key kpos, then at key kpos + 2
         uint32_t seen[2][NT][2];  // (positions x rows) the rows that see each position, as f16 ones
         bool whole[2];
         float inv_vs[2];
 #pragma unroll
         for (int k2 = 0; k2 < 2; k2++) {
-            const uint32_t slot = mine + (i + k2) % T::DEPTH * (T::PIECES * 512);
-            float sc[NT][4] = {};
+            const uint32_t slot = pair + k2 * (T::PIECES * 512) + k_from;
+            float sc[NT][4] = {}, sd[NT][4] = {};  // (two sums: half as long a chain of MMAs)
 #pragma unroll
             for (int k = 0; k < T::KS; k++) {
-                const uint4 u0 = lds16(slot + (2 * k) * 512), u1 = lds16(slot + (2 * k + 1) * 512);
+                const int at = HD == 64 ? 0 : 64 * (k ^ (g & 1));
+                const uint4 u0 = lds16(slot + at), u1 = lds16(slot + 2 * HD + at);
                 const uint32_t w0[4] = { u0.x, u0.y, u0.z, u0.w }, w1[4] = { u1.x, u1.y, u1.z, u1.w };
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const uint32_t a0 = e4m3x2_to_h2((uint16_t) w0[j]), a2 = e4m3x2_to_h2((uint16_t) (w0[j] >> 16));
                     const uint32_t a1 = e4m3x2_to_h2((uint16_t) w1[j]), a3 = e4m3x2_to_h2((uint16_t) (w1[j] >> 16));
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) mma16816(sc[nt], a0, a1, a2, a3, qf[nt][k][2 * j], qf[nt][k][2 * j + 1]);
+                    for (int nt = 0; nt < NT; nt++) mma16816(j & 1 ? sd[nt] : sc[nt], a0, a1, a2, a3, qf[nt][k][2 * j], qf[nt][k][2 * j + 1]);
                 }
             }
-            const float ks = __shfl_sync(0xffffffffu, my_ks, (i + k2) & 31), vs = __shfl_sync(0xffffffffu, my_vs, (i + k2) & 31);
-            const int key0 = (base + (i + k2) * WARPS) << 4;  // (past the range: past every row's limit or masked below)
             const bool there = i + k2 < n;
+            const float ks = scales[warp][there ? i + k2 : 0].x, vs = scales[warp][there ? i + k2 : 0].y;
+            const int key0 = (base + (i + k2) * WARPS) << 4;
             const float ev = (float) exponent_of(vs);
             inv_vs[k2] = pow2f(-exponent_of(vs));
             whole[k2] = there && key0 >= full_lo && key0 + 16 <= full_hi;
@@ -537,7 +563,7 @@ __global__ void __launch_bounds__(32 * WARPS) kv8_attn_small_kernel(const AttnAr
             for (int nt = 0; nt < NT; nt++) {
                 const float c0 = coef[nt][0] * ks, c1 = coef[nt][1] * ks;
 #pragma unroll
-                for (int j = 0; j < 4; j++) x[k2][nt][j] = fmaf(sc[nt][j], j & 1 ? c1 : c0, ev);
+                for (int j = 0; j < 4; j++) x[k2][nt][j] = fmaf(sc[nt][j] + sd[nt][j], j & 1 ? c1 : c0, ev);
                 if (!whole[k2]) {
                     uint32_t one[4];
 #pragma unroll
@@ -552,6 +578,9 @@ __global__ void __launch_bounds__(32 * WARPS) kv8_attn_small_kernel(const AttnAr
                 }
             }
         }
+        // (also past the end, where it copies zeros: the waits count groups)
+        __syncwarp();
+        fetch_k(i + 2 * T::AHEAD);
         uint32_t wb[2][NT][2];
         bool moved = false;
         float corr[NT][2];
@@ -590,9 +619,11 @@ __global__ void __launch_bounds__(32 * WARPS) kv8_attn_small_kernel(const AttnAr
 #pragma unroll
                     for (int i2 = 0; i2 < 4; i2++) o[nt][j][i2] *= corr[nt][i2 & 1];
         }
+        asm volatile("cp.async.wait_group %0;" ::"n"(2 * T::AHEAD - 1) : "memory");  // the values
+        __syncwarp();
 #pragma unroll
         for (int k2 = 0; k2 < 2; k2++) {
-            const uint32_t slot = mine + (i + k2) % T::DEPTH * (T::PIECES * 512);
+            const uint32_t slot = pair + k2 * (T::PIECES * 512) + 16 * lane;
             uint4 vw[T::VS];
 #pragma unroll
             for (int j = 0; j < T::VS; j++) vw[j] = lds16(slot + (2 * T::KS + j) * 512);
@@ -644,6 +675,8 @@ __global__ void __launch_bounds__(32 * WARPS) kv8_attn_small_kernel(const AttnAr
                 }
             }
         }
+        __syncwarp();
+        fetch_v(i + 2 * T::AHEAD);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();  // the rings become the warps' outputs
@@ -859,12 +892,23 @@ Plan plan_of(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int c
     if (causal && window > 0) keys = std::min<long long>(keys, (long long) window + (p.rows + group - 1) / group + 1 + 15);
     const int blocks = (int) std::max<long long>(1, (keys + 15) / 16 + (window > 0 ? 1 : 0));
     const long long units = std::max<long long>(1, (long long) b.n_seq * c.n_kv * p.row_tiles);
-    // few-row kernel: enough CTAs for two waves of four per SM, at least eight blocks (two a warp) in each range;
-    // tile kernel: one CTA per SM, at least two tiles of 128 keys in each range
-    const long long want = std::max<long long>(1, (p.tile ? 148 : 148 * 8) / units);
-    p.chunk_blocks = (int) std::max<long long>(p.tile ? 16 : 8, (blocks + want - 1) / want);
-    if (p.tile) p.chunk_blocks = (p.chunk_blocks + 7) / 8 * 8;
-    else p.chunk_blocks = std::min(p.chunk_blocks, kSmallRange);
+    if (p.tile) {
+        // one CTA per SM, at least two tiles of 128 keys in each range
+        const long long want = std::max<long long>(1, 148 / units);
+        p.chunk_blocks = (int) std::max<long long>(16, (blocks + want - 1) / want);
+        p.chunk_blocks = (p.chunk_blocks + 7) / 8 * 8;
+    } else {
+        // ranges that fill whole waves of the CTAs an SM holds; a CTA's start and end cost about as much as
+        // 32 blocks
+        const long long slots = 148ll * small_ctas(c.head_dim, p.nt);
+        double best = 0;
+        for (int n = (blocks + kSmallRange - 1) / kSmallRange; n <= blocks; n++) {
+            const int size = (blocks + n - 1) / n;
+            const double cost = (double) ((units * n + slots - 1) / slots) * (size + 32);
+            if (best == 0 || cost < best) best = cost, p.chunk_blocks = size;
+            if (units * n >= 6 * slots || size <= 2 * kSmallWarps) break;
+        }
+    }
     p.chunks = (blocks + p.chunk_blocks - 1) / p.chunk_blocks;
     return p;
 }

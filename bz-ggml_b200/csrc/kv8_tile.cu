@@ -112,14 +112,14 @@ struct Work {
 
 __device__ __forceinline__ bool find_work(const AttnArgs & a, Work & w) {
     const Kv & kv = a.kv;
-    long long id = blockIdx.x;
-    w.h = (int) (id % kv.n_kv);
-    id /= kv.n_kv;
-    w.chunk = (int) (id % a.chunks);
-    id /= a.chunks;
+    unsigned id = blockIdx.x;
+    w.h = (int) (id % (unsigned) kv.n_kv);
+    id /= (unsigned) kv.n_kv;
+    w.chunk = (int) (id % (unsigned) a.chunks);
+    id /= (unsigned) a.chunks;
     // the last tiles of causal sequences have the most keys: they start first
-    w.b = (int) (id % kv.n_seq);
-    w.tile = a.row_tiles - 1 - (int) (id / kv.n_seq);
+    w.b = (int) (id % (unsigned) kv.n_seq);
+    w.tile = a.row_tiles - 1 - (int) (id / (unsigned) kv.n_seq);
     w.s = load_seq(kv, w.b);
     if (w.s.slot < 0) return false;
     w.rows = w.s.n * a.group;
