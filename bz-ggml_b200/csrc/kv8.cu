@@ -871,12 +871,17 @@ struct Plan {
     int row_tiles = 1, chunks = 1, chunk_blocks = 1;
 };
 constexpr int kFewRows = 32;
+// (sequence, row tile, kv head) units that may be split: their counters lie at a fixed place of the workspace, so
+// that calls of different shapes can share one
+constexpr long long kSplitUnits = 1 << 16;
+constexpr long long kCounterBytes = kSplitUnits * 4;
 
 Plan plan_of(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int causal, int window) {
     Plan p;
     const int group = n_head / c.n_kv;
     const long long rows = (long long) b.max_new * group;
-    p.tile = rows > kFewRows;
+    // (a range of the few-row kernel is limited; without splitting it could not reach longer contexts)
+    p.tile = rows > kFewRows || (b.max_len > 16 * kSmallRange && (long long) b.n_seq * c.n_kv * 4 > kSplitUnits);
     if (p.tile) {
         p.rows = kTileRows;
     } else {
@@ -892,7 +897,9 @@ Plan plan_of(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int c
     if (causal && window > 0) keys = std::min<long long>(keys, (long long) window + (p.rows + group - 1) / group + 1 + 15);
     const int blocks = (int) std::max<long long>(1, (keys + 15) / 16 + (window > 0 ? 1 : 0));
     const long long units = std::max<long long>(1, (long long) b.n_seq * c.n_kv * p.row_tiles);
-    if (p.tile) {
+    if (units > kSplitUnits) {
+        p.chunk_blocks = (blocks + 7) / 8 * 8;
+    } else if (p.tile) {
         // one CTA per SM, at least two tiles of 128 keys in each range
         const long long want = std::max<long long>(1, 148 / units);
         p.chunk_blocks = (int) std::max<long long>(16, (blocks + want - 1) / want);
@@ -912,8 +919,6 @@ Plan plan_of(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int c
     p.chunks = (blocks + p.chunk_blocks - 1) / p.chunk_blocks;
     return p;
 }
-
-long long counter_bytes(long long units) { return (units * 4 + 15) / 16 * 16; }
 
 template <int HD, int NT>
 void run_small(const AttnArgs & a, cudaStream_t s) {
@@ -1010,7 +1015,7 @@ long long kv8_attention_workspace(const bzb_kv8_cache & c, const bzb_kv8_batch &
     const Plan p = plan_of(c, b, n_head, causal, window);
     if (p.chunks == 1) return 0;
     const long long units = (long long) b.n_seq * p.row_tiles * c.n_kv;
-    return counter_bytes(units) + units * p.chunks * p.rows * (c.head_dim + 4) * 4;
+    return kCounterBytes + units * p.chunks * p.rows * (c.head_dim + 4) * 4;
 }
 
 void kv8_attention(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_kv8_rows & q, const bzb_kv8_rows & out,
@@ -1045,8 +1050,7 @@ void kv8_attention(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_k
     a.chunks = p.chunks;
     a.chunk_blocks = p.chunk_blocks;
     a.counters = static_cast<int *>(workspace);
-    a.part = need > 0 ? reinterpret_cast<float *>(static_cast<char *>(workspace) +
-                                                  counter_bytes((long long) b.n_seq * p.row_tiles * c.n_kv)) : nullptr;
+    a.part = need > 0 ? reinterpret_cast<float *>(static_cast<char *>(workspace) + kCounterBytes) : nullptr;
     if (p.tile) {
         launch_attn_tile(a, c.head_dim, s);
     } else if (c.head_dim == 64) {

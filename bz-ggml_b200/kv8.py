@@ -8,7 +8,7 @@ workspace, which a batch allocates at its first use on a stream.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional
+import os
 
 from . import lib
 
@@ -23,16 +23,29 @@ class _Cache(ctypes.Structure):
 
 class _Batch(ctypes.Structure):
     _fields_ = [("q_start", _p), ("kv_len", _p), ("slots", _p), ("n_seq", _i), ("n_tok", _i), ("max_new", _i),
-                ("max_len", _i)]
+                ("max_len", _i), ("device", _i)]  # (the device is for csrc/kv8_torch.cpp, behind the C struct)
 
 
-class _Rows(ctypes.Structure):
-    _fields_ = [("data", _p), ("row_stride", _ll), ("head_stride", _ll), ("n_head", _i), ("type", _i)]
+_EXT = None
 
 
-_TYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
-_TYPE_OF: dict = {}  # torch dtype -> bzb type
-_null = ctypes.c_void_p()
+def _ext(library):
+    """The compiled PyTorch side of the calls (csrc/kv8_torch.cpp), bound to the loaded libbreeze.so."""
+    global _EXT
+    if _EXT is None:
+        import importlib.util
+        import torch  # noqa: F401  (its libraries must be loaded first)
+        path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_kv8_torch.so")
+        if not os.path.exists(path):
+            raise FileNotFoundError(f"_kv8_torch.so not found at {path}; run `make -C {os.path.dirname(path)}`")
+        spec = importlib.util.spec_from_file_location("_kv8_torch", path)
+        ext = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(ext)
+        at = lambda name: ctypes.cast(getattr(library.lib, name), ctypes.c_void_p).value  # noqa: E731
+        ext.bind(at("bzb_kv8_append"), at("bzb_kv8_read"), at("bzb_kv8_attention"), at("bzb_kv8_attention_workspace"),
+                 at("breeze_last_error"))
+        _EXT = ext
+    return _EXT
 
 
 def _check(t, name: str, dtype: str, dims: int, device: int, contiguous: bool = True) -> None:
@@ -62,9 +75,9 @@ class KV8Batch:
         self.device, self.n_tok = dev, int(n_tok)
         self._held = (q_start, kv_len, slots)
         self._c = _Batch(q_start.data_ptr(), kv_len.data_ptr(), None if slots is None else slots.data_ptr(), n, n_tok,
-                         max_new, max_len)
-        self._ref = ctypes.byref(self._c)
-        self._workspaces: dict = {}
+                         max_new, max_len, dev)
+        self._at = ctypes.addressof(self._c)
+        self._workspaces: dict = {}  # attention's, one for each stream and size
 
 
 class KV8Cache:
@@ -87,83 +100,31 @@ class KV8Cache:
             raise ValueError("pages and scales must be contiguous within a page")
         self.device, self.n_kv, self.head_dim, self.page_tokens = dev, n_kv, hd, page_tokens
         self.status = torch.zeros(1, dtype=torch.int32, device=pages.device)
-        self._stream = torch.cuda.current_stream
         self._held = (pages, scales, page_table)
         one = n_pages == 1  # (a single page's stride says nothing)
         self._c = _Cache(pages.data_ptr(), scales.data_ptr(), page_table.data_ptr(), self.status.data_ptr(),
                          2 * n_kv * page_tokens * hd if one else pages.stride(0),
                          2 * n_kv * (page_tokens // 16) if one else scales.stride(0), n_pages, page_table.shape[0],
                          page_table.shape[1], page_tokens, n_kv, hd, dev)
-        self._ref = ctypes.byref(self._c)
-        self._lib = lib()
-        self._append, self._read = self._lib.lib.bzb_kv8_append, self._lib.lib.bzb_kv8_read
-        self._attention, self._space = self._lib.lib.bzb_kv8_attention, self._lib.lib.bzb_kv8_attention_workspace
-
-    def _rows(self, t, name: str, batch: KV8Batch) -> _Rows:
-        shape = t.shape
-        if len(shape) != 3 or shape[0] != batch.n_tok or shape[2] != self.head_dim:
-            raise ValueError(f"{name}: [{batch.n_tok}, heads, {self.head_dim}] expected, got {tuple(shape)}")
-        row, head, unit = t.stride()
-        if unit != 1 or t.get_device() != self.device:
-            raise ValueError(f"{name}: contiguous heads on cuda:{self.device} expected")
-        dtype = t.dtype
-        kind = _TYPE_OF.get(dtype)
-        if kind is None:
-            kind = _TYPE_OF.setdefault(dtype, _TYPES.get(str(dtype), -1))
-        return _Rows(t.data_ptr(), row, head, shape[1], kind)
-
-    def _vector(self, t, name: str, shape: tuple):
-        if t is None:
-            return None
-        if tuple(t.shape) != shape or str(t.dtype) != "torch.float32" or t.get_device() != self.device or not t.is_contiguous():
-            raise ValueError(f"{name}: contiguous float32 {shape} on cuda:{self.device} expected")
-        return t.data_ptr()
-
-    def _done(self, rc: int) -> None:
-        if rc < 0:
-            raise RuntimeError(self._lib.last_error())
+        self._at = ctypes.addressof(self._c)
+        ext = _ext(lib())
+        self._append, self._read, self._attention = ext.append, ext.read, ext.attention
 
     def append(self, batch: KV8Batch, q, k, v, q_out, q_norm=None, k_norm=None, eps: float = 1e-6, rope=None) -> None:
         """Norms (q_norm / k_norm [head_dim] f32) and rotates (rope [positions, head_dim / 2, 2] f32: cos,
         sin) the batch's queries q [n_tok, n_head, head_dim] into q_out and its keys k [n_tok, n_kv,
         head_dim], and appends the keys and the values v. q and q_out may both be None."""
-        hd = self.head_dim
-        rk, rv = self._rows(k, "k", batch), self._rows(v, "v", batch)
-        rq = None if q is None else ctypes.byref(self._rows(q, "q", batch))
-        ro = None if q_out is None else ctypes.byref(self._rows(q_out, "q_out", batch))
-        wq, wk = self._vector(q_norm, "q_norm", (hd,)), self._vector(k_norm, "k_norm", (hd,))
-        n = 0 if rope is None else rope.shape[0]
-        self._done(self._append(self._ref, batch._ref, rq, ctypes.byref(rk), ctypes.byref(rv), ro, wq, wk, eps,
-                                self._vector(rope, "rope", (n, hd // 2, 2)), n, self._stream(self.device).cuda_stream))
+        self._append(self._at, batch._at, q, k, v, q_out, q_norm, k_norm, eps, rope)
 
     def read(self, batch: KV8Batch, k_out, v_out) -> None:
         """The batch's positions back as rows k_out, v_out [n_tok, n_kv, head_dim] (f32, f16 or bf16)."""
-        rk, rv = self._rows(k_out, "k_out", batch), self._rows(v_out, "v_out", batch)
-        self._done(self._read(self._ref, batch._ref, ctypes.byref(rk), ctypes.byref(rv),
-                              self._stream(self.device).cuda_stream))
+        self._read(self._at, batch._at, k_out, v_out)
 
     def attention(self, batch: KV8Batch, q, out, scale: float, causal: bool = True, window: int = 0, lse=None) -> None:
         """out [n_tok, n_head, head_dim] = softmax(scale q k^T) v over each row's cached keys (those up to
         its own position when causal, of them the last `window` when that is positive); lse [n_tok, n_head]
         f32, when given, gets the rows' log-sum-exp."""
-        rq, ro = self._rows(q, "q", batch), self._rows(out, "out", batch)
-        stream = self._stream(self.device).cuda_stream
-        key = (self, stream, rq.n_head, causal, window)
-        space = batch._workspaces.get(key)
-        if space is None:
-            space = batch._workspaces[key] = self._workspace(batch, rq.n_head, causal, window)
-        self._done(self._attention(self._ref, batch._ref, ctypes.byref(rq), ctypes.byref(ro),
-                                   None if lse is None else self._vector(lse, "lse", (batch.n_tok, rq.n_head)), scale,
-                                   causal, window, space[0], space[1], stream))
-
-    def _workspace(self, batch: KV8Batch, n_head: int, causal: bool, window: int):
-        import torch
-        n = self._space(self._ref, batch._ref, n_head, causal, window)
-        self._done(int(min(n, 0)))
-        if n == 0:
-            return None, 0, None
-        t = torch.zeros(n, dtype=torch.uint8, device=f"cuda:{self.device}")
-        return t.data_ptr(), n, t
+        self._attention(self._at, batch._at, batch._workspaces, q, out, scale, causal, window, lse)
 
     def check(self) -> None:
         """Waits for the device and raises if a call met a page, slot or length out of range since the last check."""
