@@ -81,6 +81,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 5) kv8_append_kernel(const App
     const Kv & kv = a.kv;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane % R::LPR;
     const int r0 = warp % R::WPB * (16 / R::WPB) + lane / R::LPR * 4;  // the lane's first row of the block
+    start_after_previous();
     const Seq s = load_seq(kv, (int) blockIdx.z);
     if (s.slot < 0) return;
     const int first = s.len - s.n;  // position of the sequence's first row (negative: padding rows)
@@ -263,6 +264,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) kv8_read_kernel(const ReadArgs
     const Kv & kv = a.kv;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane % R::LPR;
     const int r0 = warp % R::WPB * (16 / R::WPB) + lane / R::LPR * 4;
+    start_after_previous();
     const Seq s = load_seq(kv, (int) blockIdx.z);
     if (s.slot < 0 || s.n == 0) return;
     // blocks count from the first row's position; `first` may be negative (padding rows, read as zeros)
@@ -415,6 +417,7 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, NT)) kv8_attn_small
     const int chunk = (int) (id % (unsigned) a.chunks);
     id /= (unsigned) a.chunks;
     const int tile = (int) (id % (unsigned) a.row_tiles), b = (int) (id / (unsigned) a.row_tiles);
+    start_after_previous();
     const Seq s = load_seq(kv, b);
     if (s.slot < 0) return;
     const int rows = s.n * a.group, row0 = tile * T::ROWS;
@@ -766,10 +769,6 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, NT)) kv8_attn_small
 
 // ---- host side ----
 
-void check_cuda(cudaError_t e, const char * what) {
-    if (e != cudaSuccess) throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(e));
-}
-
 void fail(const std::string & what) { throw std::runtime_error(what); }
 
 Kv view(const bzb_kv8_cache & c, const bzb_kv8_batch & b) {
@@ -851,16 +850,13 @@ dim3 row_grid(const Kv & kv, int heads, int per_cta) {
 template <int HD, int TYPE>
 void run_append(const AppendArgs & a, bool vec, cudaStream_t s) {
     const dim3 grid = row_grid(a.kv, a.n_head + 2 * a.kv.n_kv, RowMap<HD>::HEADS);
-    if (vec) kv8_append_kernel<HD, TYPE, true><<<grid, 32 * kRowWarps, 0, s>>>(a);
-    else kv8_append_kernel<HD, TYPE, false><<<grid, 32 * kRowWarps, 0, s>>>(a);
-    check_cuda(cudaGetLastError(), "launch");
+    launch_chained(vec ? kv8_append_kernel<HD, TYPE, true> : kv8_append_kernel<HD, TYPE, false>, grid, 32 * kRowWarps, 0, s, a);
 }
 
 template <int HD, int TYPE>
 void run_read(const ReadArgs & a, cudaStream_t s) {
     const dim3 grid = row_grid(a.kv, 2 * a.kv.n_kv, RowMap<HD>::HEADS);
-    kv8_read_kernel<HD, TYPE><<<grid, 32 * kRowWarps, 0, s>>>(a);
-    check_cuda(cudaGetLastError(), "launch");
+    launch_chained(kv8_read_kernel<HD, TYPE>, grid, 32 * kRowWarps, 0, s, a);
 }
 
 // How the rows and the cache of a call are cut up.
@@ -905,13 +901,13 @@ Plan plan_of(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int c
         p.chunk_blocks = (int) std::max<long long>(16, (blocks + want - 1) / want);
         p.chunk_blocks = (p.chunk_blocks + 7) / 8 * 8;
     } else {
-        // ranges that fill whole waves of the CTAs an SM holds; a CTA's start and end cost about as much as
-        // 32 blocks
+        // ranges that fill whole waves of the CTAs an SM holds; a CTA's start and end cost about as much time as
+        // 32 blocks, joining the ranges as much as 24 more
         const long long slots = 148ll * small_ctas(c.head_dim, p.nt);
         double best = 0;
         for (int n = (blocks + kSmallRange - 1) / kSmallRange; n <= blocks; n++) {
             const int size = (blocks + n - 1) / n;
-            const double cost = (double) ((units * n + slots - 1) / slots) * (size + 32);
+            const double cost = (double) ((units * n + slots - 1) / slots) * (size + 32) + (n > 1 ? 24 : 0);
             if (best == 0 || cost < best) best = cost, p.chunk_blocks = size;
             if (units * n >= 6 * slots || size <= 2 * kSmallWarps) break;
         }
@@ -926,8 +922,7 @@ void run_small(const AttnArgs & a, cudaStream_t s) {
     constexpr int bytes = SmallTile<HD, NT, kSmallWarps>::BYTES;
     static std::atomic<uint64_t> ready{ 0 };
     allow_shared_memory(kv8_attn_small_kernel<HD, NT, kSmallWarps>, bytes, ready);
-    kv8_attn_small_kernel<HD, NT, kSmallWarps><<<grid, 32 * kSmallWarps, bytes, s>>>(a);
-    check_cuda(cudaGetLastError(), "launch");
+    launch_chained(kv8_attn_small_kernel<HD, NT, kSmallWarps>, dim3(grid), 32 * kSmallWarps, bytes, s, a);
 }
 
 void check_attention(const bzb_kv8_cache & c, int n_head, int causal, int window) {

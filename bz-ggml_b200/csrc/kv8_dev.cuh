@@ -17,6 +17,7 @@
 #include <cstdint>
 #include <stdexcept>
 #include <string>
+#include <utility>
 
 namespace bzb {
 namespace kv8 {
@@ -204,6 +205,29 @@ void allow_shared_memory(K kernel, int bytes, std::atomic<uint64_t> & ready) {
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) throw std::runtime_error(std::string("shared memory: ") + cudaGetErrorString(e));
     ready.fetch_or(bit, std::memory_order_release);
+}
+
+// Launches with programmatic dependent launch: the kernel's CTAs may take their places while the kernel before it in
+// the stream still runs, and begin each with start_after_previous(), before which they touch no memory.
+template <typename... P, typename... A>
+void launch_chained(void (*kernel)(P...), dim3 grid, int threads, int shared, cudaStream_t s, A &&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = shared;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
+    if (e != cudaSuccess) throw std::runtime_error(std::string("launch: ") + cudaGetErrorString(e));
+}
+// lets the next kernel's CTAs be placed, then waits until the kernels before this one are done and their writes visible
+__device__ __forceinline__ void start_after_previous() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // the attention of many rows (kv8_tile.cu): rows of a kv head in tiles of kTileRows

@@ -327,6 +327,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
     using M = Smem<HD>;
     extern __shared__ uint8_t raw[];
     __shared__ Shared sh;
+    start_after_previous();
     Work w;
     if (!find_work(a, w)) return;  // (the whole CTA)
     uint8_t * base = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
@@ -679,9 +680,7 @@ void launch(const AttnArgs & a, cudaStream_t s) {
             throw std::runtime_error("kv8_attn_tile_kernel: built with another register count than its split needs");
     }
     allow_shared_memory(kv8_attn_tile_kernel<HD>, (int) Smem<HD>::kBytes, ready);
-    kv8_attn_tile_kernel<HD><<<(unsigned) grid, kTileThreads, Smem<HD>::kBytes, s>>>(a);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) throw std::runtime_error(std::string("launch: ") + cudaGetErrorString(e));
+    launch_chained(kv8_attn_tile_kernel<HD>, dim3((unsigned) grid), kTileThreads, (int) Smem<HD>::kBytes, s, a);
 }
 
 }  // namespace
