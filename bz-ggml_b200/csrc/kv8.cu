@@ -367,29 +367,31 @@ __device__ __forceinline__ void load_q16(const AttnArgs & a, long long i, float 
 }
 
 // Few query rows (a step of each sequence, or a few guessed tokens): one CTA per (sequence, kv head, tile
-// of 8 NT query rows, range of the cache), its warps taking the range's blocks in turn, two at a time. The rows
-// of a kv head are (token, head of the group) pairs, so a block read once serves the whole group.
+// of rows, range of the cache), taking two blocks of 16 positions at a time. The rows of a kv head are (token,
+// head of the group) pairs, so a block read once serves the whole group. Up to 8 rows: the warps share out
+// the range's blocks, each with a ring of its own, and join their results (SHARED false). More: each warp has
+// 8 of the rows and all read every block from one ring (SHARED true).
 //
 // The matrix products are m16n8k16 with the cache as the 16-row operand: S^T = K Q^T (16 positions x 8
 // rows) and O^T = V^T W^T (16 of head_dim x 8 rows): no half of a tile is empty when a group has at
 // most 8 rows. A lane's 16 bytes of a key row are the four k-steps' values of head_dim for it (the queries are
 // read in the same order, and any order of the sum's terms will do), and the value patches are stored in operand
-// order: no transposition but the 8x8 one of the weights. Each warp copies its blocks by itself, as they lie in
-// memory (cp.async), AHEAD pairs of blocks in advance: a pair's keys are copied as soon as the scores are
-// done with the pair before it in the ring, its values after the second product.
-// CTAs that an SM holds, by their registers
-constexpr int small_ctas(int hd, int nt) { return hd == 64 ? (nt == 1 ? 5 : nt == 2 ? 3 : 2) : (nt == 1 ? 4 : 2); }
+// order: no transposition but the 8x8 one of the weights. The blocks are copied as they lie in memory
+// (cp.async), AHEAD pairs in advance: a pair's keys as soon as the scores are done with the pair that had
+// their place, its values after the second product.
+constexpr int kSmallBlocks = 512;  // blocks of a range at most
 
-template <int HD, int NT, int WARPS>
+// CTAs that an SM holds, by their registers (96 and 128 a thread)
+constexpr int small_ctas(int hd, int warps) { return (hd == 64 ? 20 : 16) / warps; }
+
+template <int HD, int WARPS, bool SHARED>
 struct SmallTile {
-    static constexpr int ROWS = 8 * NT, KS = HD / 64, VS = HD / 32, MT = HD / 16, PL = HD + 4;
-    static constexpr int PIECES = 2 * KS + VS;            // 16-byte pieces of a block for each lane
-    static constexpr int AHEAD = HD == 64 ? 2 : 1;   // pairs of blocks that a warp's ring holds
-    static constexpr int RING = WARPS * AHEAD * 2 * PIECES * 512, MERGE = WARPS * ROWS * (HD + 4) * 4;
+    static constexpr int ROWS = SHARED ? 8 * WARPS : 8, KS = HD / 64, VS = HD / 32, MT = HD / 16, PL = HD + 4;
+    static constexpr int PIECES = 2 * KS + VS;            // 512-byte pieces of a block
+    static constexpr int AHEAD = SHARED ? 4 : HD == 64 ? 2 : 1;  // pairs of blocks that a ring holds
+    static constexpr int RING = (SHARED ? 1 : WARPS) * AHEAD * 2 * PIECES * 512, MERGE = WARPS * 8 * (HD + 4) * 4;
     static constexpr int BYTES = RING > MERGE ? RING : MERGE;
 };
-constexpr int kSmallWarps = 4, kSmallBlocks = 128;
-constexpr int kSmallRange = kSmallBlocks * kSmallWarps;  // blocks of a range at most
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void * src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
@@ -400,14 +402,16 @@ __device__ __forceinline__ uint4 lds16(uint32_t a) {
     return v;
 }
 
-template <int HD, int NT, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, NT)) kv8_attn_small_kernel(const AttnArgs a) {
-    using T = SmallTile<HD, NT, WARPS>;
+template <int HD, int WARPS, bool SHARED>
+__global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, WARPS)) kv8_attn_small_kernel(const AttnArgs a) {
+    using T = SmallTile<HD, WARPS, SHARED>;
+    constexpr int NT = 1;  // tiles of 8 rows of a warp
+    constexpr int STRIDE = SHARED ? 1 : WARPS;  // between the blocks of a warp
     extern __shared__ __align__(16) uint8_t ring[];
-    __shared__ float sm_ml[WARPS][T::ROWS][2];
-    // the blocks of a warp's range: the head's keys (its values lie one plane on), the scales of both
-    __shared__ const uint8_t * block_at[WARPS][kSmallBlocks];
-    __shared__ float2 scales[WARPS][kSmallBlocks];
+    __shared__ float sm_ml[WARPS][8][2];
+    // the range's blocks: the head's keys (its values lie one plane on), the scales of both
+    __shared__ const uint8_t * block_at[kSmallBlocks];
+    __shared__ float2 scales[kSmallBlocks];
     const Kv & kv = a.kv;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     // (heads fastest: neighbouring CTAs read neighbouring bytes of the same pages)
@@ -427,66 +431,68 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, NT)) kv8_attn_small
     // the keys that any row of the tile looks at: [key_lo, key_hi)
     const int key_hi = max(0, a.causal ? pos_hi + 1 : s.len);
     const int key_lo = a.window > 0 ? max(0, pos_lo - a.window + 1) : 0;
-    // every row sees [full_lo, full_hi)
-    const int full_hi = a.causal ? pos_lo + 1 : s.len, full_lo = a.window > 0 ? max(0, pos_hi - a.window + 1) : 0;
+    // this warp's rows, and the keys that all of them see: [full_lo, full_hi)
+    const int wrow0 = row0 + (SHARED ? 8 * warp : 0), last_row = max(wrow0, min(rows - 1, wrow0 + 7));
+    const int full_hi = a.causal ? first + wrow0 / a.group + 1 : s.len;
+    const int full_lo = a.window > 0 ? max(0, first + last_row / a.group - a.window + 1) : 0;
     const int blk_lo = key_lo >> 4, blk_hi = (key_hi + 15) >> 4;
     const int my_chunks = max(1, (blk_hi - blk_lo + a.chunk_blocks - 1) / a.chunk_blocks);
     if (chunk >= my_chunks) return;
     const int c_lo = blk_lo + chunk * a.chunk_blocks, c_hi = min(blk_hi, c_lo + a.chunk_blocks);
 
-    // this warp's blocks: base, base + WARPS, ...
-    const int base = c_lo + warp, n = max(0, (c_hi - base + WARPS - 1) / WARPS);
-    auto look_up = [&](int i) {
-        if (i >= n) return;
-        const int blk = base + i * WARPS, pg = max(page_of(kv, s.slot, blk), 0);
-        block_at[warp][i] = block_ptr(kv, pg, blk, 0, h, HD);
-        scales[warp][i] = make_float2(__ldg(scale_ptr(kv, pg, blk, 0, h)), __ldg(scale_ptr(kv, pg, blk, 1, h)));
+    // this warp's blocks: base, base + STRIDE, ..., looked up by itself (SHARED: by the whole CTA)
+    const int base = c_lo + (SHARED ? 0 : warp), n = max(0, (c_hi - base + STRIDE - 1) / STRIDE);
+    auto sync = [] {
+        if (SHARED) __syncthreads();
+        else __syncwarp();
     };
+    constexpr int FINDERS = SHARED ? 32 * WARPS : 32;
+    const int me = SHARED ? (int) threadIdx.x : lane, mine0 = SHARED ? 0 : warp * (kSmallBlocks / WARPS);
     // (the first blocks' copies do not wait for their scales)
     float2 sc0 = make_float2(0.0f, 0.0f);
-    if (lane < n) {
-        const int blk = base + lane * WARPS, pg = max(page_of(kv, s.slot, blk), 0);
-        block_at[warp][lane] = block_ptr(kv, pg, blk, 0, h, HD);
+    if (me < n) {
+        const int blk = base + me * STRIDE, pg = max(page_of(kv, s.slot, blk), 0);
+        block_at[mine0 + me] = block_ptr(kv, pg, blk, 0, h, HD);
         sc0 = make_float2(__ldg(scale_ptr(kv, pg, blk, 0, h)), __ldg(scale_ptr(kv, pg, blk, 1, h)));
     }
-    __syncwarp();
+    sync();
     const int kpos = (g >> 1) * 4 + (g & 1);  // the lane's key rows: kpos and kpos + 2 (see the patches' position order)
     const long long v_at = (long long) kv.n_kv * kv.page_tokens * HD;
-    const uint32_t mine = (uint32_t) __cvta_generic_to_shared(ring) + warp * (T::AHEAD * 2 * T::PIECES * 512);
+    const uint32_t slots = (uint32_t) __cvta_generic_to_shared(ring) + (SHARED ? 0 : warp) * (T::AHEAD * 2 * T::PIECES * 512);
     // where the lane's 16 bytes of 512 go: rows of 128 bytes have their halves swapped in every second row,
     // which keeps the reading lanes on different banks
     const int k_to = HD == 64 ? 16 * lane : (lane >> 3) * 128 + (((lane & 7) ^ ((lane >> 3 & 1) << 2)) << 4);
     const int k_from = kpos * HD + 16 * t;
     // keys, or values, of blocks i and i + 1 into the ring; a block past the last is zeros
-    auto fetch_k = [&](int i) {
+    auto fetch = [&](int i, bool values) {
+        constexpr int PK = 2 * T::KS;
+        const uint32_t slot = slots + i / 2 % T::AHEAD * 2 * (T::PIECES * 512);
 #pragma unroll
-        for (int k2 = 0; k2 < 2; k2++) {
+        for (int x = 0; x < 2 * (PK > T::VS ? PK : T::VS); x++) {
+            const int per = values ? T::VS : PK, k2 = x / per, k = x % per;
+            if (k2 > 1 || (SHARED && x % WARPS != warp)) continue;
             const bool there = i + k2 < n;
-            const uint8_t * p = block_at[warp][there ? i + k2 : 0] + 16 * lane;
-            const uint32_t slot = mine + (i / 2 % T::AHEAD * 2 + k2) * (T::PIECES * 512);
-#pragma unroll
-            for (int k = 0; k < 2 * T::KS; k++) copy16(slot + 512 * k + k_to, p + 512 * k, there);
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    auto fetch_v = [&](int i) {
-#pragma unroll
-        for (int k2 = 0; k2 < 2; k2++) {
-            const bool there = i + k2 < n;
-            const uint8_t * p = block_at[warp][there ? i + k2 : 0] + v_at + 16 * lane;
-            const uint32_t slot = mine + (i / 2 % T::AHEAD * 2 + k2) * (T::PIECES * 512) + 2 * T::KS * 512 + 16 * lane;
-#pragma unroll
-            for (int j = 0; j < T::VS; j++) copy16(slot + 512 * j, p + 512 * j, there);
+            const uint8_t * p = block_at[mine0 + (there ? i + k2 : 0)] + 16 * lane + 512 * k;
+            if (values) copy16(slot + (k2 * T::PIECES + PK + k) * 512 + 16 * lane, p + v_at, there);
+            else copy16(slot + (k2 * T::PIECES + k) * 512 + k_to, p, there);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     if (n > 0) {
 #pragma unroll
-        for (int i = 0; i < T::AHEAD; i++) fetch_k(2 * i), fetch_v(2 * i);
+        for (int i = 0; i < T::AHEAD; i++) {
+            // (a range's first 32 blocks, or more, are in the table by now)
+            fetch(2 * i, false);
+            fetch(2 * i, true);
+        }
     }
-    if (lane < n) scales[warp][lane] = sc0;
-    for (int i = 32; i < n; i += 32) look_up(i + lane);
-    __syncwarp();
+    if (me < n) scales[mine0 + me] = sc0;
+    for (int i = me + FINDERS; i < n; i += FINDERS) {
+        const int blk = base + i * STRIDE, pg = max(page_of(kv, s.slot, blk), 0);
+        block_at[mine0 + i] = block_ptr(kv, pg, blk, 0, h, HD);
+        scales[mine0 + i] = make_float2(__ldg(scale_ptr(kv, pg, blk, 0, h)), __ldg(scale_ptr(kv, pg, blk, 1, h)));
+    }
+    sync();
 
     // queries as the 8-column operand: lane (g, t) holds row 8 nt + g, elements 64 k + 16 t ..+15
     uint32_t qf[NT][T::KS][8];
@@ -494,7 +500,7 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, NT)) kv8_attn_small
     int lim_hi[NT][2], lim_lo[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-        const int r = row0 + 8 * nt + g;
+        const int r = wrow0 + 8 * nt + g;
         float unit = 1.0f;
         if (r < rows) {
             const long long at = (long long) (s.row0 + r / a.group) * a.q.row + (h * a.group + r % a.group) * a.q.head + 16 * t;
@@ -520,7 +526,7 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, NT)) kv8_attn_small
         }
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            const int rr = row0 + 8 * nt + 2 * t + i, pos = first + rr / a.group;
+            const int rr = wrow0 + 8 * nt + 2 * t + i, pos = first + rr / a.group;
             coef[nt][i] = a.scale2 * __shfl_sync(0xffffffffu, unit, (2 * t + i) * 4);
             lim_hi[nt][i] = rr < rows ? (a.causal ? pos + 1 : s.len) : 0;
             lim_lo[nt][i] = a.window > 0 ? pos - a.window + 1 : 0;
@@ -533,8 +539,8 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, NT)) kv8_attn_small
 
     for (int i = 0; i < n; i += 2) {
         asm volatile("cp.async.wait_group %0;" ::"n"(2 * T::AHEAD - 1) : "memory");  // the keys
-        __syncwarp();
-        const uint32_t pair = mine + i / 2 % T::AHEAD * 2 * (T::PIECES * 512);
+        sync();
+        const uint32_t pair = slots + i / 2 % T::AHEAD * 2 * (T::PIECES * 512);
         float x[2][NT][4];  // columns 2t, 2t+1 at key kpos, then at key kpos + 2
         uint32_t seen[2][NT][2];  // (positions x rows) the rows that see each position, as f16 ones
         bool whole[2];
@@ -557,8 +563,9 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, NT)) kv8_attn_small
                 }
             }
             const bool there = i + k2 < n;
-            const float ks = scales[warp][there ? i + k2 : 0].x, vs = scales[warp][there ? i + k2 : 0].y;
-            const int key0 = (base + (i + k2) * WARPS) << 4;
+            const float2 kvs = scales[mine0 + (there ? i + k2 : 0)];
+            const float ks = kvs.x, vs = kvs.y;
+            const int key0 = (base + (i + k2) * STRIDE) << 4;
             const float ev = (float) exponent_of(vs);
             inv_vs[k2] = pow2f(-exponent_of(vs));
             whole[k2] = there && key0 >= full_lo && key0 + 16 <= full_hi;
@@ -582,8 +589,8 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, NT)) kv8_attn_small
             }
         }
         // (also past the end, where it copies zeros: the waits count groups)
-        __syncwarp();
-        fetch_k(i + 2 * T::AHEAD);
+        sync();
+        fetch(i + 2 * T::AHEAD, false);
         uint32_t wb[2][NT][2];
         bool moved = false;
         float corr[NT][2];
@@ -623,7 +630,7 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, NT)) kv8_attn_small
                     for (int i2 = 0; i2 < 4; i2++) o[nt][j][i2] *= corr[nt][i2 & 1];
         }
         asm volatile("cp.async.wait_group %0;" ::"n"(2 * T::AHEAD - 1) : "memory");  // the values
-        __syncwarp();
+        sync();
 #pragma unroll
         for (int k2 = 0; k2 < 2; k2++) {
             const uint32_t slot = pair + k2 * (T::PIECES * 512) + 16 * lane;
@@ -678,12 +685,12 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, NT)) kv8_attn_small
                 }
             }
         }
-        __syncwarp();
-        fetch_v(i + 2 * T::AHEAD);
+        sync();
+        fetch(i + 2 * T::AHEAD, true);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();  // the rings become the warps' outputs
-    float (*sm_o)[T::ROWS][HD + 4] = reinterpret_cast<float (*)[T::ROWS][HD + 4]>(ring);
+    float (*sm_o)[8][HD + 4] = reinterpret_cast<float (*)[8][HD + 4]>(ring);
 
     // the warps' states to shared memory: [row][element]; element of (mt, half, g): 32 (mt/2) + 4 g + 2 (mt%2) + half
 #pragma unroll
@@ -717,16 +724,21 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, NT)) kv8_attn_small
     for (int i = threadIdx.x; i < live * (HD / 4); i += 32 * WARPS) {
         const int r = i / (HD / 4), d = i % (HD / 4) * 4;
         float mm = -INFINITY, ll = 0.0f;
-#pragma unroll
-        for (int w = 0; w < WARPS; w++) mm = fmaxf(mm, sm_ml[w][r][0]);
-        const float ref = mm == -INFINITY ? 0.0f : mm;
         float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (SHARED) {
+            mm = sm_ml[r >> 3][r & 7][0], ll = sm_ml[r >> 3][r & 7][1];
+            x = *reinterpret_cast<const float4 *>(&sm_o[r >> 3][r & 7][d]);
+        } else {
 #pragma unroll
-        for (int w = 0; w < WARPS; w++) {
-            const float f = exp2_approx(sm_ml[w][r][0] - ref);
-            const float4 y = *reinterpret_cast<const float4 *>(&sm_o[w][r][d]);
-            ll = fmaf(sm_ml[w][r][1], f, ll);
-            x.x = fmaf(y.x, f, x.x), x.y = fmaf(y.y, f, x.y), x.z = fmaf(y.z, f, x.z), x.w = fmaf(y.w, f, x.w);
+            for (int w = 0; w < WARPS; w++) mm = fmaxf(mm, sm_ml[w][r][0]);
+            const float ref = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+            for (int w = 0; w < WARPS; w++) {
+                const float f = exp2_approx(sm_ml[w][r][0] - ref);
+                const float4 y = *reinterpret_cast<const float4 *>(&sm_o[w][r][d]);
+                ll = fmaf(sm_ml[w][r][1], f, ll);
+                x.x = fmaf(y.x, f, x.x), x.y = fmaf(y.y, f, x.y), x.z = fmaf(y.z, f, x.z), x.w = fmaf(y.w, f, x.w);
+            }
         }
         if (my_chunks == 1) {
             finish(r, d, x, mm, ll);
@@ -834,12 +846,6 @@ void check_distinct(const bzb_kv8_rows & r, const char * name, int hd, int n_tok
     if (n_tok > 1 && !by_row && !by_head) fail(std::string(name) + ": rows overlap");
 }
 
-unsigned grid_of(long long tasks, int per_cta) {
-    const long long n = (tasks + per_cta - 1) / per_cta;
-    if (n > INT_MAX) fail("the batch is too large for one call");
-    return (unsigned) n;
-}
-
 // append and read: (heads, blocks of 16 positions that max_new rows can touch, sequences)
 dim3 row_grid(const Kv & kv, int heads, int per_cta) {
     const int blocks = (kv.max_new + 30) / 16;
@@ -862,11 +868,11 @@ void run_read(const ReadArgs & a, cudaStream_t s) {
 // How the rows and the cache of a call are cut up.
 struct Plan {
     bool tile = false;      // kv8_tile.cu's kernel
-    int nt = 1;             // else: tiles of 8 rows that a CTA of the few-row kernel holds
-    int rows = 8;           // rows of a CTA
+    int warps = 4;          // else: of a CTA of the few-row kernel
+    int rows = 8;           // rows of a CTA: 8, each warp working on all of them, or 8 for each warp
     int row_tiles = 1, chunks = 1, chunk_blocks = 1;
 };
-constexpr int kFewRows = 32;
+constexpr int kFewRows = 64;
 // (sequence, row tile, kv head) units that may be split: their counters lie at a fixed place of the workspace, so
 // that calls of different shapes can share one
 constexpr long long kSplitUnits = 1 << 16;
@@ -877,13 +883,12 @@ Plan plan_of(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int c
     const int group = n_head / c.n_kv;
     const long long rows = (long long) b.max_new * group;
     // (a range of the few-row kernel is limited; without splitting it could not reach longer contexts)
-    p.tile = rows > kFewRows || (b.max_len > 16 * kSmallRange && (long long) b.n_seq * c.n_kv * 4 > kSplitUnits);
+    p.tile = rows > kFewRows || (b.max_len > 16 * kSmallBlocks && (long long) b.n_seq * c.n_kv * 4 > kSplitUnits);
     if (p.tile) {
         p.rows = kTileRows;
     } else {
-        const int most = c.head_dim == 64 ? 4 : 2;
-        while (p.nt < most && rows > 8 * p.nt) p.nt *= 2;
-        p.rows = 8 * p.nt;
+        if (rows > 8) p.warps = (int) (rows + 7) / 8;
+        p.rows = rows > 8 ? 8 * p.warps : 8;
     }
     const long long tiles = std::max<long long>(1, (rows + p.rows - 1) / p.rows);
     if (tiles > INT_MAX) fail("max_new x heads per kv head is too large");
@@ -902,27 +907,45 @@ Plan plan_of(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int c
         p.chunk_blocks = (p.chunk_blocks + 7) / 8 * 8;
     } else {
         // ranges that fill whole waves of the CTAs an SM holds; a CTA's start and end cost about as much time as
-        // 32 blocks, joining the ranges as much as 24 more
-        const long long slots = 148ll * small_ctas(c.head_dim, p.nt);
+        // its share of 32 blocks, joining the ranges as much as 24 more (with rows of their own, warps take a
+        // quarter as many blocks in that time)
+        const int pair = 2 * c.head_dim / 16 * 512, merge = 32 * p.warps * (c.head_dim + 4);  // shared memory, as SmallTile has it
+        const int shared = std::max(p.rows > 8 ? 4 * pair : c.head_dim == 64 ? 8 * pair : 4 * pair, merge) + (10 << 10);
+        const long long slots = 148ll * std::min(small_ctas(c.head_dim, p.warps), (227 << 10) / shared);
+        const int start = p.rows > 8 ? 8 : 32, join = p.rows > 8 ? 6 : 24;
         double best = 0;
-        for (int n = (blocks + kSmallRange - 1) / kSmallRange; n <= blocks; n++) {
+        for (int n = (blocks + kSmallBlocks - 1) / kSmallBlocks; n <= blocks; n++) {
             const int size = (blocks + n - 1) / n;
-            const double cost = (double) ((units * n + slots - 1) / slots) * (size + 32) + (n > 1 ? 24 : 0);
+            const double cost = (double) ((units * n + slots - 1) / slots) * (size + start) + (n > 1 ? join : 0);
             if (best == 0 || cost < best) best = cost, p.chunk_blocks = size;
-            if (units * n >= 6 * slots || size <= 2 * kSmallWarps) break;
+            if (units * n >= 6 * slots || size <= (p.rows > 8 ? 2 : 8)) break;
         }
     }
     p.chunks = (blocks + p.chunk_blocks - 1) / p.chunk_blocks;
     return p;
 }
 
-template <int HD, int NT>
+template <int HD, int WARPS, bool SHARED>
 void run_small(const AttnArgs & a, cudaStream_t s) {
-    const unsigned grid = grid_of((long long) a.kv.n_seq * a.row_tiles * a.chunks * a.kv.n_kv, 1);
-    constexpr int bytes = SmallTile<HD, NT, kSmallWarps>::BYTES;
+    const long long grid = (long long) a.kv.n_seq * a.row_tiles * a.chunks * a.kv.n_kv;
+    if (grid > INT_MAX) fail("the batch is too large for one call");
+    constexpr int bytes = SmallTile<HD, WARPS, SHARED>::BYTES;
     static std::atomic<uint64_t> ready{ 0 };
-    allow_shared_memory(kv8_attn_small_kernel<HD, NT, kSmallWarps>, bytes, ready);
-    launch_chained(kv8_attn_small_kernel<HD, NT, kSmallWarps>, dim3(grid), 32 * kSmallWarps, bytes, s, a);
+    allow_shared_memory(kv8_attn_small_kernel<HD, WARPS, SHARED>, bytes, ready);
+    launch_chained(kv8_attn_small_kernel<HD, WARPS, SHARED>, dim3((unsigned) grid), 32 * WARPS, bytes, s, a);
+}
+template <int HD>
+void run_small(const AttnArgs & a, const Plan & p, cudaStream_t s) {
+    if (p.rows == 8) return run_small<HD, 4, false>(a, s);
+    switch (p.warps) {
+        case 2: return run_small<HD, 2, true>(a, s);
+        case 3: return run_small<HD, 3, true>(a, s);
+        case 4: return run_small<HD, 4, true>(a, s);
+        case 5: return run_small<HD, 5, true>(a, s);
+        case 6: return run_small<HD, 6, true>(a, s);
+        case 7: return run_small<HD, 7, true>(a, s);
+        default: return run_small<HD, 8, true>(a, s);
+    }
 }
 
 void check_attention(const bzb_kv8_cache & c, int n_head, int causal, int window) {
@@ -1049,12 +1072,9 @@ void kv8_attention(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_k
     if (p.tile) {
         launch_attn_tile(a, c.head_dim, s);
     } else if (c.head_dim == 64) {
-        if (p.nt == 1) run_small<64, 1>(a, s);
-        else if (p.nt == 2) run_small<64, 2>(a, s);
-        else run_small<64, 4>(a, s);
+        run_small<64>(a, p, s);
     } else {
-        if (p.nt == 1) run_small<128, 1>(a, s);
-        else run_small<128, 2>(a, s);
+        run_small<128>(a, p, s);
     }
 }
 
