@@ -1046,7 +1046,7 @@ void kv8_attention(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_k
     if (!std::isfinite(scale * kLog2e)) fail("scale must be finite");
     if (q.type != out.type) fail("q and out must be of one type");
     a.q_vec = check_rows(q, "q", q.n_head, c.head_dim, false, 8, b.n_tok);
-    a.out_vec = check_rows(out, "out", q.n_head, c.head_dim, false, 4, b.n_tok);
+    a.out_vec = check_rows(out, "out", q.n_head, c.head_dim, false, 8, b.n_tok);
     check_distinct(out, "out", c.head_dim, b.n_tok);
     if ((uintptr_t) lse % 4) fail("lse is misaligned");
     const long long need = kv8_attention_workspace(c, b, q.n_head, causal, window);

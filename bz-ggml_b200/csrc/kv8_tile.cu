@@ -52,7 +52,7 @@ struct Smem {
 };
 
 struct Shared {
-    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], o_full[2], drain[4];
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], q_full[2], o_full[2], drain[4];
     uint64_t s_full[2][2], w_full[2][2], pv_done[2][2];  // [tile][step & 1]
     uint64_t c_full[4], n_full[4];  // scale[] and nan_v[] of a tile (rings of four: see the producers)
     uint32_t tmem;
@@ -176,7 +176,7 @@ __device__ __forceinline__ void load_queries(const AttnArgs & a, const Work & w,
 #pragma unroll
             for (int j = 0; j < 4; j++) x[2 * j] = __uint_as_float(v[j] << 16), x[2 * j + 1] = __uint_as_float(v[j] & 0xffff0000u);
 #pragma unroll
-            for (int j = 0; j < 8; j++) amax = fmaxf(amax, fabsf(x[j]));
+            for (int j = 0; j < 8; j += 2) amax = fmaxf(fmaxf(amax, fabsf(x[j])), fabsf(x[j + 1]));
 #pragma unroll
             for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
             const int e = amax < INFINITY && amax > 0.0f ? min(126, max(-125, (__float_as_int(amax) >> 23) - 127)) : 0;
@@ -339,6 +339,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
             mbar_init(&sh.v_full[i], kProducers);
             mbar_init(&sh.k_empty[i], tiles);
             mbar_init(&sh.v_empty[i], tiles);
+            mbar_init(&sh.q_full[i], 4);
             mbar_init(&sh.o_full[i], 1);
             for (int b = 0; b < 2; b++) {
                 mbar_init(&sh.s_full[i][b], 1);
@@ -355,10 +356,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
         fence_mbar_init();
     }
     if (warp == kMmaWarp) tmem_alloc(&sh.tmem, 512);
-    if (warp < 4 * tiles) {
-        load_queries<HD>(a, w, sh, base + M::oQ + (warp >> 2) * M::kQ, warp >> 2, warp & 3, lane);
-        fence_proxy_async();
-    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -386,6 +383,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         const int i = warp >> 2, r = threadIdx.x & 127, rr = w.row0 + 128 * i + r;
         if (i < tiles) {
+            uint8_t * sq = base + M::oQ + i * M::kQ;
+            load_queries<HD>(a, w, sh, sq, i, warp & 3, lane);
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.q_full[i]);
             const uint32_t lanes = (uint32_t) (warp & 3) << 21;  // tensor memory lanes 32 (warp % 4) ..
             const uint32_t ts = tmem + lanes + i * 2 * kStep, to = tmem + lanes + M::cO + i * HD;
             const bool real = rr < w.rows;
@@ -490,33 +492,73 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
             if (ok && n > 0) ok = warp_wait(&sh.o_full[i], 0, err);
             if (ok) {
                 tc_fence_after();
+                // rows go out through this tile's query buffer, whose products are done, so that a warp writes whole
+                // rows; its 32 rows are its own. f16 rows fit at once, f32 partials half a row at a time
                 const float inv = inverse(l);
-                float * pp = part ? part + ((size_t) w.chunk * kTileRows + 128 * i + r) * PL : nullptr;
-#pragma unroll
-                for (int c = 0; c < HD / 16; c++) {
-                    float y[16];
+                uint8_t * mine = sq + (warp & 3) * (32 * HD * 2);
+                const int me = 128 * i + (warp & 3) * 32, live = min(32, w.rows - w.row0 - me);
+                const auto pull = [&](int d, float (&y)[16]) {
                     if (n > 0) {
-                        tmem_ld16(to + 16 * c, y);
+                        tmem_ld16(to + d, y);
                         tmem_wait_ld();
                     }
 #pragma unroll
                     for (int t = 0; t < 16; t++) {
                         if (n == 0) y[t] = 0.0f;
-                        if (nan_d[c / 2] >> (16 * (c & 1) + t) & 1) y[t] = __int_as_float(0x7fffffff);
+                        if (nan_d[d / 32] >> (d % 32 + t) & 1) y[t] = __int_as_float(0x7fffffff);
                     }
-                    if (real) {
+                };
+                constexpr int C = HD / 8;  // 16-byte chunks of a row in the buffer
+                if (part) {
+                    float * pp = part + ((size_t) w.chunk * kTileRows + me) * PL;
 #pragma unroll
-                        for (int t = 0; t < 16; t += 4) {
-                            const float4 x = make_float4(y[t], y[t + 1], y[t + 2], y[t + 3]);
-                            if (part) *reinterpret_cast<float4 *>(pp + 16 * c + t) = x;
-                            else finish(128 * i + r, 16 * c + t, x, inv);
+                    for (int half_ = 0; half_ < 2; half_++) {
+#pragma unroll
+                        for (int d = 0; d < HD / 2; d += 16) {
+                            float y[16];
+                            pull(half_ * (HD / 2) + d, y);
+#pragma unroll
+                            for (int t = 0; t < 16; t += 4)
+                                *reinterpret_cast<float4 *>(mine + lane * (HD * 2) + (((d + t) / 4 ^ (lane & 7)) << 4)) = make_float4(y[t], y[t + 1], y[t + 2], y[t + 3]);
                         }
+                        __syncwarp();
+                        for (int x = lane; x < live * C; x += 32) {
+                            const int row = x / C, c = x % C;
+                            *reinterpret_cast<float4 *>(pp + row * PL + half_ * (HD / 2) + c * 4) =
+                                *reinterpret_cast<const float4 *>(mine + row * (HD * 2) + ((c ^ (row & 7)) << 4));
+                        }
+                        __syncwarp();
+                    }
+                    if (real) *reinterpret_cast<float2 *>(pp + lane * PL + HD) = make_float2(m, l);
+                } else {
+#pragma unroll
+                    for (int d = 0; d < HD; d += 16) {
+                        float y[16];
+                        pull(d, y);
+                        uint32_t z[8];
+#pragma unroll
+                        for (int t = 0; t < 8; t++)
+                            z[t] = a.type == BZB_F16 ? pack_half(y[2 * t] * inv, y[2 * t + 1] * inv) : pack_bf16(y[2 * t] * inv, y[2 * t + 1] * inv);
+#pragma unroll
+                        for (int t = 0; t < 2; t++)
+                            *reinterpret_cast<uint4 *>(mine + lane * (HD * 2) + ((d / 8 + t ^ (lane & 7)) << 4)) =
+                                make_uint4(z[4 * t], z[4 * t + 1], z[4 * t + 2], z[4 * t + 3]);
                     }
                     __syncwarp();
-                }
-                if (real) {
-                    if (part) *reinterpret_cast<float2 *>(pp + HD) = make_float2(m, l);
-                    else put_lse(128 * i + r, m, l);
+                    for (int x = lane; x < live * C; x += 32) {
+                        const int row = x / C, c = x % C, rr = w.row0 + me + row;
+                        const uint4 v = *reinterpret_cast<const uint4 *>(mine + row * (HD * 2) + ((c ^ (row & 7)) << 4));
+                        uint16_t * to_row = static_cast<uint16_t *>(a.out.p) + (long long) (w.s.row0 + rr / a.group) * a.out.row +
+                                            (w.h * a.group + rr % a.group) * a.out.head + c * 8;
+                        if (a.out_vec) {
+                            *reinterpret_cast<uint4 *>(to_row) = v;
+                        } else {
+                            const uint32_t e[4] = { v.x, v.y, v.z, v.w };
+#pragma unroll
+                            for (int t = 0; t < 4; t++) to_row[2 * t] = (uint16_t) e[t], to_row[2 * t + 1] = (uint16_t) (e[t] >> 16);
+                        }
+                    }
+                    if (real) put_lse(me + lane, m, l);
                 }
             }
             tc_fence_before();
@@ -584,9 +626,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
                 // the buffer's last weights have been read (MMAs of different accumulators have no guaranteed
                 // order, so that product is waited for; the other buffer's scores keep the softmax busy)
                 if (u >= 2) ok = warp_wait(&sh.pv_done[mt][u & 1], ((u - 2) >> 1) & 1, err);
+                else if (u == 0 && mt == 0) ok = warp_wait(&sh.q_full[0], 0, err);
                 // the second tile starts when the first has done its first step: the two softmaxes then take the
                 // exponential units in turn instead of both at once and both not at all
-                else if (u == 0 && mt == 1) ok = warp_wait(&sh.w_full[0][0], 0, err);
+                else if (u == 0) ok = warp_wait(&sh.q_full[1], 0, err) && warp_wait(&sh.w_full[0][0], 0, err);
                 if (ok && !(u & 1)) ok = warp_wait(&sh.k_full[st], (u >> 2) & 1, err);
                 if (!ok) break;
                 tc_fence_after();
