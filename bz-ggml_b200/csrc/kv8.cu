@@ -424,21 +424,15 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, WARPS)) kv8_attn_sm
     start_after_previous();
     const Seq s = load_seq(kv, b);
     if (s.slot < 0) return;
-    const int rows = s.n * a.group, row0 = tile * T::ROWS;
-    if (row0 >= rows) return;
-    const int first = s.len - s.n;
-    const int pos_lo = first + row0 / a.group, pos_hi = first + min(rows - 1, row0 + T::ROWS - 1) / a.group;
-    // the keys that any row of the tile looks at: [key_lo, key_hi)
-    const int key_hi = max(0, a.causal ? pos_hi + 1 : s.len);
-    const int key_lo = a.window > 0 ? max(0, pos_lo - a.window + 1) : 0;
+    const int row0 = tile * T::ROWS;
+    const Span span = span_of(a, s, row0, T::ROWS);
+    const int first = span.first, rows = span.rows, my_chunks = span.chunks;
+    if (row0 >= rows || chunk >= my_chunks) return;
     // this warp's rows, and the keys that all of them see: [full_lo, full_hi)
     const int wrow0 = row0 + (SHARED ? 8 * warp : 0), last_row = max(wrow0, min(rows - 1, wrow0 + 7));
     const int full_hi = a.causal ? first + wrow0 / a.group + 1 : s.len;
     const int full_lo = a.window > 0 ? max(0, first + last_row / a.group - a.window + 1) : 0;
-    const int blk_lo = key_lo >> 4, blk_hi = (key_hi + 15) >> 4;
-    const int my_chunks = max(1, (blk_hi - blk_lo + a.chunk_blocks - 1) / a.chunk_blocks);
-    if (chunk >= my_chunks) return;
-    const int c_lo = blk_lo + chunk * a.chunk_blocks, c_hi = min(blk_hi, c_lo + a.chunk_blocks);
+    const int c_lo = span.blk_lo + chunk * a.chunk_blocks, c_hi = min(span.blk_hi, c_lo + a.chunk_blocks);
 
     // this warp's blocks: base, base + STRIDE, ..., looked up by itself (SHARED: by the whole CTA)
     const int base = c_lo + (SHARED ? 0 : warp), n = max(0, (c_hi - base + STRIDE - 1) / STRIDE);
@@ -744,39 +738,76 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, WARPS)) kv8_attn_sm
             finish(r, d, x, mm, ll);
         } else {
             float * pp = part + ((size_t) chunk * T::ROWS + r) * T::PL;
-            *reinterpret_cast<float2 *>(pp + d) = make_float2(x.x, x.y);
-            *reinterpret_cast<float2 *>(pp + d + 2) = make_float2(x.z, x.w);
-            if (d == 0) pp[HD] = mm, pp[HD + 1] = ll;
+            *reinterpret_cast<float4 *>(pp + d) = x;
+            if (d == 0) *reinterpret_cast<float2 *>(pp + HD) = make_float2(mm, ll);
         }
     }
-    if (my_chunks == 1) return;
-    // the last range of this (sequence, tile, head) to finish joins them all, in the ranges' order
-    __shared__ int last;
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        last = atomicAdd(a.counters + unit, 1) == my_chunks - 1;
-        if (last) a.counters[unit] = 0;
-    }
-    __syncthreads();
-    if (!last) return;
-    __threadfence();
-    for (int i = threadIdx.x; i < live * (HD / 4); i += 32 * WARPS) {
-        const int r = i / (HD / 4), d = i % (HD / 4) * 4;
-        float mm = -INFINITY, ll = 0.0f;
-        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int c = 0; c < my_chunks; c++) {
-            const float * pp = part + ((size_t) c * T::ROWS + r) * T::PL;
-            const float mc = __ldcg(pp + HD), lc = __ldcg(pp + HD + 1);
-            const float to = fmaxf(mm, mc), ref = to == -INFINITY ? 0.0f : to;
-            const float f = exp2_approx(mm - ref), fc = exp2_approx(mc - ref);
-            const float2 y0 = __ldcg(reinterpret_cast<const float2 *>(pp + d)), y1 = __ldcg(reinterpret_cast<const float2 *>(pp + d + 2));
-            mm = to;
-            ll = ll * f + lc * fc;
-            x = make_float4(x.x * f + y0.x * fc, x.y * f + y0.y * fc, x.z * f + y1.x * fc, x.w * f + y1.y * fc);
+}
+
+// Joins the ranges' results of the rows that have several, in the ranges' order: one warp a row, its loads
+// of all ranges under way together. (A launch of its own: joined by the last range's CTA to finish, one
+// row after another behind a fence and an atomic, 64 units of 40 rows and 6 ranges took 12 us.)
+template <int HD>
+__global__ void __launch_bounds__(256) kv8_attn_join_kernel(const AttnArgs a, int tile_rows) {
+    start_after_previous();
+    constexpr int PL = HD + 4, E = HD / 32;
+    const Kv & kv = a.kv;
+    const int lane = threadIdx.x & 31;
+    const unsigned id = blockIdx.x * 8 + (threadIdx.x >> 5), r = id % (unsigned) tile_rows, unit = id / (unsigned) tile_rows;
+    const int h = (int) (unit % (unsigned) kv.n_kv), bt = (int) (unit / (unsigned) kv.n_kv);
+    const int tile = bt % a.row_tiles, b = bt / a.row_tiles;
+    if (b >= kv.n_seq) return;
+    const Seq s = load_seq(kv, b);
+    if (s.slot < 0) return;
+    const Span span = span_of(a, s, tile * tile_rows, tile_rows);
+    const int row = tile * tile_rows + (int) r;
+    if (row >= span.rows || span.chunks == 1) return;
+    const float * part = a.part + ((size_t) unit * a.chunks * tile_rows + r) * PL;
+    const size_t step = (size_t) tile_rows * PL;
+    float m = -INFINITY, l = 0.0f, o[E] = {};
+    for (int c0 = 0; c0 < span.chunks; c0 += 32) {
+        const int n = min(32, span.chunks - c0);
+        const float2 ml = lane < n ? *reinterpret_cast<const float2 *>(part + (c0 + lane) * step + HD) : make_float2(-INFINITY, 0.0f);
+        float top = ml.x;
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        top = fmaxf(top, m);
+        const float ref = top == -INFINITY ? 0.0f : top, f = exp2_approx(ml.x - ref), keep = exp2_approx(m - ref);
+        m = top;
+        l *= keep;
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] *= keep;
+        for (int c = 0; c < n; c += 8) {
+            float v[8][E];
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+#pragma unroll
+                for (int e = 0; e < E; e++) v[k][e] = c + k < n ? part[(c0 + c + k) * step + lane * E + e] : 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float w = __shfl_sync(0xffffffffu, f, (c + k) & 31), lc = __shfl_sync(0xffffffffu, ml.y, (c + k) & 31);
+                if (c + k < n) {
+                    l = fmaf(lc, w, l);
+#pragma unroll
+                    for (int e = 0; e < E; e++) o[e] = fmaf(v[k][e], w, o[e]);
+                }
+            }
         }
-        finish(r, d, x, mm, ll);
     }
+    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // (NaN stays NaN)
+    const int tok = s.row0 + row / a.group, qh = h * a.group + row % a.group;
+    uint16_t * out = static_cast<uint16_t *>(a.out.p) + (long long) tok * a.out.row + qh * a.out.head + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+        const uint32_t x = a.type == BZB_F16 ? pack_half(o[e] * inv, o[e + 1] * inv) : pack_bf16(o[e] * inv, o[e + 1] * inv);
+        if (a.out_vec) {
+            *reinterpret_cast<uint32_t *>(out + e) = x;
+        } else {
+            out[e] = (uint16_t) x;
+            out[e + 1] = (uint16_t) (x >> 16);
+        }
+    }
+    if (a.lse && lane == 0) a.lse[(size_t) tok * a.n_head + qh] = l == 0.0f ? -INFINITY : kLn2 * (m + log2f(l));
 }
 
 // ---- host side ----
@@ -873,17 +904,11 @@ struct Plan {
     int row_tiles = 1, chunks = 1, chunk_blocks = 1;
 };
 constexpr int kFewRows = 64;
-// (sequence, row tile, kv head) units that may be split: their counters lie at a fixed place of the workspace, so
-// that calls of different shapes can share one
-constexpr long long kSplitUnits = 1 << 16;
-constexpr long long kCounterBytes = kSplitUnits * 4;
-
 Plan plan_of(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int causal, int window) {
     Plan p;
     const int group = n_head / c.n_kv;
     const long long rows = (long long) b.max_new * group;
-    // (a range of the few-row kernel is limited; without splitting it could not reach longer contexts)
-    p.tile = rows > kFewRows || (b.max_len > 16 * kSmallBlocks && (long long) b.n_seq * c.n_kv * 4 > kSplitUnits);
+    p.tile = rows > kFewRows;
     if (p.tile) {
         p.rows = kTileRows;
     } else {
@@ -898,9 +923,7 @@ Plan plan_of(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int c
     if (causal && window > 0) keys = std::min<long long>(keys, (long long) window + (p.rows + group - 1) / group + 1 + 15);
     const int blocks = (int) std::max<long long>(1, (keys + 15) / 16 + (window > 0 ? 1 : 0));
     const long long units = std::max<long long>(1, (long long) b.n_seq * c.n_kv * p.row_tiles);
-    if (units > kSplitUnits) {
-        p.chunk_blocks = (blocks + 7) / 8 * 8;
-    } else if (p.tile) {
+    if (p.tile) {
         // one CTA per SM, at least two tiles of 128 keys in each range
         const long long want = std::max<long long>(1, 148 / units);
         p.chunk_blocks = (int) std::max<long long>(16, (blocks + want - 1) / want);
@@ -1033,7 +1056,7 @@ long long kv8_attention_workspace(const bzb_kv8_cache & c, const bzb_kv8_batch &
     const Plan p = plan_of(c, b, n_head, causal, window);
     if (p.chunks == 1) return 0;
     const long long units = (long long) b.n_seq * p.row_tiles * c.n_kv;
-    return kCounterBytes + units * p.chunks * p.rows * (c.head_dim + 4) * 4;
+    return units * p.chunks * p.rows * (c.head_dim + 4) * 4;
 }
 
 void kv8_attention(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_kv8_rows & q, const bzb_kv8_rows & out,
@@ -1067,14 +1090,19 @@ void kv8_attention(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_k
     a.row_tiles = p.row_tiles;
     a.chunks = p.chunks;
     a.chunk_blocks = p.chunk_blocks;
-    a.counters = static_cast<int *>(workspace);
-    a.part = need > 0 ? reinterpret_cast<float *>(static_cast<char *>(workspace) + kCounterBytes) : nullptr;
+    a.part = static_cast<float *>(workspace);
     if (p.tile) {
         launch_attn_tile(a, c.head_dim, s);
     } else if (c.head_dim == 64) {
         run_small<64>(a, p, s);
     } else {
         run_small<128>(a, p, s);
+    }
+    if (p.chunks > 1) {
+        const long long warps = (long long) b.n_seq * p.row_tiles * c.n_kv * p.rows;
+        if (warps > (long long) INT_MAX) fail("the batch is too large for one call");
+        launch_chained(c.head_dim == 64 ? kv8_attn_join_kernel<64> : kv8_attn_join_kernel<128>, dim3((unsigned) ((warps + 7) / 8)), 256, 0, s, a,
+                       p.rows);
     }
 }
 

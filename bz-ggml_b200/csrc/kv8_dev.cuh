@@ -182,9 +182,26 @@ struct AttnArgs {
     int type;      // of q and out
     bool q_vec, out_vec;
     int row_tiles, chunks, chunk_blocks;  // chunk_blocks: blocks of 16 positions in a range
-    float * part;
-    int * counters;
+    float * part;  // ranges' results, when there are several: [unit][range][row][head_dim, maximum, sum, 0, 0]
 };
+
+// The blocks of the cache that a tile's rows look at, and the ranges they are cut into.
+struct Span {
+    int first, rows;             // position of the sequence's first row (negative: padding); its (token, head) rows
+    int blk_lo, blk_hi, chunks;  // blocks of 16 keys [blk_lo, blk_hi) of any row; ranges, at least one
+};
+__device__ __forceinline__ Span span_of(const AttnArgs & a, const Seq & s, int row0, int tile_rows) {
+    Span p;
+    p.first = s.len - s.n;
+    p.rows = s.n * a.group;
+    const int pos_lo = p.first + row0 / a.group, pos_hi = p.first + min(p.rows - 1, row0 + tile_rows - 1) / a.group;
+    const int key_hi = max(0, a.causal ? pos_hi + 1 : s.len), key_lo = a.window > 0 ? max(0, pos_lo - a.window + 1) : 0;
+    p.blk_lo = key_lo >> 4;
+    p.blk_hi = (key_hi + 15) >> 4;
+    p.chunks = max(1, (p.blk_hi - p.blk_lo + a.chunk_blocks - 1) / a.chunk_blocks);
+    return p;
+}
+
 
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;

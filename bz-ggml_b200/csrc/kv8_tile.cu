@@ -57,7 +57,6 @@ struct Shared {
     uint64_t c_full[4], n_full[4];  // scale[] and nan_v[] of a tile (rings of four: see the producers)
     uint32_t tmem;
     int err;
-    int last;
     int nan_v[4][kProducers];   // a producer warp found NaN values in this tile (only where it looked)
     float4 scale[4];            // of a stage: the keys' scale, the values' exponent, 2^-it
     float unit[2][128];         // power of two taken out of each query row
@@ -122,20 +121,17 @@ __device__ __forceinline__ bool find_work(const AttnArgs & a, Work & w) {
     w.tile = a.row_tiles - 1 - (int) (id / (unsigned) kv.n_seq);
     w.s = load_seq(kv, w.b);
     if (w.s.slot < 0) return false;
-    w.rows = w.s.n * a.group;
     w.row0 = w.tile * kTileRows;
-    if (w.row0 >= w.rows) return false;
-    w.first = w.s.len - w.s.n;
+    const Span p = span_of(a, w.s, w.row0, kTileRows);
+    w.rows = p.rows;
+    if (w.row0 >= w.rows || w.chunk >= p.chunks) return false;
+    w.first = p.first;
+    w.my_chunks = p.chunks;
     const int pos_lo = w.first + w.row0 / a.group, pos_hi = w.first + min(w.rows - 1, w.row0 + kTileRows - 1) / a.group;
-    const int key_hi = max(0, a.causal ? pos_hi + 1 : w.s.len), key_lo = a.window > 0 ? max(0, pos_lo - a.window + 1) : 0;
     w.full_hi = a.causal ? pos_lo + 1 : w.s.len;
     w.full_lo = a.window > 0 ? max(0, pos_hi - a.window + 1) : 0;
-    const int lo = key_lo >> 4;
-    w.blk_hi = (key_hi + 15) >> 4;
-    w.my_chunks = max(1, (w.blk_hi - lo + a.chunk_blocks - 1) / a.chunk_blocks);
-    if (w.chunk >= w.my_chunks) return false;
-    w.blk0 = lo + w.chunk * a.chunk_blocks;
-    w.blk_hi = min(w.blk_hi, w.blk0 + a.chunk_blocks);
+    w.blk0 = p.blk_lo + w.chunk * a.chunk_blocks;
+    w.blk_hi = min(p.blk_hi, w.blk0 + a.chunk_blocks);
     w.n_tiles = max(0, (w.blk_hi - w.blk0 + 7) / 8);
     return true;
 }
@@ -366,12 +362,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
     const size_t unit = ((size_t) w.b * a.row_tiles + w.tile) * a.kv.n_kv + w.h;
     float * part = w.my_chunks > 1 ? a.part + unit * a.chunks * ((size_t) kTileRows * PL) : nullptr;
 
-    auto finish = [&](int r, int d, float4 x, float inv) {
-        const int rr = w.row0 + r;
-        store4(a.type, a.out_vec, a.out.p,
-               (long long) (w.s.row0 + rr / a.group) * a.out.row + (w.h * a.group + rr % a.group) * a.out.head + d,
-               make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
-    };
     auto inverse = [](float l) { return l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l); };  // (NaN stays NaN)
     auto put_lse = [&](int r, float m, float l) {
         const int rr = w.row0 + r;
@@ -678,36 +668,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
     tc_fence_after();
     if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
     if (threadIdx.x == 0 && sh.err && a.kv.status) atomicExch(a.kv.status, 2);
-    if (w.my_chunks == 1) return;
-
-    // the last range of these rows to finish joins them all, in the ranges' order
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        sh.last = atomicAdd(a.counters + unit, 1) == w.my_chunks - 1;
-        if (sh.last) a.counters[unit] = 0;
-    }
-    __syncthreads();
-    if (!sh.last) return;
-    __threadfence();
-    const int live = min(kTileRows, w.rows - w.row0);
-    for (int x = threadIdx.x; x < live * (HD / 4); x += kTileThreads) {
-        const int r = x / (HD / 4), d = x % (HD / 4) * 4;
-        float m = -INFINITY, l = 0.0f;
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int c = 0; c < w.my_chunks; c++) {
-            const float * pp = part + ((size_t) c * kTileRows + r) * PL;
-            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(pp + HD));
-            const float4 y = __ldcg(reinterpret_cast<const float4 *>(pp + d));
-            const float mx = fmaxf(m, ml.x), ref = mx == -INFINITY ? 0.0f : mx;
-            const float f = exp2_approx(m - ref), fc = exp2_approx(ml.x - ref);
-            m = mx;
-            l = l * f + ml.y * fc;
-            o = make_float4(o.x * f + y.x * fc, o.y * f + y.y * fc, o.z * f + y.z * fc, o.w * f + y.w * fc);
-        }
-        finish(r, d, o, inverse(l));
-        if (d == 0) put_lse(r, m, l);
-    }
 }
 
 template <int HD>

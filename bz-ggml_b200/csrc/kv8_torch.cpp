@@ -171,7 +171,7 @@ PyObject * attention(PyObject *, PyObject * const * a, Py_ssize_t n) {
             if (held) {
                 space = THPVariable_Unpack(held).data_ptr();
             } else if (!PyErr_Occurred()) {
-                at::Tensor t = at::zeros({ (int64_t) need }, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, c.device));
+                at::Tensor t = at::empty({ (int64_t) need }, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, c.device));
                 space = t.data_ptr();
                 PyObject * py = THPVariable_Wrap(t);
                 if (py) PyDict_SetItem(a[2], key, py);

@@ -199,8 +199,7 @@ BREEZE_API int bzb_kv8_read(const bzb_kv8_cache * cache, const bzb_kv8_batch * b
  * causal == 0 (window 0): all kv_len keys. A row without any key gives zeros. lse, when not NULL, gets
  * log(sum_j exp(scale q . k_j)) as [n_tok][n_head] (-inf without keys), for merging with attention over
  * other keys. q and out of one type, f16 or bf16. `workspace`: bzb_kv8_attention_workspace() bytes
- * (0: none needed) on the device, 16-byte aligned, zeroed once by the caller before its first use and left fit for
- * the next call, of whatever shape it is large enough for, by every call; calls that may overlap need one each. 0, or -1 with breeze_last_error(). */
+ * (0: none needed) on the device, 16-byte aligned, of any content; calls that may overlap need one each. 0, or -1 with breeze_last_error(). */
 BREEZE_API long long bzb_kv8_attention_workspace(const bzb_kv8_cache * cache, const bzb_kv8_batch * batch, int n_head,
                                                  int causal, int window);
 BREEZE_API int bzb_kv8_attention(const bzb_kv8_cache * cache, const bzb_kv8_batch * batch, const bzb_kv8_rows * q,
