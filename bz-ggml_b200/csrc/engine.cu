@@ -407,12 +407,36 @@ void Engine::alloc_buffers() {
     size_t pool_bytes = (size_t) 8 << 30;
     if (const char * e = std::getenv("BZB_KV_POOL_MB")) pool_bytes = (size_t) std::atoll(e) << 20;
     pool_bytes = std::min(pool_bytes, free_b / 2);
-    n_pages_ = (int) std::max<size_t>(16, pool_bytes / (page_elems * sizeof(half)));
-    kv_pool_ = dalloc<half>((size_t) n_pages_ * page_elems);
+    if (const char * c = std::getenv("BZB_KV_CACHE")) {
+        kv8_ = std::strcmp(c, "e4m3") == 0;
+        if (!kv8_ && c[0] && std::strcmp(c, "f16") != 0) throw std::runtime_error("BZB_KV_CACHE must be f16 or e4m3");
+    }
+    if (kv8_) {
+        const size_t page_scales = (size_t) bb.n_layer * 2 * bb.n_kv;
+        n_pages_ = (int) std::max<size_t>(16, pool_bytes / (page_elems + page_scales * sizeof(float)));
+        kv8_pages_ = dalloc<uint8_t>((size_t) n_pages_ * page_elems);
+        kv8_scales_ = dalloc<float>((size_t) n_pages_ * page_scales);
+        kv8_start_ = dalloc<int>(std::max(rmax_, kPackSegs) + 1);
+        kv8_len_ = dalloc<int>(std::max(rmax_, kPackSegs));
+        kv8_slot_ = dalloc<int>(std::max(rmax_, kPackSegs));
+        bq16_ = dalloc<half>((size_t) rmax_ * bb.n_head * bb.hd);
+    } else {
+        n_pages_ = (int) std::max<size_t>(16, pool_bytes / (page_elems * sizeof(half)));
+        kv_pool_ = dalloc<half>((size_t) n_pages_ * page_elems);
+    }
     free_pages_.clear();
     for (int p = n_pages_ - 1; p >= 0; p--) free_pages_.push_back(p);
     page_table_ = dalloc<int>((size_t) max_slots_ * max_pages_);
     CK(cudaMemsetAsync(page_table_, 0, (size_t) max_slots_ * max_pages_ * sizeof(int), stream_));
+    if (kv8_) {
+        // the attention's workspace at any batch size (prompts take no more than a wave of row tiles needs)
+        for (int R = 1; R <= rmax_; R++) {
+            const bzb_kv8_batch b = { kv8_start_, kv8_len_, kv8_slot_, R, R, 1, kv8_max_len() };
+            kv8_ws_bytes_ = std::max(kv8_ws_bytes_, (size_t) kv8_attention_workspace(kv8_cache(0), b, bb.n_head, 1, 0));
+        }
+        kv8_ws_bytes_ = std::max(kv8_ws_bytes_, (size_t) 32 << 20);
+        kv8_ws_ = dalloc<uint8_t>(kv8_ws_bytes_);
+    }
     st_ = dalloc<SessState>(max_slots_);
     CK(cudaMemsetAsync(st_, 0, (size_t) max_slots_ * sizeof(SessState), stream_));
     hist_ld_ = round_up(vbb_, 8);
@@ -499,6 +523,7 @@ void Engine::ensure_prefill_capacity(int T) {
     pff16_ = (half *) pa((size_t) tmax_ * bb.ffn * 2);
     pqkv_ = (float *) pa((size_t) tmax_ * (bbq + 2 * bbkv) * 4);
     patt16_ = (half *) pa((size_t) tmax_ * bbq * 2);
+    if (kv8_) pq16_ = (half *) pa((size_t) tmax_ * bbq * 2);
     plog_ = (float *) pa((size_t) 2 * vbb_ * 4);   // conditional and unconditional branch
     ptok_ = (int *) pa((size_t) tmax_ * 4);
     pframes_ = (int *) pa((size_t) tmax_ * cfg.nc * 4);
@@ -565,25 +590,65 @@ void Engine::depth_layer(int l, int rows, int R, int n_new, int start) {
     gemv(w.down, dff16_, dd.ffn, rows, GemvOut{ EPI_RESID, dx_, nullptr, D });
 }
 
+bzb_kv8_cache Engine::kv8_cache(int layer) const {
+    const BbConfig & bb = cfg.bb;
+    const long long bytes = 2ll * bb.n_kv * 16 * bb.hd, scales = 2ll * bb.n_kv;  // of a layer's part of a page
+    bzb_kv8_cache c = {};
+    c.pages = kv8_pages_ + layer * bytes;
+    c.scales = kv8_scales_ + layer * scales;
+    c.page_table = page_table_;
+    c.page_stride = bb.n_layer * bytes;
+    c.scale_stride = bb.n_layer * scales;
+    c.n_pages = n_pages_;
+    c.n_slots = max_slots_;
+    c.max_pages = max_pages_;
+    c.page_tokens = 16;
+    c.n_kv = bb.n_kv;
+    c.head_dim = bb.hd;
+    CK(cudaGetDevice(&c.device));
+    return c;
+}
+
+// one backbone layer's attention over the 8-bit cache: the fused projection's rows are normed, rotated and
+// appended, then attended
+void Engine::kv8_attend(int layer, const bzb_kv8_batch & batch, const float * qkv, half * q16, half * out) {
+    const BbConfig & bb = cfg.bb;
+    const LayerW & w = bb_[layer];
+    const long long ld = (long long) (bb.n_head + 2 * bb.n_kv) * bb.hd, q = (long long) bb.n_head * bb.hd;
+    float * rows = const_cast<float *>(qkv);
+    const bzb_kv8_rows rq = { rows, ld, bb.hd, bb.n_head, BZB_F32 }, rk = { rows + q, ld, bb.hd, bb.n_kv, BZB_F32 },
+                       rv = { rows + q + (long long) bb.n_kv * bb.hd, ld, bb.hd, bb.n_kv, BZB_F32 },
+                       ro = { q16, q, bb.hd, bb.n_head, BZB_F16 }, rout = { out, q, bb.hd, bb.n_head, BZB_F16 };
+    const bzb_kv8_cache cache = kv8_cache(layer);
+    kv8_append(cache, batch, &rq, rk, rv, &ro, w.q_norm, w.k_norm, bb.eps, reinterpret_cast<const float *>(rope_bb_),
+               rope_bb_max_, stream_);
+    kv8_attention(cache, batch, ro, rout, nullptr, 1.0f / std::sqrt((float) bb.hd), 1, 0, kv8_ws_, (long long) kv8_ws_bytes_,
+                  stream_);
+}
+
 void Engine::bb_decode_layer(int l, int R) {
     const BbConfig & bb = cfg.bb;
     const LayerW & w = bb_[l];
     const int H = cfg.hidden, q = bb.n_head * bb.hd, kv = bb.n_kv * bb.hd, qkvd = q + 2 * kv;
     launch_rmsnorm(bx_, H, w.attn_norm, H, bb.eps, bh16_, H, nullptr, 0, 0, R, nullptr, stream_);
     gemv(w.qkv, bh16_, H, R, GemvOut{ EPI_STORE, bqkv_, nullptr, qkvd });
-    AttnDecodeArgs a;
-    a.qkv = bqkv_; a.ldq = qkvd; a.n_head = bb.n_head; a.n_kv = bb.n_kv; a.hd = bb.hd;
-    a.R = R; a.n_new = 1; a.row_slot = row_slot_; a.row_active = row_active_; a.st = st_;
-    a.q_norm = w.q_norm; a.k_norm = w.k_norm; a.eps = bb.eps; a.rope = rope_bb_;
-    a.scale = 1.0f / std::sqrt((float) bb.hd);
-    a.kv.pool = kv_pool_; a.kv.page_table = page_table_; a.kv.max_pages = max_pages_; a.kv.n_layer = bb.n_layer; a.kv.layer = l;
-    a.out = batt16_; a.ldo = q;
-    // split the cached positions over up to 8 CTAs per (session, kv head) while the grid is
-    // small (about 2048 CTAs for the whole batch); BZB_ATTN_SPLITS overrides
-    int splits = std::max(1, std::min(kAttnMaxSplits, 2048 / std::max(1, R * bb.n_kv)));
-    if (const char * e = std::getenv("BZB_ATTN_SPLITS")) splits = std::max(1, std::min(kAttnMaxSplits, std::atoi(e)));
-    a.splits = splits; a.part = battn_part_; a.counters = battn_ctr_;
-    launch_attn_decode(a, true, stream_);
+    if (kv8_) {
+        kv8_attend(l, { kv8_start_, kv8_len_, kv8_slot_, R, R, 1, kv8_max_len() }, bqkv_, bq16_, batt16_);
+    } else {
+        AttnDecodeArgs a;
+        a.qkv = bqkv_; a.ldq = qkvd; a.n_head = bb.n_head; a.n_kv = bb.n_kv; a.hd = bb.hd;
+        a.R = R; a.n_new = 1; a.row_slot = row_slot_; a.row_active = row_active_; a.st = st_;
+        a.q_norm = w.q_norm; a.k_norm = w.k_norm; a.eps = bb.eps; a.rope = rope_bb_;
+        a.scale = 1.0f / std::sqrt((float) bb.hd);
+        a.kv.pool = kv_pool_; a.kv.page_table = page_table_; a.kv.max_pages = max_pages_; a.kv.n_layer = bb.n_layer; a.kv.layer = l;
+        a.out = batt16_; a.ldo = q;
+        // split the cached positions over up to 8 CTAs per (session, kv head) while the grid is
+        // small (about 2048 CTAs for the whole batch); BZB_ATTN_SPLITS overrides
+        int splits = std::max(1, std::min(kAttnMaxSplits, 2048 / std::max(1, R * bb.n_kv)));
+        if (const char * e = std::getenv("BZB_ATTN_SPLITS")) splits = std::max(1, std::min(kAttnMaxSplits, std::atoi(e)));
+        a.splits = splits; a.part = battn_part_; a.counters = battn_ctr_;
+        launch_attn_decode(a, true, stream_);
+    }
     gemv(w.o, batt16_, q, R, GemvOut{ EPI_RESID, bx_, nullptr, H });
     launch_rmsnorm(bx_, H, w.ffn_norm, H, bb.eps, bh16_, H, nullptr, 0, 0, R, nullptr, stream_);
     gemv(w.gu, bh16_, H, R, GemvOut{ EPI_SWIGLU, nullptr, bff16_, bb.ffn });
@@ -872,6 +937,7 @@ void Engine::enqueue_step(int R, int flags) {
     }
     // backbone: one token per session over its own paged cache
     launch_audio_embed(audio_embd_, (flags & kFlagFeed) ? cur_feed_ : cur_frames_, nc, nc, vs, R, bx_, row_active_, stream_);
+    if (kv8_) launch_kv8_rows(row_slot_, row_active_, st_, R, kv8_start_, kv8_slot_, kv8_len_, stream_);
     for (int l = 0; l < cfg.bb.n_layer; l++) bb_decode_layer(l, R);
     launch_rmsnorm(bx_, H, bb_out_norm_, H, cfg.bb.eps, bh16_, H, hid32_, H, 0, R, row_slot_, stream_);
     gemv(lm_head_, bh16_, H, R, GemvOut{ EPI_STORE, blog_, nullptr, vbb_ });
@@ -1182,6 +1248,13 @@ void Engine::te_forward(const std::vector<int> & tokens, float * out_rows) {
 void Engine::bb_prefill(int slot, int T, float * logits) {
     const BbConfig & bb = cfg.bb;
     const int H = cfg.hidden, q = bb.n_head * bb.hd, kv = bb.n_kv * bb.hd, qkvd = q + 2 * kv;
+    if (kv8_) {
+        // (copies from pageable host memory are staged at the call)
+        const int start[2] = { 0, T };
+        CK(cudaMemcpyAsync(kv8_start_, start, sizeof(start), cudaMemcpyHostToDevice, stream_));
+        CK(cudaMemcpyAsync(kv8_len_, &T, sizeof(int), cudaMemcpyHostToDevice, stream_));
+        CK(cudaMemcpyAsync(kv8_slot_, &slot, sizeof(int), cudaMemcpyHostToDevice, stream_));
+    }
     for (int l = 0; l < bb.n_layer; l++) {
         const LayerW & w = bb_[l];
         launch_rmsnorm(px_, H, w.attn_norm, H, bb.eps, ph16_, H, nullptr, 0, 0, T, nullptr, stream_);
@@ -1195,8 +1268,12 @@ void Engine::bb_prefill(int slot, int T, float * logits) {
         pa.page_row = page_table_ + (size_t) slot * max_pages_;
         pa.causal = true;
         pa.out = patt16_; pa.ldo = q;
-        launch_qk_prep(pa, true, stream_);
-        launch_attn_prefill(pa, true, stream_);
+        if (kv8_) {
+            kv8_attend(l, { kv8_start_, kv8_len_, kv8_slot_, 1, T, T, T }, pqkv_, pq16_, patt16_);
+        } else {
+            launch_qk_prep(pa, true, stream_);
+            launch_attn_prefill(pa, true, stream_);
+        }
         gemv(w.o, patt16_, q, T, GemvOut{ EPI_RESID, px_, nullptr, H });
         launch_rmsnorm(px_, H, w.ffn_norm, H, bb.eps, ph16_, H, nullptr, 0, 0, T, nullptr, stream_);
         gemv(w.gu, ph16_, H, T, GemvOut{ EPI_SWIGLU, nullptr, pff16_, bb.ffn });
@@ -1460,6 +1537,20 @@ void Engine::bb_prefill_packed(const std::vector<int4> & segs, float * logits) {
     CK(cudaMemcpyAsync(pqb_, qb.data(), qb.size() * sizeof(int2), cudaMemcpyHostToDevice, stream_));
     CK(cudaMemcpyAsync(pidx_, last.data(), nb * sizeof(int), cudaMemcpyHostToDevice, stream_));
     CK(cudaMemcpyAsync(pslot_, slots.data(), nb * sizeof(int), cudaMemcpyHostToDevice, stream_));
+    int longest = 0;
+    if (kv8_) {
+        // packed rows: every segment starts where the one before it ends
+        std::vector<int> start(nb + 1, 0), len(nb);
+        for (int b = 0; b < nb; b++) {
+            start[b] = segs[b].x;
+            start[b + 1] = segs[b].x + segs[b].y;
+            len[b] = segs[b].y;
+            longest = std::max(longest, len[b]);
+        }
+        CK(cudaMemcpyAsync(kv8_start_, start.data(), (nb + 1) * sizeof(int), cudaMemcpyHostToDevice, stream_));
+        CK(cudaMemcpyAsync(kv8_len_, len.data(), nb * sizeof(int), cudaMemcpyHostToDevice, stream_));
+        CK(cudaMemcpyAsync(kv8_slot_, slots.data(), nb * sizeof(int), cudaMemcpyHostToDevice, stream_));
+    }
     for (int l = 0; l < bb.n_layer; l++) {
         const LayerW & w = bb_[l];
         launch_rmsnorm(px_, H, w.attn_norm, H, bb.eps, ph16_, H, nullptr, 0, 0, T, nullptr, stream_);
@@ -1474,8 +1565,12 @@ void Engine::bb_prefill_packed(const std::vector<int4> & segs, float * logits) {
         pa.causal = true;
         pa.out = patt16_; pa.ldo = q;
         pa.row_seg = pseg_; pa.segs = psegs_; pa.qblocks = pqb_; pa.n_qblocks = (int) qb.size();
-        launch_qk_prep(pa, true, stream_);
-        launch_attn_prefill(pa, true, stream_);
+        if (kv8_) {
+            kv8_attend(l, { kv8_start_, kv8_len_, kv8_slot_, nb, T, longest, longest }, pqkv_, pq16_, patt16_);
+        } else {
+            launch_qk_prep(pa, true, stream_);
+            launch_attn_prefill(pa, true, stream_);
+        }
         gemv(w.o, patt16_, q, T, GemvOut{ EPI_RESID, px_, nullptr, H });
         launch_rmsnorm(px_, H, w.ffn_norm, H, bb.eps, ph16_, H, nullptr, 0, 0, T, nullptr, stream_);
         gemv(w.gu, ph16_, H, T, GemvOut{ EPI_SWIGLU, nullptr, pff16_, bb.ffn });
@@ -2066,7 +2161,9 @@ size_t Engine::weight_bytes_per_step() const {
 }
 
 size_t Engine::kv_bytes_per_position() const {
-    return (size_t) cfg.bb.n_layer * 2 * cfg.bb.n_kv * cfg.bb.hd * sizeof(half);
+    // (8 bits: a byte for each value, and a scale for each 16 positions of a head)
+    const size_t heads = (size_t) cfg.bb.n_layer * 2 * cfg.bb.n_kv;
+    return kv8_ ? heads * cfg.bb.hd + heads * sizeof(float) / 16 : heads * cfg.bb.hd * sizeof(half);
 }
 
 }  // namespace bzb

@@ -5,6 +5,7 @@
 #include "depth_persist.cuh"
 #include "host.h"
 #include "kernels.cuh"
+#include "kv8.h"
 
 #include <functional>
 #include <map>
@@ -272,6 +273,19 @@ private:
 
     // KV pool and sessions
     half * kv_pool_ = nullptr;
+    // BZB_KV_CACHE=e4m3: the same pages in 8 bits (kv8.h) instead, [page][layer] of keys and values and
+    // [page][layer] of their scales; the step's rows as its batch, the backbone's turned queries, and
+    // the attention's workspace
+    bool kv8_ = false;
+    uint8_t * kv8_pages_ = nullptr;
+    float * kv8_scales_ = nullptr;
+    int * kv8_start_ = nullptr, * kv8_len_ = nullptr, * kv8_slot_ = nullptr;
+    half * bq16_ = nullptr, * pq16_ = nullptr;
+    void * kv8_ws_ = nullptr;
+    size_t kv8_ws_bytes_ = 0;
+    int kv8_max_len() const { return std::min(max_pages_ * 16, rope_bb_max_); }
+    bzb_kv8_cache kv8_cache(int layer) const;
+    void kv8_attend(int layer, const bzb_kv8_batch & batch, const float * qkv, half * q16, half * out);
     int n_pages_ = 0, max_pages_ = 0, max_slots_ = 0;
     std::vector<int> free_pages_;
     int * page_table_ = nullptr;

@@ -1330,6 +1330,18 @@ __global__ void step_init_kernel(const StepArgs a) {
     }
 }
 
+__global__ void kv8_rows_kernel(const int * row_slot, const int * row_active, const SessState * st, int R, int * start,
+                                int * slot, int * len) {
+    pdl_trigger();
+    pdl_wait();
+    const int r = blockIdx.x * blockDim.x + threadIdx.x;
+    if (r <= R) start[r] = r;
+    if (r >= R) return;
+    const int s = row_slot[r];
+    slot[r] = max(s, 0);
+    len[r] = s >= 0 && row_active[r] ? st[s].pos + 1 : 0;
+}
+
 // dst[0..K) = f16(q * d) of one Q8_0 embedding row, 8 values per 8-byte load
 __device__ __forceinline__ void embed_row_f16(const QRows & e, size_t row, half * dst) {
     const int8_t * q = e.qs + row * e.K;
@@ -1998,6 +2010,11 @@ void launch_attn_prefill(const PrefillArgs & a, bool paged, cudaStream_t s) {
         default: throw std::runtime_error("prefill attention: head_dim must be 64, 128 or 256");
     }
     BZB_CUDA_CHECK(cudaGetLastError());
+}
+
+void launch_kv8_rows(const int * row_slot, const int * row_active, const SessState * st, int R, int * start, int * slot,
+                     int * len, cudaStream_t s) {
+    launch_k(kv8_rows_kernel, dim3(R / 128 + 1), dim3(128), 0, s, row_slot, row_active, st, R, start, slot, len);
 }
 
 void launch_step_init(const StepArgs & a, cudaStream_t s) {

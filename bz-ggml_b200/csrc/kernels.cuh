@@ -232,6 +232,10 @@ struct StepArgs {
     const int * force = nullptr;
 };
 void launch_step_init(const StepArgs & a, cudaStream_t s);
+// the step's rows as a batch of one-row sequences of the 8-bit cache: start[r] = r (R + 1 entries), slot[r], and
+// len[r] = the row's positions with its new one, 0 for a row that is not stepped (padding)
+void launch_kv8_rows(const int * row_slot, const int * row_active, const SessState * st, int R, int * start, int * slot,
+                     int * len, cudaStream_t s);
 // codes[r] = first argmax of logits[r]; frames[..][r][col] = code; when gather_cb >= 0 the
 // next sub-step's input row din16[r] = embedding row (gather_cb*vs + code)
 void launch_argmax_gather(const StepArgs & a, const float * logits, int ld, int V, int col, int gather_cb,
