@@ -54,7 +54,7 @@ struct Smem {
 struct Shared {
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], q_full[2], o_full[2], drain[4];
     uint64_t s_full[2][2], w_full[2][2], pv_done[2][2];  // [tile][step & 1]
-    uint64_t c_full[4], n_full[4];  // scale[] and nan_v[] of a tile (rings of four: see the producers)
+    uint64_t n_full[4];  // nan_v[] of a stage (a ring of four, as scale[]: see the producers)
     uint32_t tmem;
     int err;
     int nan_v[4][kProducers];   // a producer warp found NaN values in this tile (only where it looked)
@@ -338,13 +338,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
             mbar_init(&sh.q_full[i], 4);
             mbar_init(&sh.o_full[i], 1);
             for (int b = 0; b < 2; b++) {
-                mbar_init(&sh.s_full[i][b], 1);
+                mbar_init(&sh.s_full[i][b], 2);
                 mbar_init(&sh.w_full[i][b], 4);
                 mbar_init(&sh.pv_done[i][b], 1);
             }
         }
         for (int i = 0; i < 4; i++) {
-            mbar_init(&sh.c_full[i], 1);
             mbar_init(&sh.n_full[i], kProducers);
             mbar_init(&sh.drain[i], 1);
         }
@@ -392,14 +391,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
             float4 c = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // the stage's keys' scale times the row's factor, values' exponent, 2^-it
             for (int u = 0; u < steps; u++) {
                 const int j = u >> 1, key0 = (w.blk0 << 4) + kStep * u;
+                ok = warp_wait(&sh.s_full[i][u & 1], j & 1, err);
+                if (!ok) break;
                 if (!(u & 1)) {
-                    ok = warp_wait(&sh.c_full[j & 3], (j >> 2) & 1, err);
-                    if (!ok) break;
                     c = sh.scale[j & 3];
                     c.x *= row_coef;
                 }
-                ok = warp_wait(&sh.s_full[i][u & 1], j & 1, err);
-                if (!ok) break;
                 tc_fence_after();
                 const bool whole = key0 >= warp_lo && key0 + kStep <= warp_hi;
                 const uint32_t at = ts + (u & 1) * kStep;
@@ -579,12 +576,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
             if (pw == 0 && lane == 0) sh.scale[j & 3] = make_float4(pow2f(sk.top), (float) sv.top, pow2f(-sv.top), 0.0f);
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&sh.k_full[st]);
-                // scale[] and nan_v[] are rings of four: tile j + 4 is stored when the products of tile j + 2
-                // have been issued, which every softmax warp's weights of tile j + 1 come before
-                if (pw == 0) mbar_arrive(&sh.c_full[j & 3]);
-            }
+            // (scale[] and nan_v[] are rings of four: those of stage j + 4 are stored when the products of stage
+            // j + 2 have been issued, which every softmax warp's weights of stage j + 1 come before)
+            if (lane == 0) mbar_arrive(&sh.k_full[st]);
             pg = next;
             next = tile_page(a, w, j + 2, lane);
             k.load(block(pg, j + 1, 0));
@@ -631,6 +625,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
                         umma_f16(sc + (u & 1) * kStep, q + at, k + at, idesc, kk > 0);
                     }
                     umma_commit(&sh.s_full[mt][u & 1]);
+                    // (and this thread's own arrival, which hands on what the wait for the keys made visible: the
+                    // stage's scales)
+                    mbar_arrive(&sh.s_full[mt][u & 1]);
                     if (u & 1) umma_commit(&sh.k_empty[st]);
                 }
                 __syncwarp();
