@@ -52,7 +52,7 @@ struct Smem {
 };
 
 struct Shared {
-    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], q_full[2], o_full[2], drain[4];
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], q_full[2], o_full[2], lead, drain[4];
     uint64_t s_full[2][2], w_full[2][2], pv_done[2][2];  // [tile][step & 1]
     uint64_t n_full[4];  // nan_v[] of a stage (a ring of four, as scale[]: see the producers)
     uint32_t tmem;
@@ -347,6 +347,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
             mbar_init(&sh.n_full[i], kProducers);
             mbar_init(&sh.drain[i], 1);
         }
+        mbar_init(&sh.lead, 4);
         sh.err = 0;
         fence_mbar_init();
     }
@@ -454,7 +455,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.w_full[i][u & 1]);
+                if (lane == 0) {
+                    mbar_arrive(&sh.w_full[i][u & 1]);
+                    if (u == 0 && i == 0) mbar_arrive(&sh.lead);
+                }
                 // NaN values in a stage that some row of the CTA does not see in whole: the producers left them
                 // out; the rows that see one get it at the end
                 const int stage0 = (w.blk0 + 8 * j) << 4;
@@ -612,8 +616,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
                 if (u >= 2) ok = warp_wait(&sh.pv_done[mt][u & 1], ((u - 2) >> 1) & 1, err);
                 else if (u == 0 && mt == 0) ok = warp_wait(&sh.q_full[0], 0, err);
                 // the second tile starts when the first has done its first step: the two softmaxes then take the
-                // exponential units in turn instead of both at once and both not at all
-                else if (u == 0) ok = warp_wait(&sh.q_full[1], 0, err) && warp_wait(&sh.w_full[0][0], 0, err);
+                // exponential units in turn instead of both at once and both not at all. (A barrier that completes
+                // once: this wait may come any time after)
+                else if (u == 0) ok = warp_wait(&sh.q_full[1], 0, err) && warp_wait(&sh.lead, 0, err);
                 if (ok && !(u & 1)) ok = warp_wait(&sh.k_full[st], (u >> 2) & 1, err);
                 if (!ok) break;
                 tc_fence_after();
