@@ -405,7 +405,6 @@ __device__ __forceinline__ uint4 lds16(uint32_t a) {
 template <int HD, int WARPS, bool SHARED>
 __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, WARPS)) kv8_attn_small_kernel(const AttnArgs a) {
     using T = SmallTile<HD, WARPS, SHARED>;
-    constexpr int NT = 1;  // tiles of 8 rows of a warp
     constexpr int STRIDE = SHARED ? 1 : WARPS;  // between the blocks of a warp
     extern __shared__ __align__(16) uint8_t ring[];
     __shared__ float sm_ml[WARPS][8][2];
@@ -488,61 +487,57 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, WARPS)) kv8_attn_sm
     }
     sync();
 
-    // queries as the 8-column operand: lane (g, t) holds row 8 nt + g, elements 64 k + 16 t ..+15
-    uint32_t qf[NT][T::KS][8];
-    float coef[NT][2];      // the score's factor for the lane's two columns (rows 8 nt + 2 t, + 1)
-    int lim_hi[NT][2], lim_lo[NT][2];
+    // queries as the 8-column operand: lane (g, t) holds the warp's row g, elements 64 k + 16 t ..+15
+    uint32_t qf[T::KS][8];
+    float coef[2];      // the score's factor for the lane's two columns (rows 2 t, 2 t + 1)
+    int lim_hi[2], lim_lo[2];
+    const int r = wrow0 + g;
+    float row_unit = 1.0f;
+    if (r < rows) {
+        const long long at = (long long) (s.row0 + r / a.group) * a.q.row + (h * a.group + r % a.group) * a.q.head + 16 * t;
+        float amax = 0.0f;
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        const int r = wrow0 + 8 * nt + g;
-        float unit = 1.0f;
-        if (r < rows) {
-            const long long at = (long long) (s.row0 + r / a.group) * a.q.row + (h * a.group + r % a.group) * a.q.head + 16 * t;
-            float amax = 0.0f;
+        for (int k = 0; k < T::KS; k++) load_q16(a, at + 64 * k, 1.0f, qf[k], &amax);
+        // bf16 may lie outside f16: the row is brought to about [1, 2) by a power of two (which the
+        // scores' factor takes back), so at most its elements below 2^-25 of the largest are lost
+        if (a.type == BZB_BF16) {
+            const unsigned quad = 0xfu << (lane & 28);
+            amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 2));
+            const int e = amax < INFINITY && amax > 0.0f ? min(126, max(-125, (__float_as_int(amax) >> 23) - 127)) : 0;
+            row_unit = pow2f(e);
 #pragma unroll
-            for (int k = 0; k < T::KS; k++) load_q16(a, at + 64 * k, 1.0f, qf[nt][k], &amax);
-            // bf16 may lie outside f16: the row is brought to about [1, 2) by a power of two (which the
-            // scores' factor takes back), so at most its elements below 2^-25 of the largest are lost
-            if (a.type == BZB_BF16) {
-                const unsigned quad = 0xfu << (lane & 28);
-                amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 1));
-                amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 2));
-                const int e = amax < INFINITY && amax > 0.0f ? min(126, max(-125, (__float_as_int(amax) >> 23) - 127)) : 0;
-                unit = pow2f(e);
-#pragma unroll
-                for (int k = 0; k < T::KS; k++) load_q16(a, at + 64 * k, pow2f(-e), qf[nt][k], nullptr);
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < T::KS; k++)
-#pragma unroll
-                for (int j = 0; j < 8; j++) qf[nt][k][j] = 0;
+            for (int k = 0; k < T::KS; k++) load_q16(a, at + 64 * k, pow2f(-e), qf[k], nullptr);
         }
+    } else {
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int rr = wrow0 + 8 * nt + 2 * t + i, pos = first + rr / a.group;
-            coef[nt][i] = a.scale2 * __shfl_sync(0xffffffffu, unit, (2 * t + i) * 4);
-            lim_hi[nt][i] = rr < rows ? (a.causal ? pos + 1 : s.len) : 0;
-            lim_lo[nt][i] = a.window > 0 ? pos - a.window + 1 : 0;
-        }
+        for (int k = 0; k < T::KS; k++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) qf[k][j] = 0;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int rr = wrow0 + 2 * t + i, pos = first + rr / a.group;
+        coef[i] = a.scale2 * __shfl_sync(0xffffffffu, row_unit, (2 * t + i) * 4);
+        lim_hi[i] = rr < rows ? (a.causal ? pos + 1 : s.len) : 0;
+        lim_lo[i] = a.window > 0 ? pos - a.window + 1 : 0;
     }
 
-    float o[NT][T::MT][4] = {}, m[NT][2], l[NT][2] = {};
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) m[nt][0] = m[nt][1] = -INFINITY;
+    float o[T::MT][4] = {}, m[2], l[2] = {};
+    m[0] = m[1] = -INFINITY;
 
     for (int i = 0; i < n; i += 2) {
         asm volatile("cp.async.wait_group %0;" ::"n"(2 * T::AHEAD - 1) : "memory");  // the keys
         sync();
         const uint32_t pair = slots + i / 2 % T::AHEAD * 2 * (T::PIECES * 512);
-        float x[2][NT][4];  // columns 2t, 2t+1 at key kpos, then at key kpos + 2
-        uint32_t seen[2][NT][2];  // (positions x rows) the rows that see each position, as f16 ones
+        float x[2][4];  // columns 2t, 2t+1 at key kpos, then at key kpos + 2
+        uint32_t seen[2][2];  // (positions x rows) the rows that see each position, as f16 ones
         bool whole[2];
         float inv_vs[2];
 #pragma unroll
         for (int k2 = 0; k2 < 2; k2++) {
             const uint32_t slot = pair + k2 * (T::PIECES * 512) + k_from;
-            float sc[NT][4] = {}, sd[NT][4] = {};  // (two sums: half as long a chain of MMAs)
+            float sc[4] = {}, sd[4] = {};  // (two sums: half as long a chain of MMAs)
 #pragma unroll
             for (int k = 0; k < T::KS; k++) {
                 const int at = HD == 64 ? 0 : 64 * (k ^ (g & 1));
@@ -552,8 +547,7 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, WARPS)) kv8_attn_sm
                 for (int j = 0; j < 4; j++) {
                     const uint32_t a0 = e4m3x2_to_h2((uint16_t) w0[j]), a2 = e4m3x2_to_h2((uint16_t) (w0[j] >> 16));
                     const uint32_t a1 = e4m3x2_to_h2((uint16_t) w1[j]), a3 = e4m3x2_to_h2((uint16_t) (w1[j] >> 16));
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++) mma16816(j & 1 ? sd[nt] : sc[nt], a0, a1, a2, a3, qf[nt][k][2 * j], qf[nt][k][2 * j + 1]);
+                    mma16816(j & 1 ? sd : sc, a0, a1, a2, a3, qf[k][2 * j], qf[k][2 * j + 1]);
                 }
             }
             const bool there = i + k2 < n;
@@ -563,65 +557,57 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, WARPS)) kv8_attn_sm
             const float ev = (float) exponent_of(vs);
             inv_vs[k2] = pow2f(-exponent_of(vs));
             whole[k2] = there && key0 >= full_lo && key0 + 16 <= full_hi;
+            const float c0 = coef[0] * ks, c1 = coef[1] * ks;
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                const float c0 = coef[nt][0] * ks, c1 = coef[nt][1] * ks;
+            for (int j = 0; j < 4; j++) x[k2][j] = fmaf(sc[j] + sd[j], j & 1 ? c1 : c0, ev);
+            if (!whole[k2]) {
+                uint32_t one[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) x[k2][nt][j] = fmaf(sc[nt][j] + sd[nt][j], j & 1 ? c1 : c0, ev);
-                if (!whole[k2]) {
-                    uint32_t one[4];
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int key = key0 + kpos + (j >> 1) * 2;
-                        const bool in = there && key >= lim_lo[nt][j & 1] && key < lim_hi[nt][j & 1];
-                        if (!in) x[k2][nt][j] = -INFINITY;
-                        one[j] = in ? 0x3c00u : 0u;
-                    }
-                    seen[k2][nt][0] = one[0] | (one[1] << 16);
-                    seen[k2][nt][1] = one[2] | (one[3] << 16);
+                for (int j = 0; j < 4; j++) {
+                    const int key = key0 + kpos + (j >> 1) * 2;
+                    const bool in = there && key >= lim_lo[j & 1] && key < lim_hi[j & 1];
+                    if (!in) x[k2][j] = -INFINITY;
+                    one[j] = in ? 0x3c00u : 0u;
                 }
+                seen[k2][0] = one[0] | (one[1] << 16);
+                seen[k2][1] = one[2] | (one[3] << 16);
             }
         }
         // (also past the end, where it copies zeros: the waits count groups)
         sync();
         fetch(i + 2 * T::AHEAD, false);
-        uint32_t wb[2][NT][2];
+        uint32_t wb[2][2];
         bool moved = false;
-        float corr[NT][2];
+        float corr[2];
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-            for (int i2 = 0; i2 < 2; i2++) {
-                float mx = fmaxf(fmaxf(x[0][nt][i2], x[0][nt][i2 + 2]), fmaxf(x[1][nt][i2], x[1][nt][i2 + 2]));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                const float to = fmaxf(m[nt][i2], mx), ref = to == -INFINITY ? 0.0f : to;
-                corr[nt][i2] = exp2_approx(m[nt][i2] - ref);
-                moved |= to != m[nt][i2];
-                m[nt][i2] = to;
-                float sum = 0.0f;
-#pragma unroll
-                for (int k2 = 0; k2 < 2; k2++) {
-                    x[k2][nt][i2] = exp2_approx(x[k2][nt][i2] - ref);
-                    x[k2][nt][i2 + 2] = exp2_approx(x[k2][nt][i2 + 2] - ref);
-                    sum = fmaf(x[k2][nt][i2] + x[k2][nt][i2 + 2], inv_vs[k2], sum);
-                }
-                l[nt][i2] = fmaf(l[nt][i2], corr[nt][i2], sum);
-            }
+        for (int i2 = 0; i2 < 2; i2++) {
+            float mx = fmaxf(fmaxf(x[0][i2], x[0][i2 + 2]), fmaxf(x[1][i2], x[1][i2 + 2]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            const float to = fmaxf(m[i2], mx), ref = to == -INFINITY ? 0.0f : to;
+            corr[i2] = exp2_approx(m[i2] - ref);
+            moved |= to != m[i2];
+            m[i2] = to;
+            float sum = 0.0f;
 #pragma unroll
             for (int k2 = 0; k2 < 2; k2++) {
-                wb[k2][nt][0] = transpose8x8(pack_half(x[k2][nt][0], x[k2][nt][1]));
-                wb[k2][nt][1] = transpose8x8(pack_half(x[k2][nt][2], x[k2][nt][3]));
+                x[k2][i2] = exp2_approx(x[k2][i2] - ref);
+                x[k2][i2 + 2] = exp2_approx(x[k2][i2 + 2] - ref);
+                sum = fmaf(x[k2][i2] + x[k2][i2 + 2], inv_vs[k2], sum);
             }
+            l[i2] = fmaf(l[i2], corr[i2], sum);
+        }
+#pragma unroll
+        for (int k2 = 0; k2 < 2; k2++) {
+            wb[k2][0] = transpose8x8(pack_half(x[k2][0], x[k2][1]));
+            wb[k2][1] = transpose8x8(pack_half(x[k2][2], x[k2][3]));
         }
         if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
+            for (int j = 0; j < T::MT; j++)
 #pragma unroll
-                for (int j = 0; j < T::MT; j++)
-#pragma unroll
-                    for (int i2 = 0; i2 < 4; i2++) o[nt][j][i2] *= corr[nt][i2 & 1];
+                for (int i2 = 0; i2 < 4; i2++) o[j][i2] *= corr[i2 & 1];
         }
         asm volatile("cp.async.wait_group %0;" ::"n"(2 * T::AHEAD - 1) : "memory");  // the values
         sync();
@@ -638,9 +624,8 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, WARPS)) kv8_attn_sm
 #pragma unroll
                 for (int j = 0; j < T::VS; j++) bad |= nan_bytes(vw[j].x) | nan_bytes(vw[j].y) | nan_bytes(vw[j].z) | nan_bytes(vw[j].w);
                 if (__any_sync(0xffffffffu, bad != 0)) {
-                    uint32_t sb0[NT], sb1[NT];
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++) sb0[nt] = transpose8x8(seen[k2][nt][0]), sb1[nt] = transpose8x8(seen[k2][nt][1]);
+                    uint32_t sb0, sb1;
+                    sb0 = transpose8x8(seen[k2][0]), sb1 = transpose8x8(seen[k2][1]);
 #pragma unroll
                     for (int j = 0; j < T::VS; j++) {
                         uint32_t w[4] = { vw[j].x, vw[j].y, vw[j].z, vw[j].w };
@@ -654,14 +639,11 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, WARPS)) kv8_attn_sm
                                 f[2 + i2] = ((nb & 0x10000u) ? 0x3c00u : 0u) | ((nb & 0x1000000u) ? 0x3c000000u : 0u);
                                 w[2 * half_ + i2] &= ~nb;
                             }
+                            float hit[4] = {};
+                            mma16816(hit, f[0], f[1], f[2], f[3], sb0, sb1);
 #pragma unroll
-                            for (int nt = 0; nt < NT; nt++) {
-                                float hit[4] = {};
-                                mma16816(hit, f[0], f[1], f[2], f[3], sb0[nt], sb1[nt]);
-#pragma unroll
-                                for (int i2 = 0; i2 < 4; i2++)
-                                    if (hit[i2] > 0.0f) o[nt][2 * j + half_][i2] = __int_as_float(0x7fffffff);
-                            }
+                            for (int i2 = 0; i2 < 4; i2++)
+                                if (hit[i2] > 0.0f) o[2 * j + half_][i2] = __int_as_float(0x7fffffff);
                         }
                         vw[j] = make_uint4(w[0], w[1], w[2], w[3]);
                     }
@@ -674,8 +656,7 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, WARPS)) kv8_attn_sm
                 for (int half_ = 0; half_ < 2; half_++) {
                     const uint32_t a0 = e4m3x2_to_h2((uint16_t) w[2 * half_]), a2 = e4m3x2_to_h2((uint16_t) (w[2 * half_] >> 16));
                     const uint32_t a1 = e4m3x2_to_h2((uint16_t) w[2 * half_ + 1]), a3 = e4m3x2_to_h2((uint16_t) (w[2 * half_ + 1] >> 16));
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++) mma16816(o[nt][2 * j + half_], a0, a1, a2, a3, wb[k2][nt][0], wb[k2][nt][1]);
+                    mma16816(o[2 * j + half_], a0, a1, a2, a3, wb[k2][0], wb[k2][1]);
                 }
             }
         }
@@ -688,22 +669,19 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, WARPS)) kv8_attn_sm
 
     // the warps' states to shared memory: [row][element]; element of (mt, half, g): 32 (mt/2) + 4 g + 2 (mt%2) + half
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            float x = l[nt][i];
-            x += __shfl_xor_sync(0xffffffffu, x, 4);
-            x += __shfl_xor_sync(0xffffffffu, x, 8);
-            x += __shfl_xor_sync(0xffffffffu, x, 16);
-            if (g == 0) sm_ml[warp][8 * nt + 2 * t + i][0] = m[nt][i], sm_ml[warp][8 * nt + 2 * t + i][1] = x;
-        }
-#pragma unroll
-        for (int j = 0; j < T::VS; j++)
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-                *reinterpret_cast<float4 *>(&sm_o[warp][8 * nt + 2 * t + i][32 * j + 4 * g]) =
-                    make_float4(o[nt][2 * j][i], o[nt][2 * j][2 + i], o[nt][2 * j + 1][i], o[nt][2 * j + 1][2 + i]);
+    for (int i = 0; i < 2; i++) {
+        float x = l[i];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        if (g == 0) sm_ml[warp][2 * t + i][0] = m[i], sm_ml[warp][2 * t + i][1] = x;
     }
+#pragma unroll
+    for (int j = 0; j < T::VS; j++)
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            *reinterpret_cast<float4 *>(&sm_o[warp][2 * t + i][32 * j + 4 * g]) =
+                make_float4(o[2 * j][i], o[2 * j][2 + i], o[2 * j + 1][i], o[2 * j + 1][2 + i]);
     __syncthreads();
     const int live = min(T::ROWS, rows - row0);
     const size_t unit = ((size_t) b * a.row_tiles + tile) * kv.n_kv + h;
@@ -899,7 +877,7 @@ void run_read(const ReadArgs & a, cudaStream_t s) {
 // How the rows and the cache of a call are cut up.
 struct Plan {
     bool tile = false;      // kv8_tile.cu's kernel
-    int warps = 4;          // else: of a CTA of the few-row kernel
+    int warps = 4;          // of a CTA of the few-row kernel
     int rows = 8;           // rows of a CTA: 8, each warp working on all of them, or 8 for each warp
     int row_tiles = 1, chunks = 1, chunk_blocks = 1;
 };

@@ -264,6 +264,104 @@ def test_attention_matches_64_bit(pkg, H, KV, hd, kind, page, layout, window, ca
     check_attention(pool, q, out, lse, seqs, scale, window, causal, kind)
 
 
+# rows of a kv head (tokens x group) on both sides of every change of kernel and tile, and contexts that are split
+EDGES = [(1, 8, 70), (1, 9, 70), (3, 5, 300), (8, 8, 100), (13, 5, 500), (16, 4, 64), (21, 3, 40), (64, 1, 33), (65, 1, 200),
+         (32, 4, 900), (129, 2, 129), (257, 1, 300), (43, 6, 2100), (2, 12, 6000), (90, 3, 5000)]
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new,group,L", EDGES)
+def test_attention_at_the_edges_of_its_tiles(pkg, hd, new, group, L):
+    new = min(new, L)
+    pool = Pool(pkg, [L], 1, hd, 16, seed=L + new, fill=[L])
+    q = torch.from_numpy(np.random.default_rng(new).standard_normal((new, group, hd)).astype(np.float32)).cuda().half()
+    out, lse = torch.full_like(q, float("nan")), torch.full((new, group), float("nan"), device="cuda")
+    pool.cache.attention(pool.batch([new], [L]), q, out, 0.1, lse=lse)
+    pool.cache.check()
+    check_attention(pool, q, out, lse, [(L - new, new)], 0.1, 0, True, "f16")
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-30, 3.0])
+def test_attention_scales(pkg, new, scale):
+    """Any finite scale: a negative one, none, and one that leaves a single key."""
+    pool = Pool(pkg, [90], 2, 64, seed=2, fill=[90])
+    q = torch.from_numpy(np.random.default_rng(9).standard_normal((new, 4, 64)).astype(np.float32)).cuda().half()
+    out, lse = torch.zeros_like(q), torch.zeros((new, 4), device="cuda")
+    pool.cache.attention(pool.batch([new], [90]), q, out, scale, lse=lse)
+    check_attention(pool, q, out, lse, [(90 - new, new)], scale, 0, True, "f16")
+    with pytest.raises(RuntimeError, match="finite"):
+        pool.cache.attention(pool.batch([new], [90]), q, out, float("inf"))
+
+
+def test_contexts_longer_than_one_range_with_many_sequences(pkg):
+    """More positions than a CTA's range may hold, in a batch that would otherwise not be split: sequences that
+    share their pages all give the one answer."""
+    L, n, KV, hd = 9000, 150, 8, 64
+    pool = Pool(pkg, [L], KV, hd, 64, seed=3, fill=[L])
+    q1 = torch.from_numpy(np.random.default_rng(5).standard_normal((1, 16, hd)).astype(np.float32)).cuda().half()
+    q = q1.expand(n, 16, hd).contiguous()
+    table = pool.table[int(pool.slots_np[0])][None].expand(n, -1).contiguous()
+    cache = pkg.KV8Cache(pool.pages, pool.scales, table)
+    batch = pkg.KV8Batch(torch.arange(n + 1, dtype=torch.int32, device="cuda"), torch.full((n,), L, dtype=torch.int32, device="cuda"),
+                         n, 1, L)
+    out, lse = torch.zeros_like(q), torch.zeros((n, 16), device="cuda")
+    cache.attention(batch, q, out, 0.125, lse=lse)
+    cache.check()
+    assert torch.equal(out, out[:1].expand_as(out)) and torch.equal(lse, lse[:1].expand_as(lse))
+    check_attention(pool, q1, out[:1], lse[:1], [(L - 1, 1)], 0.125, 0, True, "f16")
+
+
+def test_ragged_rows_of_one_call(pkg):
+    """Sequences with one row, with none and with hundreds in the same call, and bounds larger than any of them."""
+    seqs = [(5, 1), (100, 0), (0, 260), (40, 7), (1000, 1), (3, 64)]
+    lens, news = [a + b for a, b in seqs], [s[1] for s in seqs]
+    pool = Pool(pkg, lens, 2, 64, 32, seed=21, fill=lens)
+    n = sum(news)
+    q = torch.from_numpy(np.random.default_rng(3).standard_normal((n, 6, 64)).astype(np.float32)).cuda().bfloat16()
+    out, lse = torch.full_like(q, float("nan")), torch.full((n, 6), float("nan"), device="cuda")
+    pool.cache.attention(pool.batch(news, lens, max_new=300, max_len=1024), q, out, 0.125, lse=lse)
+    pool.cache.check()
+    check_attention(pool, q, out, lse, seqs, 0.125, 0, True, "bf16")
+
+
+def test_c_calls_with_a_workspace_of_any_content(pkg):
+    """The C entry points on plain pointers: the workspace's content does not matter, its size does."""
+    import ctypes
+    from bz_ggml_b200.kv8 import _Batch, _Cache
+    lib = pkg.lib().lib
+    pool = Pool(pkg, [3000], 2, 128, seed=6, fill=[3000])
+
+    class Rows(ctypes.Structure):
+        _fields_ = [("data", ctypes.c_void_p), ("row", ctypes.c_longlong), ("head", ctypes.c_longlong), ("n", ctypes.c_int),
+                    ("type", ctypes.c_int)]
+
+    q = torch.from_numpy(np.random.default_rng(8).standard_normal((1, 4, 128)).astype(np.float32)).cuda().half()
+    batch = pool.batch([1], [3000])
+    c, b = ctypes.byref(pool.cache._c), ctypes.byref(batch._c)
+    need = lib.bzb_kv8_attention_workspace(c, b, 4, 1, 0)
+    assert need > 0
+    stream = torch.cuda.current_stream().cuda_stream
+    got = []
+    for fill in (0, 255, 127):
+        ws = torch.full((need + 64,), fill, dtype=torch.uint8, device="cuda")
+        out = torch.zeros_like(q)
+        rq, ro = (ctypes.byref(Rows(t.data_ptr(), 512, 128, 4, 1)) for t in (q, out))
+        assert lib.bzb_kv8_attention(c, b, rq, ro, None, 0.09, 1, 0, ws.data_ptr(), need, stream) == 0
+        torch.cuda.synchronize()
+        assert (ws[need:] == fill).all(), "wrote past the workspace"
+        got.append(out)
+        assert lib.bzb_kv8_attention(c, b, rq, ro, None, 0.09, 1, 0, ws.data_ptr(), need - 1, stream) == -1
+        assert b"workspace" in lib.breeze_last_error()
+        assert lib.bzb_kv8_attention(c, b, rq, ro, None, 0.09, 1, 0, None, need, stream) == -1
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+    lse = torch.zeros((1, 4), device="cuda")
+    pool.cache.attention(batch, q, out, 0.09, lse=lse)
+    assert torch.equal(out, got[0])
+    check_attention(pool, q, out, lse, [(2999, 1)], 0.09, 0, True, "f16")
+    assert isinstance(pool.cache._c, _Cache) and isinstance(batch._c, _Batch)
+
+
 @pytest.mark.parametrize("new", [1, 3, 150])
 def test_attention_with_value_scales_far_apart(pkg, new):
     """Blocks whose scales differ by 2^40: weights carry the values' scales, sums must not."""
