@@ -74,28 +74,23 @@ struct AppendArgs {
     bool q_out_vec, norm_vec;
 };
 
-template <int HD, int TYPE, bool VEC>
-__global__ void __launch_bounds__(32 * kRowWarps, 5) kv8_append_kernel(const AppendArgs a) {
+// FULL: all 16 positions of the block are new
+template <int HD, int TYPE, bool VEC, bool FULL>
+__device__ __forceinline__ void append_block(const AppendArgs & a, const Seq & s, int first, int blk, float * tops) {
     using R = RowMap<HD>;
-    __shared__ float tops[kRowWarps];
     const Kv & kv = a.kv;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = lane % R::LPR;
     const int r0 = warp % R::WPB * (16 / R::WPB) + lane / R::LPR * 4;  // the lane's first row of the block
-    start_after_previous();
-    const Seq s = load_seq(kv, (int) blockIdx.z);
-    if (s.slot < 0) return;
-    const int first = s.len - s.n;  // position of the sequence's first row (negative: padding rows)
-    const int blk = (max(first, 0) >> 4) + (int) blockIdx.y, p0 = blk << 4;
-    if (p0 >= s.len || s.n == 0) return;  // (the whole CTA, as above)
+    const int p0 = blk << 4;
     const int nq = a.n_head, nkv = kv.n_kv;
     const int any = (int) blockIdx.x * R::HEADS + warp / R::WPB;
     const int kind = any < nq ? 0 : any < nq + nkv ? 1 : any < nq + 2 * nkv ? 2 : 3;
     const int head = kind == 0 ? any : kind == 1 ? any - nq : any - nq - nkv;
     const Rows src = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-    const int live_lo = max(first - p0, 0), live_hi = min(16, s.len - p0);  // the block's new rows
+    const int live_lo = FULL ? 0 : max(first - p0, 0), live_hi = FULL ? 16 : min(16, s.len - p0);  // the block's new rows
     bool live[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) live[i] = kind < 3 && r0 + i >= live_lo && r0 + i < live_hi;
+    for (int i = 0; i < 4; i++) live[i] = kind < 3 && (FULL || (r0 + i >= live_lo && r0 + i < live_hi));
     const long long row = s.row0 + p0 + r0 - first;  // packed row of the lane's first position
 
     // rows, (cos, sin) and weights on the way together
@@ -123,7 +118,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 5) kv8_append_kernel(const App
         wl = a.norm_vec ? load4<BZB_F32, true>(w, 4 * c) : load4<BZB_F32, false>(w, 4 * c);
         wh = a.norm_vec ? load4<BZB_F32, true>(w, HD / 2 + 4 * c) : load4<BZB_F32, false>(w, HD / 2 + 4 * c);
     }
-    const bool cached = kind == 1 || kind == 2, older = cached && p0 < first;  // older: the block holds earlier positions
+    const bool cached = kind == 1 || kind == 2, older = !FULL && cached && p0 < first;  // older: the block holds earlier positions
     const int pg = cached ? page_of(kv, s.slot, blk) : -1;
     uint8_t * dst = pg < 0 ? nullptr : block_ptr(kv, pg, blk, kind - 1, head, HD);
     float * sp = pg < 0 ? nullptr : scale_ptr(kv, pg, blk, kind - 1, head);
@@ -192,16 +187,31 @@ __global__ void __launch_bounds__(32 * kRowWarps, 5) kv8_append_kernel(const App
     // the block's largest finite magnitude; what is not finite becomes NaN
     float top = 0.0f;
     if (cached) {
-        auto finite = [&](float & x) {
-            const float m = fabsf(x);
-            if (m < INFINITY) top = fmaxf(top, m);
-            else x = __int_as_float(0x7fffffff);
+        // (a maximum that keeps NaNs tells whether any value needs a second look)
+        auto larger = [](float m, float x) {
+            float r;
+            asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(x)));
+            return r;
         };
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            finite(lo[i].x), finite(lo[i].y), finite(lo[i].z), finite(lo[i].w);
-            finite(hi[i].x), finite(hi[i].y), finite(hi[i].z), finite(hi[i].w);
+            top = larger(larger(larger(larger(top, lo[i].x), lo[i].y), lo[i].z), lo[i].w);
+            top = larger(larger(larger(larger(top, hi[i].x), hi[i].y), hi[i].z), hi[i].w);
         }
+        if (!(top < INFINITY)) {
+            top = 0.0f;
+            auto finite = [&](float & x) {
+                const float m = fabsf(x);
+                if (m < INFINITY) top = fmaxf(top, m);
+                else x = __int_as_float(0x7fffffff);
+            };
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                finite(lo[i].x), finite(lo[i].y), finite(lo[i].z), finite(lo[i].w);
+                finite(hi[i].x), finite(hi[i].y), finite(hi[i].z), finite(hi[i].w);
+            }
+        }
+        __syncwarp();
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     }
@@ -250,6 +260,19 @@ __global__ void __launch_bounds__(32 * kRowWarps, 5) kv8_append_kernel(const App
                                     word(hi[0].z, hi[1].z, hi[2].z, hi[3].z, old[6]), word(hi[0].w, hi[1].w, hi[2].w, hi[3].w, old[7]));
     }
     if (lane == 0 && warp % R::WPB == 0) *sp = pow2f(e);
+}
+
+template <int HD, int TYPE, bool VEC>
+__global__ void __launch_bounds__(32 * kRowWarps, 6) kv8_append_kernel(const AppendArgs a) {
+    __shared__ float tops[kRowWarps];
+    start_after_previous();
+    const Seq s = load_seq(a.kv, (int) blockIdx.z);
+    if (s.slot < 0) return;
+    const int first = s.len - s.n;  // position of the sequence's first row (negative: padding rows)
+    const int blk = (max(first, 0) >> 4) + (int) blockIdx.y, p0 = blk << 4;
+    if (p0 >= s.len || s.n == 0) return;  // (the whole CTA, as above)
+    if (p0 >= first && p0 + 16 <= s.len) append_block<HD, TYPE, VEC, true>(a, s, first, blk, tops);
+    else append_block<HD, TYPE, VEC, false>(a, s, first, blk, tops);
 }
 
 struct ReadArgs {
