@@ -16,6 +16,9 @@ using namespace kv8;
 
 // ---- append and read ----
 //
+// Append: x' = x rsqrt(mean x^2 + eps) w, pairs (x'_j, x'_{j + hd/2}) turned by (cos, sin), then for keys and values
+// of a block 2^e from its largest magnitude and the bytes. Read: bytes times 2^e.
+//
 // A CTA takes one block of 16 positions of a sequence and a few heads of q, k or v: a warp holds 16 rows of
 // a head of 64, or 8 of one of 128 (two warps share a block, and its maximum through shared memory). A lane
 // holds, of each of four consecutive rows, the four elements from 4c and the four from hd/2 + 4c, c its
@@ -24,6 +27,12 @@ using namespace kv8;
 // issued before the first is used; what an append needs of the page (its scale, earlier bytes) is
 // on the way while the norm and the rotation run. No other CTA touches the block: no atomics, and the
 // same bytes whatever the launch's shape.
+//
+// Bound by loads and the arithmetic between them, not by DRAM: 16384 rows of 32 + 2 x 8 heads of 128 in bf16 are
+// appended in 100 us (363 MB, 3.6 TB/s), 14 of them the (cos, sin) loads, which every head repeats (from L1
+// and L2), and 12 the keys' 64-bit arithmetic. Reading 16 x 700 to 4096 positions of 8 heads of 128 takes 48 us (236 MB,
+// 4.9 TB/s). A batch of 64 single rows: 8.8 us. With a lane on one row the first took 246 us; with 8 warps
+// a CTA it takes 8 us more, with 5 CTAs an SM (fewer spills) 6 more, with one launch for q and one for the cache 10 more.
 constexpr int kRowWarps = 4;
 template <int HD>
 struct RowMap {
@@ -55,10 +64,10 @@ template <int TYPE, bool VEC>
 __device__ __forceinline__ Raw4<TYPE> raw4(const void * p, long long i) {
     Raw4<TYPE> r;
     if constexpr (TYPE == BZB_F32) {
-        r.u = load4<BZB_F32, VEC>(p, i);
+        r.u = load4<VEC>(static_cast<const float *>(p) + i);
     } else {
         const uint16_t * h = static_cast<const uint16_t *>(p) + i;
-        if constexpr (VEC) r.u = __ldg(reinterpret_cast<const uint2 *>(h));
+        if constexpr (VEC) r.u = *reinterpret_cast<const uint2 *>(h);
         else r.u = make_uint2((uint32_t) h[0] | (uint32_t) h[1] << 16, (uint32_t) h[2] | (uint32_t) h[3] << 16);
     }
     return r;
@@ -73,6 +82,38 @@ struct AppendArgs {
     int n_head, q_out_type;
     bool q_out_vec, norm_vec;
 };
+
+// the f32 next to x towards zero, its last bit set where it is not x: rounded once more to fewer bits, it goes
+// the way x would
+__device__ __forceinline__ float to_odd(double x) {
+    const float f = __double2float_rz(x);
+    return (double) f == x ? f : __int_as_float(__float_as_int(f) | 1);
+}
+// a row's norm and rotation in 64 bits, for the lanes of RowMap (without a rotation: cos 1, sin 0)
+template <int HD>
+__device__ __forceinline__ void turn_exactly(float4 & lo, float4 & hi, bool norm, float4 wl, float4 wh, float eps, float4 t0, float4 t1) {
+    double x[4] = { lo.x, lo.y, lo.z, lo.w }, y[4] = { hi.x, hi.y, hi.z, hi.w };
+    if (norm) {
+        const float u[4] = { wl.x, wl.y, wl.z, wl.w }, v[4] = { wh.x, wh.y, wh.z, wh.w };
+        double ss = 0.0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) ss = fma(x[j], x[j], fma(y[j], y[j], ss));
+#pragma unroll
+        for (int o = HD / 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const double r = rsqrt(ss * (1.0 / HD) + (double) eps);
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[j] *= r * u[j], y[j] *= r * v[j];
+    }
+    const float c[4] = { t0.x, t0.z, t1.x, t1.z }, s[4] = { t0.y, t0.w, t1.y, t1.w };
+    float p[4], q[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        p[j] = to_odd(fma(x[j], (double) c[j], -(y[j] * s[j])));
+        q[j] = to_odd(fma(x[j], (double) s[j], y[j] * c[j]));
+    }
+    lo = make_float4(p[0], p[1], p[2], p[3]);
+    hi = make_float4(q[0], q[1], q[2], q[3]);
+}
 
 // FULL: all 16 positions of the block are new
 template <int HD, int TYPE, bool VEC, bool FULL>
@@ -93,31 +134,28 @@ __device__ __forceinline__ void append_block(const AppendArgs & a, const Seq & s
     for (int i = 0; i < 4; i++) live[i] = kind < 3 && (FULL || (r0 + i >= live_lo && r0 + i < live_hi));
     const long long row = s.row0 + p0 + r0 - first;  // packed row of the lane's first position
 
-    // rows, (cos, sin) and weights on the way together
     Raw4<TYPE> lo_raw[4] = {}, hi_raw[4] = {};
-    float4 turn[4][2];  // of pairs 4c, 4c + 1 and of 4c + 2, 4c + 3
     long long at = row * src.row + head * src.head + 4 * c;
-    const bool turned = kind < 2 && a.rope;
 #pragma unroll
     for (int i = 0; i < 4; i++, at += src.row) {
         if (!live[i]) continue;
         lo_raw[i] = raw4<TYPE, VEC>(src.p, at);
         hi_raw[i] = raw4<TYPE, VEC>(src.p, at + HD / 2);
     }
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        turn[i][0] = turn[i][1] = make_float4(1.0f, 0.0f, 1.0f, 0.0f);
-        if (!live[i] || !turned) continue;
-        const float4 * t = reinterpret_cast<const float4 *>(a.rope + (size_t) (p0 + r0 + i) * (HD / 2) + 4 * c);
-        turn[i][0] = __ldg(t);
-        turn[i][1] = __ldg(t + 1);
-    }
     const float * w = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
     float4 wl = make_float4(0.0f, 0.0f, 0.0f, 0.0f), wh = wl;
     if (w) {
-        wl = a.norm_vec ? load4<BZB_F32, true>(w, 4 * c) : load4<BZB_F32, false>(w, 4 * c);
-        wh = a.norm_vec ? load4<BZB_F32, true>(w, HD / 2 + 4 * c) : load4<BZB_F32, false>(w, HD / 2 + 4 * c);
+        wl = a.norm_vec ? load4<true>(w + 4 * c) : load4<false>(w + 4 * c);
+        wh = a.norm_vec ? load4<true>(w + HD / 2 + 4 * c) : load4<false>(w + HD / 2 + 4 * c);
     }
+    // row i's (cos, sin) of pairs 4c, 4c + 1 and of 4c + 2, 4c + 3
+    auto turn_of = [&](int i, float4 & t0, float4 & t1) {
+        t0 = t1 = make_float4(1.0f, 0.0f, 1.0f, 0.0f);
+        if (!live[i] || !a.rope) return;
+        const float4 * t = reinterpret_cast<const float4 *>(a.rope + (size_t) (p0 + r0 + i) * (HD / 2) + 4 * c);
+        t0 = t[0];
+        t1 = t[1];
+    };
     const bool cached = kind == 1 || kind == 2, older = !FULL && cached && p0 < first;  // older: the block holds earlier positions
     const int pg = cached ? page_of(kv, s.slot, blk) : -1;
     uint8_t * dst = pg < 0 ? nullptr : block_ptr(kv, pg, blk, kind - 1, head, HD);
@@ -143,44 +181,55 @@ __device__ __forceinline__ void append_block(const AppendArgs & a, const Seq & s
         }
     }
     float4 lo[4], hi[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) lo[i] = lo_raw[i].value(), hi[i] = hi_raw[i].value();
-    if (w) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            float4 & x = lo[i], & y = hi[i];
-            float2 sq = __fmul2_rn(make_float2(x.x, x.y), make_float2(x.x, x.y));
-            sq = __ffma2_rn(make_float2(x.z, x.w), make_float2(x.z, x.w), sq);
-            sq = __ffma2_rn(make_float2(y.x, y.y), make_float2(y.x, y.y), sq);
-            sq = __ffma2_rn(make_float2(y.z, y.w), make_float2(y.z, y.w), sq);
-            float ss = sq.x + sq.y;
-#pragma unroll
-            for (int o = R::LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            const float r = rsqrtf(ss * (1.0f / HD) + a.eps);
-            auto scale = [&](float4 & v, const float4 & w) {
-                const float2 p = __fmul2_rn(__fmul2_rn(make_float2(v.x, v.y), make_float2(r, r)), make_float2(w.x, w.y));
-                const float2 q = __fmul2_rn(__fmul2_rn(make_float2(v.z, v.w), make_float2(r, r)), make_float2(w.z, w.w));
-                v = make_float4(p.x, p.y, q.x, q.y);
-            };
-            scale(x, wl);
-            scale(y, wh);
-        }
-    }
-    if (turned) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float4 t0 = turn[i][0], t1 = turn[i][1], x = lo[i], y = hi[i];
-            lo[i] = make_float4(x.x * t0.x - y.x * t0.y, x.y * t0.z - y.y * t0.w, x.z * t1.x - y.z * t1.y, x.w * t1.z - y.w * t1.w);
-            hi[i] = make_float4(x.x * t0.y + y.x * t0.x, x.y * t0.w + y.y * t0.z, x.z * t1.y + y.z * t1.x, x.w * t1.w + y.w * t1.z);
-        }
-    }
     if (kind == 0) {
-        long long at = row * a.q_out.row + head * a.q_out.head + 4 * c;
+        // (the table's loads of all rows are on the way while the norms are summed)
+        float4 turn[4][2];
 #pragma unroll
-        for (int i = 0; i < 4; i++, at += a.q_out.row) {
+        for (int i = 0; i < 4; i++) turn_of(i, turn[i][0], turn[i][1]);
+        long long to = row * a.q_out.row + head * a.q_out.head + 4 * c;
+#pragma unroll
+        for (int i = 0; i < 4; i++, to += a.q_out.row) {
+            if (!FULL && !__any_sync(0xffffffffu, live[i])) continue;
+            float4 x = lo_raw[i].value(), y = hi_raw[i].value();
+            if (w) {
+                float2 sq = __fmul2_rn(make_float2(x.x, x.y), make_float2(x.x, x.y));
+                sq = __ffma2_rn(make_float2(x.z, x.w), make_float2(x.z, x.w), sq);
+                sq = __ffma2_rn(make_float2(y.x, y.y), make_float2(y.x, y.y), sq);
+                sq = __ffma2_rn(make_float2(y.z, y.w), make_float2(y.z, y.w), sq);
+                float ss = sq.x + sq.y;
+#pragma unroll
+                for (int o = R::LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                const float r = rsqrtf(ss * (1.0f / HD) + a.eps);
+                auto scale = [&](float4 & v, const float4 & w) {
+                    const float2 p = __fmul2_rn(__fmul2_rn(make_float2(v.x, v.y), make_float2(r, r)), make_float2(w.x, w.y));
+                    const float2 q = __fmul2_rn(__fmul2_rn(make_float2(v.z, v.w), make_float2(r, r)), make_float2(w.z, w.w));
+                    v = make_float4(p.x, p.y, q.x, q.y);
+                };
+                scale(x, wl);
+                scale(y, wh);
+            }
+            const float4 t0 = turn[i][0], t1 = turn[i][1];
             if (!live[i]) continue;
-            store4(a.q_out_type, a.q_out_vec, a.q_out.p, at, lo[i]);
-            store4(a.q_out_type, a.q_out_vec, a.q_out.p, at + HD / 2, hi[i]);
+            store4(a.q_out_type, a.q_out_vec, a.q_out.p, to,
+                   make_float4(x.x * t0.x - y.x * t0.y, x.y * t0.z - y.y * t0.w, x.z * t1.x - y.z * t1.y, x.w * t1.z - y.w * t1.w));
+            store4(a.q_out_type, a.q_out_vec, a.q_out.p, to + HD / 2,
+                   make_float4(x.x * t0.y + y.x * t0.x, x.y * t0.w + y.y * t0.z, x.z * t1.y + y.z * t1.x, x.w * t1.w + y.w * t1.z));
+        }
+    } else {
+        const bool exact = kind == 1 && (w || a.rope);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            lo[i] = lo_raw[i].value();
+            hi[i] = hi_raw[i].value();
+            // Keys in 64 bits, then to odd f32: every cached byte is the correctly rounded one. (In f32, which took
+            // 10 % less time, three of a million fell on the other side of a tie.)
+            if (exact && (FULL || __any_sync(0xffffffffu, live[i]))) {
+                float4 t0, t1;
+                turn_of(i, t0, t1);
+                turn_exactly<HD>(lo[i], hi[i], w != nullptr, wl, wh, a.eps, t0, t1);
+            }
+            // (a row that is not there has norm zero, which without eps is no number)
+            if (!live[i]) lo[i] = hi[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
     }
 
@@ -301,20 +350,20 @@ __global__ void __launch_bounds__(32 * kRowWarps) kv8_read_kernel(const ReadArgs
     if (blk >= 0) {
         const int pg = max(page_of(kv, s.slot, blk), 0);
         const uint8_t * src = block_ptr(kv, pg, blk, plane, head, HD);
-        const float scale = __ldg(scale_ptr(kv, pg, blk, plane, head));
+        const float scale = *scale_ptr(kv, pg, blk, plane, head);
         uint32_t w[8];
         if (plane == 0) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const uint32_t * row = reinterpret_cast<const uint32_t *>(src + (r0 + i) * HD);
-                w[2 * i] = __ldg(row + c);
-                w[2 * i + 1] = __ldg(row + c + HD / 8);
+                w[2 * i] = row[c];
+                w[2 * i + 1] = row[c + HD / 8];
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) lo[i] = e4m3x4_to_f4(w[2 * i]), hi[i] = e4m3x4_to_f4(w[2 * i + 1]);
         } else {
             const uint4 * pl = reinterpret_cast<const uint4 *>(src + c * 64 + r0 * 4);
-            const uint4 x = __ldg(pl), y = __ldg(pl + HD / 8 * 4);
+            const uint4 x = pl[0], y = pl[HD / 8 * 4];
             auto patch = [&](float4 (&o)[4], uint4 w) {
                 const float4 e0 = e4m3x4_to_f4(w.x), e1 = e4m3x4_to_f4(w.y), e2 = e4m3x4_to_f4(w.z), e3 = e4m3x4_to_f4(w.w);
                 o[0] = make_float4(e0.x, e1.x, e2.x, e3.x);
@@ -469,7 +518,7 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, WARPS)) kv8_attn_sm
     if (me < n) {
         const int blk = base + me * STRIDE, pg = max(page_of(kv, s.slot, blk), 0);
         block_at[mine0 + me] = block_ptr(kv, pg, blk, 0, h, HD);
-        sc0 = make_float2(__ldg(scale_ptr(kv, pg, blk, 0, h)), __ldg(scale_ptr(kv, pg, blk, 1, h)));
+        sc0 = make_float2(*scale_ptr(kv, pg, blk, 0, h), *scale_ptr(kv, pg, blk, 1, h));
     }
     sync();
     const int kpos = (g >> 1) * 4 + (g & 1);  // the lane's key rows: kpos and kpos + 2 (see the patches' position order)
@@ -506,7 +555,7 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, WARPS)) kv8_attn_sm
     for (int i = me + FINDERS; i < n; i += FINDERS) {
         const int blk = base + i * STRIDE, pg = max(page_of(kv, s.slot, blk), 0);
         block_at[mine0 + i] = block_ptr(kv, pg, blk, 0, h, HD);
-        scales[mine0 + i] = make_float2(__ldg(scale_ptr(kv, pg, blk, 0, h)), __ldg(scale_ptr(kv, pg, blk, 1, h)));
+        scales[mine0 + i] = make_float2(*scale_ptr(kv, pg, blk, 0, h), *scale_ptr(kv, pg, blk, 1, h));
     }
     sync();
 

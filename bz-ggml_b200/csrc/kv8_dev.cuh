@@ -69,7 +69,7 @@ __device__ __forceinline__ Seq load_seq(const Kv & kv, int b) {
 
 // the page of block `blk` (16 positions) of a sequence, or -1
 __device__ __forceinline__ int page_of(const Kv & kv, int slot, int blk) {
-    const int pg = __ldg(kv.table + (size_t) slot * kv.max_pages + (blk >> (kv.page_shift - 4)));
+    const int pg = kv.table[(size_t) slot * kv.max_pages + (blk >> (kv.page_shift - 4))];
     if ((unsigned) pg >= (unsigned) kv.n_pages) {
         complain(kv);
         return -1;
@@ -113,31 +113,11 @@ __device__ __forceinline__ float4 e4m3x4_to_f4(uint32_t w) {
     return make_float4(a.x, a.y, b.x, b.y);
 }
 
-// ---- four consecutive elements of a row, by type; VEC: they are aligned to their size ----
-template <int TYPE, bool VEC>
-__device__ __forceinline__ float4 load4(const void * p, long long i) {
-    if constexpr (TYPE == BZB_F32) {
-        const float * f = static_cast<const float *>(p) + i;
-        if constexpr (VEC) return __ldg(reinterpret_cast<const float4 *>(f));
-        return make_float4(f[0], f[1], f[2], f[3]);
-    } else if constexpr (TYPE == BZB_F16) {
-        const half * h = static_cast<const half *>(p) + i;
-        if constexpr (VEC) {
-            const uint2 u = __ldg(reinterpret_cast<const uint2 *>(h));
-            const float2 a = __half22float2(*reinterpret_cast<const half2 *>(&u.x));
-            const float2 b = __half22float2(*reinterpret_cast<const half2 *>(&u.y));
-            return make_float4(a.x, a.y, b.x, b.y);
-        }
-        return make_float4(__half2float(h[0]), __half2float(h[1]), __half2float(h[2]), __half2float(h[3]));
-    } else {
-        const __nv_bfloat16 * h = static_cast<const __nv_bfloat16 *>(p) + i;
-        if constexpr (VEC) {
-            const uint2 u = __ldg(reinterpret_cast<const uint2 *>(h));
-            return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
-                               __uint_as_float(u.y & 0xffff0000u));
-        }
-        return make_float4(__bfloat162float(h[0]), __bfloat162float(h[1]), __bfloat162float(h[2]), __bfloat162float(h[3]));
-    }
+// ---- four consecutive elements of a row; VEC: they are aligned to their size ----
+template <bool VEC>
+__device__ __forceinline__ float4 load4(const float * f) {
+    if constexpr (VEC) return *reinterpret_cast<const float4 *>(f);
+    return make_float4(f[0], f[1], f[2], f[3]);
 }
 __device__ __forceinline__ uint32_t pack_half(float a, float b) {
     const half2 h = __floats2half2_rn(a, b);
@@ -241,7 +221,9 @@ void launch_chained(void (*kernel)(P...), dim3 grid, int threads, int shared, cu
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
     if (e != cudaSuccess) throw std::runtime_error(std::string("launch: ") + cudaGetErrorString(e));
 }
-// lets the next kernel's CTAs be placed, then waits until the kernels before this one are done and their writes visible
+// Lets the next kernel's CTAs be placed, then waits until the kernels before this one are done and their writes visible.
+// What they may have written -- which for a caller's buffers is everything -- is read with ordinary loads:
+// the compiler is free to move non-coherent ones (__ldg) ahead of this wait.
 __device__ __forceinline__ void start_after_previous() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");

@@ -241,7 +241,7 @@ struct Keys {
         for (int i = 0; i < N; i++) {
             const uint8_t * p = shfl_ptr(block, first + step * i);
             x[i] = make_uint4(0, 0, 0, 0);
-            if (p) x[i] = __ldg(reinterpret_cast<const uint4 *>(p + in_block));
+            if (p) x[i] = *reinterpret_cast<const uint4 *>(p + in_block);
         }
     }
     __device__ void store(uint8_t * tile, uint32_t factor) const {
@@ -280,8 +280,8 @@ struct Values {
             x[i][0] = x[i][1] = make_uint4(0, 0, 0, 0);
             if (p) {
                 const uint4 * src = reinterpret_cast<const uint4 *>(p + in_block + quads_of(i) * 64);
-                x[i][0] = __ldg(src);
-                x[i][1] = __ldg(src + 1);
+                x[i][0] = src[0];
+                x[i][1] = src[1];
             }
         }
     }
@@ -566,8 +566,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
         float ks = 0.0f, vs = 0.0f;
         auto load_scales = [&](int j) {
             if (pg < 0) return;
-            ks = __ldg(scale_ptr(a.kv, pg, w.blk0 + 8 * j + (lane & 7), 0, w.h));
-            vs = __ldg(scale_ptr(a.kv, pg, w.blk0 + 8 * j + (lane & 7), 1, w.h));
+            ks = *scale_ptr(a.kv, pg, w.blk0 + 8 * j + (lane & 7), 0, w.h);
+            vs = *scale_ptr(a.kv, pg, w.blk0 + 8 * j + (lane & 7), 1, w.h);
         };
         k.load(block(pg, 0, 0));
         v.load(block(pg, 0, 1));

@@ -189,6 +189,24 @@ def test_append_extreme_values(pkg):
     check_append(pool, 0, 0, len(x))
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+def test_keys_are_the_correctly_rounded_ones(pkg, hd):
+    """Normed and rotated keys are rounded once, from the exact value: byte for byte the 64-bit result's. Without eps
+    too, in whole blocks and in one whose last positions are empty (and stay zero)."""
+    rng = np.random.default_rng(hd)
+    n = 16 * 900 + 5
+    x = rng.standard_normal((n, 1, hd)).astype(np.float32)
+    w = (1 + 0.3 * rng.standard_normal(hd)).astype(np.float32)
+    table = rope_table(n, hd)
+    pool = Pool(pkg, [n], 1, hd, 256, seed=1)
+    g = lambda a: torch.from_numpy(a).cuda()  # noqa: E731
+    pool.cache.append(pool.batch([n], [n]), None, g(x), g(x), None, k_norm=g(w), eps=0.0, rope=g(table))
+    append_expected(pool, 0, turned(x, w, 0.0, table), x.astype(np.float64), 0)
+    got, e, behind = pool.held(0, n)
+    assert np.array_equal(e, pool.exps[0]) and not behind.any()
+    assert np.array_equal(got, round_e4m3(pool.values[0]))
+
+
 def test_padding_rows_and_empty_sequences(pkg):
     rng = np.random.default_rng(8)
     pool = Pool(pkg, [20, 20, 20, 20], 2, 64, seed=4, fill=[0, 0, 12, 0])
