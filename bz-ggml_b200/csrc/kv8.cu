@@ -6,6 +6,8 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <cstdlib>
+#include <cstring>
 #include <stdexcept>
 #include <string>
 
@@ -438,11 +440,15 @@ __device__ __forceinline__ void load_q16(const AttnArgs & a, long long i, float 
     for (int j = 0; j < 8; j++) o[j] = pack_half(x[2 * j] * f, x[2 * j + 1] * f);
 }
 
-// Few query rows (a step of each sequence, or a few guessed tokens): one CTA per (sequence, kv head, tile
-// of rows, range of the cache), taking two blocks of 16 positions at a time. The rows of a kv head are (token,
-// head of the group) pairs, so a block read once serves the whole group. Up to 8 rows: the warps share out
-// the range's blocks, each with a ring of its own, and join their results (SHARED false). More: each warp has
-// 8 of the rows and all read every block from one ring (SHARED true).
+// Few query rows (a step of each sequence, a few guessed tokens, short prompts): o = sum_j w_j v_j / sum_j w_j 2^-e_j,
+// w_j = 2^(s_j + e_j - M), s_j = scale log2(e) q k_j, 2^e_j the values' scale, M the running maximum of
+// s_j + e_j. One CTA per (sequence, kv head, 8 rows, range of the cache); the rows of a kv head are (token, head of the
+// group) pairs, so a block read once serves the group. Four warps share out the range's blocks, two at a time,
+// each with a ring of its own, and join their results at the end.
+//
+// Calls with more than 8 rows have more CTAs, which read the same blocks from L2 at about the same time: against a CTA
+// with one ring for all rows, a warp for each 8, which waits on all its warps twice for each pair of blocks, that takes
+// 20 against 21 us (16 sequences of 2000, 16 rows), 23 against 34 (64 of 1000, 16 rows), 40 against 49 (32 rows).
 //
 // The matrix products are m16n8k16 with the cache as the 16-row operand: S^T = K Q^T (16 positions x 8
 // rows) and O^T = V^T W^T (16 of head_dim x 8 rows): no half of a tile is empty when a group has at
@@ -451,17 +457,23 @@ __device__ __forceinline__ void load_q16(const AttnArgs & a, long long i, float 
 // order: no transposition but the 8x8 one of the weights. The blocks are copied as they lie in memory
 // (cp.async), AHEAD pairs in advance: a pair's keys as soon as the scores are done with the pair that had
 // their place, its values after the second product.
+//
+// Bound by DRAM with long contexts (8 sequences of 32000 positions, 8 kv heads of 128, 4 rows: 532 MB in 93 us,
+// 5.7 TB/s; loads into registers instead of rings: 133). Ragged steps (64 sequences of 90 to 2030 positions, 8 kv heads
+// of 64, 4 rows: 70 MB in 23 us, 3.0 TB/s) are bound by latency: 5 us from the sequence through its page to the data,
+// then the longest contexts; 17 us remain without the arithmetic. One sequence of 218 positions: 4.3 us, a launch.
+constexpr int kSmallWarps = 4, kSmallRows = 8;
 constexpr int kSmallBlocks = 512;  // blocks of a range at most
 
 // CTAs that an SM holds, by their registers (96 and 128 a thread)
-constexpr int small_ctas(int hd, int warps) { return (hd == 64 ? 20 : 16) / warps; }
+constexpr int small_ctas(int hd) { return (hd == 64 ? 20 : 16) / kSmallWarps; }
 
-template <int HD, int WARPS, bool SHARED>
+template <int HD>
 struct SmallTile {
-    static constexpr int ROWS = SHARED ? 8 * WARPS : 8, KS = HD / 64, VS = HD / 32, MT = HD / 16, PL = HD + 4;
+    static constexpr int KS = HD / 64, VS = HD / 32, MT = HD / 16, PL = HD + 4;
     static constexpr int PIECES = 2 * KS + VS;            // 512-byte pieces of a block
-    static constexpr int AHEAD = SHARED ? 4 : HD == 64 ? 2 : 1;  // pairs of blocks that a ring holds
-    static constexpr int RING = (SHARED ? 1 : WARPS) * AHEAD * 2 * PIECES * 512, MERGE = WARPS * 8 * (HD + 4) * 4;
+    static constexpr int AHEAD = HD == 64 ? 2 : 1;        // pairs of blocks that a warp's ring holds
+    static constexpr int RING = kSmallWarps * AHEAD * 2 * PIECES * 512, MERGE = kSmallWarps * kSmallRows * PL * 4;
     static constexpr int BYTES = RING > MERGE ? RING : MERGE;
 };
 
@@ -474,12 +486,11 @@ __device__ __forceinline__ uint4 lds16(uint32_t a) {
     return v;
 }
 
-template <int HD, int WARPS, bool SHARED>
-__global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, WARPS)) kv8_attn_small_kernel(const AttnArgs a) {
-    using T = SmallTile<HD, WARPS, SHARED>;
-    constexpr int STRIDE = SHARED ? 1 : WARPS;  // between the blocks of a warp
+template <int HD>
+__global__ void __launch_bounds__(32 * kSmallWarps, small_ctas(HD)) kv8_attn_small_kernel(const AttnArgs a) {
+    using T = SmallTile<HD>;
     extern __shared__ __align__(16) uint8_t ring[];
-    __shared__ float sm_ml[WARPS][8][2];
+    __shared__ float sm_ml[kSmallWarps][kSmallRows][2];
     // the range's blocks: the head's keys (its values lie one plane on), the scales of both
     __shared__ const uint8_t * block_at[kSmallBlocks];
     __shared__ float2 scales[kSmallBlocks];
@@ -495,35 +506,29 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, WARPS)) kv8_attn_sm
     start_after_previous();
     const Seq s = load_seq(kv, b);
     if (s.slot < 0) return;
-    const int row0 = tile * T::ROWS;
-    const Span span = span_of(a, s, row0, T::ROWS);
+    const int row0 = tile * kSmallRows;
+    const Span span = span_of(a, s, row0, kSmallRows);
     const int first = span.first, rows = span.rows, my_chunks = span.chunks;
     if (row0 >= rows || chunk >= my_chunks) return;
-    // this warp's rows, and the keys that all of them see: [full_lo, full_hi)
-    const int wrow0 = row0 + (SHARED ? 8 * warp : 0), last_row = max(wrow0, min(rows - 1, wrow0 + 7));
-    const int full_hi = a.causal ? first + wrow0 / a.group + 1 : s.len;
+    // the keys that all rows see: [full_lo, full_hi)
+    const int last_row = min(rows, row0 + kSmallRows) - 1;
+    const int full_hi = a.causal ? first + row0 / a.group + 1 : s.len;
     const int full_lo = a.window > 0 ? max(0, first + last_row / a.group - a.window + 1) : 0;
     const int c_lo = span.blk_lo + chunk * a.chunk_blocks, c_hi = min(span.blk_hi, c_lo + a.chunk_blocks);
 
-    // this warp's blocks: base, base + STRIDE, ..., looked up by itself (SHARED: by the whole CTA)
-    const int base = c_lo + (SHARED ? 0 : warp), n = max(0, (c_hi - base + STRIDE - 1) / STRIDE);
-    auto sync = [] {
-        if (SHARED) __syncthreads();
-        else __syncwarp();
-    };
-    constexpr int FINDERS = SHARED ? 32 * WARPS : 32;
-    const int me = SHARED ? (int) threadIdx.x : lane, mine0 = SHARED ? 0 : warp * (kSmallBlocks / WARPS);
+    // this warp's blocks: base, base + kSmallWarps, ..., looked up by itself
+    const int base = c_lo + warp, n = max(0, (c_hi - base + kSmallWarps - 1) / kSmallWarps), mine0 = warp * (kSmallBlocks / kSmallWarps);
     // (the first blocks' copies do not wait for their scales)
     float2 sc0 = make_float2(0.0f, 0.0f);
-    if (me < n) {
-        const int blk = base + me * STRIDE, pg = max(page_of(kv, s.slot, blk), 0);
-        block_at[mine0 + me] = block_ptr(kv, pg, blk, 0, h, HD);
+    if (lane < n) {
+        const int blk = base + lane * kSmallWarps, pg = max(page_of(kv, s.slot, blk), 0);
+        block_at[mine0 + lane] = block_ptr(kv, pg, blk, 0, h, HD);
         sc0 = make_float2(*scale_ptr(kv, pg, blk, 0, h), *scale_ptr(kv, pg, blk, 1, h));
     }
-    sync();
+    __syncwarp();
     const int kpos = (g >> 1) * 4 + (g & 1);  // the lane's key rows: kpos and kpos + 2 (see the patches' position order)
     const long long v_at = (long long) kv.n_kv * kv.page_tokens * HD;
-    const uint32_t slots = (uint32_t) __cvta_generic_to_shared(ring) + (SHARED ? 0 : warp) * (T::AHEAD * 2 * T::PIECES * 512);
+    const uint32_t slots = (uint32_t) __cvta_generic_to_shared(ring) + warp * (T::AHEAD * 2 * T::PIECES * 512);
     // where the lane's 16 bytes of 512 go: rows of 128 bytes have their halves swapped in every second row,
     // which keeps the reading lanes on different banks
     const int k_to = HD == 64 ? 16 * lane : (lane >> 3) * 128 + (((lane & 7) ^ ((lane >> 3 & 1) << 2)) << 4);
@@ -535,7 +540,7 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, WARPS)) kv8_attn_sm
 #pragma unroll
         for (int x = 0; x < 2 * (PK > T::VS ? PK : T::VS); x++) {
             const int per = values ? T::VS : PK, k2 = x / per, k = x % per;
-            if (k2 > 1 || (SHARED && x % WARPS != warp)) continue;
+            if (k2 > 1) continue;
             const bool there = i + k2 < n;
             const uint8_t * p = block_at[mine0 + (there ? i + k2 : 0)] + 16 * lane + 512 * k;
             if (values) copy16(slot + (k2 * T::PIECES + PK + k) * 512 + 16 * lane, p + v_at, there);
@@ -546,24 +551,24 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, WARPS)) kv8_attn_sm
     if (n > 0) {
 #pragma unroll
         for (int i = 0; i < T::AHEAD; i++) {
-            // (a range's first 32 blocks, or more, are in the table by now)
+            // (a range's first 32 blocks are in the table by now)
             fetch(2 * i, false);
             fetch(2 * i, true);
         }
     }
-    if (me < n) scales[mine0 + me] = sc0;
-    for (int i = me + FINDERS; i < n; i += FINDERS) {
-        const int blk = base + i * STRIDE, pg = max(page_of(kv, s.slot, blk), 0);
+    if (lane < n) scales[mine0 + lane] = sc0;
+    for (int i = lane + 32; i < n; i += 32) {
+        const int blk = base + i * kSmallWarps, pg = max(page_of(kv, s.slot, blk), 0);
         block_at[mine0 + i] = block_ptr(kv, pg, blk, 0, h, HD);
         scales[mine0 + i] = make_float2(*scale_ptr(kv, pg, blk, 0, h), *scale_ptr(kv, pg, blk, 1, h));
     }
-    sync();
+    __syncwarp();
 
     // queries as the 8-column operand: lane (g, t) holds the warp's row g, elements 64 k + 16 t ..+15
     uint32_t qf[T::KS][8];
     float coef[2];      // the score's factor for the lane's two columns (rows 2 t, 2 t + 1)
     int lim_hi[2], lim_lo[2];
-    const int r = wrow0 + g;
+    const int r = row0 + g;
     float row_unit = 1.0f;
     if (r < rows) {
         const long long at = (long long) (s.row0 + r / a.group) * a.q.row + (h * a.group + r % a.group) * a.q.head + 16 * t;
@@ -589,7 +594,7 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, WARPS)) kv8_attn_sm
     }
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-        const int rr = wrow0 + 2 * t + i, pos = first + rr / a.group;
+        const int rr = row0 + 2 * t + i, pos = first + rr / a.group;
         coef[i] = a.scale2 * __shfl_sync(0xffffffffu, row_unit, (2 * t + i) * 4);
         lim_hi[i] = rr < rows ? (a.causal ? pos + 1 : s.len) : 0;
         lim_lo[i] = a.window > 0 ? pos - a.window + 1 : 0;
@@ -600,7 +605,7 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, WARPS)) kv8_attn_sm
 
     for (int i = 0; i < n; i += 2) {
         asm volatile("cp.async.wait_group %0;" ::"n"(2 * T::AHEAD - 1) : "memory");  // the keys
-        sync();
+        __syncwarp();
         const uint32_t pair = slots + i / 2 % T::AHEAD * 2 * (T::PIECES * 512);
         float x[2][4];  // columns 2t, 2t+1 at key kpos, then at key kpos + 2
         uint32_t seen[2][2];  // (positions x rows) the rows that see each position, as f16 ones
@@ -625,7 +630,7 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, WARPS)) kv8_attn_sm
             const bool there = i + k2 < n;
             const float2 kvs = scales[mine0 + (there ? i + k2 : 0)];
             const float ks = kvs.x, vs = kvs.y;
-            const int key0 = (base + (i + k2) * STRIDE) << 4;
+            const int key0 = (base + (i + k2) * kSmallWarps) << 4;
             const float ev = (float) exponent_of(vs);
             inv_vs[k2] = pow2f(-exponent_of(vs));
             whole[k2] = there && key0 >= full_lo && key0 + 16 <= full_hi;
@@ -646,7 +651,7 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, WARPS)) kv8_attn_sm
             }
         }
         // (also past the end, where it copies zeros: the waits count groups)
-        sync();
+        __syncwarp();
         fetch(i + 2 * T::AHEAD, false);
         uint32_t wb[2][2];
         bool moved = false;
@@ -682,7 +687,7 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, WARPS)) kv8_attn_sm
                 for (int i2 = 0; i2 < 4; i2++) o[j][i2] *= corr[i2 & 1];
         }
         asm volatile("cp.async.wait_group %0;" ::"n"(2 * T::AHEAD - 1) : "memory");  // the values
-        sync();
+        __syncwarp();
 #pragma unroll
         for (int k2 = 0; k2 < 2; k2++) {
             const uint32_t slot = pair + k2 * (T::PIECES * 512) + 16 * lane;
@@ -732,7 +737,7 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, WARPS)) kv8_attn_sm
                 }
             }
         }
-        sync();
+        __syncwarp();
         fetch(i + 2 * T::AHEAD, true);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -755,9 +760,9 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, WARPS)) kv8_attn_sm
             *reinterpret_cast<float4 *>(&sm_o[warp][2 * t + i][32 * j + 4 * g]) =
                 make_float4(o[2 * j][i], o[2 * j][2 + i], o[2 * j + 1][i], o[2 * j + 1][2 + i]);
     __syncthreads();
-    const int live = min(T::ROWS, rows - row0);
+    const int live = min(kSmallRows, rows - row0);
     const size_t unit = ((size_t) b * a.row_tiles + tile) * kv.n_kv + h;
-    float * part = a.part ? a.part + unit * a.chunks * (T::ROWS * T::PL) : nullptr;
+    float * part = a.part ? a.part + unit * a.chunks * (kSmallRows * T::PL) : nullptr;
     auto finish = [&](int r, int d, float4 x, float mm, float ll) {
         const float inv = ll > 0.0f ? 1.0f / ll : (ll == 0.0f ? 0.0f : ll);  // (NaN stays NaN)
         const int rr = row0 + r, tok = s.row0 + rr / a.group, qh = h * a.group + rr % a.group;
@@ -765,29 +770,24 @@ __global__ void __launch_bounds__(32 * WARPS, small_ctas(HD, WARPS)) kv8_attn_sm
                make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
         if (a.lse && d == 0) a.lse[(size_t) tok * a.n_head + qh] = ll == 0.0f ? -INFINITY : kLn2 * (mm + log2f(ll));
     };
-    for (int i = threadIdx.x; i < live * (HD / 4); i += 32 * WARPS) {
+    for (int i = threadIdx.x; i < live * (HD / 4); i += 32 * kSmallWarps) {
         const int r = i / (HD / 4), d = i % (HD / 4) * 4;
         float mm = -INFINITY, ll = 0.0f;
         float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (SHARED) {
-            mm = sm_ml[r >> 3][r & 7][0], ll = sm_ml[r >> 3][r & 7][1];
-            x = *reinterpret_cast<const float4 *>(&sm_o[r >> 3][r & 7][d]);
-        } else {
 #pragma unroll
-            for (int w = 0; w < WARPS; w++) mm = fmaxf(mm, sm_ml[w][r][0]);
-            const float ref = mm == -INFINITY ? 0.0f : mm;
+        for (int w = 0; w < kSmallWarps; w++) mm = fmaxf(mm, sm_ml[w][r][0]);
+        const float ref = mm == -INFINITY ? 0.0f : mm;
 #pragma unroll
-            for (int w = 0; w < WARPS; w++) {
-                const float f = exp2_approx(sm_ml[w][r][0] - ref);
-                const float4 y = *reinterpret_cast<const float4 *>(&sm_o[w][r][d]);
-                ll = fmaf(sm_ml[w][r][1], f, ll);
-                x.x = fmaf(y.x, f, x.x), x.y = fmaf(y.y, f, x.y), x.z = fmaf(y.z, f, x.z), x.w = fmaf(y.w, f, x.w);
-            }
+        for (int w = 0; w < kSmallWarps; w++) {
+            const float f = exp2_approx(sm_ml[w][r][0] - ref);
+            const float4 y = *reinterpret_cast<const float4 *>(&sm_o[w][r][d]);
+            ll = fmaf(sm_ml[w][r][1], f, ll);
+            x.x = fmaf(y.x, f, x.x), x.y = fmaf(y.y, f, x.y), x.z = fmaf(y.z, f, x.z), x.w = fmaf(y.w, f, x.w);
         }
         if (my_chunks == 1) {
             finish(r, d, x, mm, ll);
         } else {
-            float * pp = part + ((size_t) chunk * T::ROWS + r) * T::PL;
+            float * pp = part + ((size_t) chunk * kSmallRows + r) * T::PL;
             *reinterpret_cast<float4 *>(pp + d) = x;
             if (d == 0) *reinterpret_cast<float2 *>(pp + HD) = make_float2(mm, ll);
         }
@@ -946,25 +946,21 @@ void run_read(const ReadArgs & a, cudaStream_t s) {
     launch_chained(kv8_read_kernel<HD, TYPE>, grid, 32 * kRowWarps, 0, s, a);
 }
 
-// How the rows and the cache of a call are cut up.
+// How the rows and the cache of a call are cut up: by which kernel, in tiles of how many rows and ranges of how many
+// blocks. Costs are in the time that a CTA of the few-row kernel takes for a block of 16 positions (0.15 us with
+// head_dim 64, 0.18 us with 128, the SM's other CTAs beside it).
 struct Plan {
     bool tile = false;      // kv8_tile.cu's kernel
-    int warps = 4;          // of a CTA of the few-row kernel
-    int rows = 8;           // rows of a CTA: 8, each warp working on all of them, or 8 for each warp
+    int rows = kSmallRows;  // rows of a CTA
     int row_tiles = 1, chunks = 1, chunk_blocks = 1;
+    double cost = 0;
 };
-constexpr int kFewRows = 64;
-Plan plan_of(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int causal, int window) {
+Plan cut(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int causal, int window, bool tile) {
     Plan p;
+    p.tile = tile;
+    if (tile) p.rows = kTileRows;
     const int group = n_head / c.n_kv;
     const long long rows = (long long) b.max_new * group;
-    p.tile = rows > kFewRows;
-    if (p.tile) {
-        p.rows = kTileRows;
-    } else {
-        if (rows > 8) p.warps = (int) (rows + 7) / 8;
-        p.rows = rows > 8 ? 8 * p.warps : 8;
-    }
     const long long tiles = std::max<long long>(1, (rows + p.rows - 1) / p.rows);
     if (tiles > INT_MAX) fail("max_new x heads per kv head is too large");
     p.row_tiles = (int) tiles;
@@ -973,52 +969,47 @@ Plan plan_of(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int c
     if (causal && window > 0) keys = std::min<long long>(keys, (long long) window + (p.rows + group - 1) / group + 1 + 15);
     const int blocks = (int) std::max<long long>(1, (keys + 15) / 16 + (window > 0 ? 1 : 0));
     const long long units = std::max<long long>(1, (long long) b.n_seq * c.n_kv * p.row_tiles);
-    if (p.tile) {
-        // one CTA per SM, at least two tiles of 128 keys in each range
-        const long long want = std::max<long long>(1, 148 / units);
-        p.chunk_blocks = (int) std::max<long long>(16, (blocks + want - 1) / want);
-        p.chunk_blocks = (p.chunk_blocks + 7) / 8 * 8;
-    } else {
-        // ranges that fill whole waves of the CTAs an SM holds; a CTA's start and end cost about as much time as
-        // its share of 32 blocks, joining the ranges as much as 24 more (with rows of their own, warps take a
-        // quarter as many blocks in that time)
-        const int pair = 2 * c.head_dim / 16 * 512, merge = 32 * p.warps * (c.head_dim + 4);  // shared memory, as SmallTile has it
-        const int shared = std::max(p.rows > 8 ? 4 * pair : c.head_dim == 64 ? 8 * pair : 4 * pair, merge) + (10 << 10);
-        const long long slots = 148ll * std::min(small_ctas(c.head_dim, p.warps), (227 << 10) / shared);
-        const int start = p.rows > 8 ? 8 : 32, join = p.rows > 8 ? 6 : 24;
-        double best = 0;
-        for (int n = (blocks + kSmallBlocks - 1) / kSmallBlocks; n <= blocks; n++) {
-            const int size = (blocks + n - 1) / n;
-            const double cost = (double) ((units * n + slots - 1) / slots) * (size + start) + (n > 1 ? join : 0);
-            if (best == 0 || cost < best) best = cost, p.chunk_blocks = size;
-            if (units * n >= 6 * slots || size <= (p.rows > 8 ? 2 : 8)) break;
-        }
+    // What a CTA's start and end cost; the join's launch and each MB of its input, written and read back.
+    const double start = tile ? 43 : 32, launch = 24, mb = tile ? 3.4 : 0;
+    // (the many-row kernel's block: one tile of 128 rows, or two whose waits overlap)
+    const double block = !tile ? 1 : rows <= 128 ? 1.7 : 2.1;
+    const long long slots = tile ? 148 : 148ll * small_ctas(c.head_dim);
+    for (long long n = tile ? 1 : (blocks + kSmallBlocks - 1) / kSmallBlocks; n <= blocks; n++) {
+        int size = (int) ((blocks + n - 1) / n);
+        if (tile) size = (size + 7) / 8 * 8;  // whole stages
+        // whole waves of the CTAs that the SMs hold: the last range to end is what counts
+        const double waves = (double) ((units * n + slots - 1) / slots);
+        const double cost = waves * (block * size + start) + (n > 1 ? launch + mb * units * n * p.rows * (c.head_dim + 4) * 4e-6 : 0);
+        if (p.cost == 0 || cost < p.cost) p.cost = cost, p.chunk_blocks = size;
+        if (tile ? units * (n + 1) > slots || size <= 16 : units * n >= 6 * slots || size <= 8) break;
     }
     p.chunks = (blocks + p.chunk_blocks - 1) / p.chunk_blocks;
+    // without ranges the last wave's CTAs run faster by themselves: half of what it lacks is no loss
+    const double waves = (double) units / slots;
+    if (p.chunks == 1 && !tile && waves > 1) p.cost *= (waves + std::ceil(waves)) / 2 / std::ceil(waves);
     return p;
 }
+// The kernel by the lower cost. Measured with 4 rows a token and kv head, 8 kv heads of 64, few | many rows' kernel in us,
+// the choice starred: one sequence of 216 positions, 64 rows *5.6 | 10.9; 64 of 1012, 48 rows *58 | 80 and 96 rows
+// 109 | *80; 16 of 2008, 32 rows *27 | 34 and 64 rows 46 | *34; 30 prompts of 16, 64 rows *12.7 | 18.2, of
+// 64, 256 rows 47 | *21. Over 216 such calls the choice cost more than 10 % in five, 34 % at most. One row tile always
+// goes to the few rows' kernel. (BZB_KV8_ATTENTION=few or many takes one of them for every call.)
+Plan plan_of(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int causal, int window) {
+    const Plan few = cut(c, b, n_head, causal, window, false), many = cut(c, b, n_head, causal, window, true);
+    const char * e = std::getenv("BZB_KV8_ATTENTION");
+    if (e && !std::strcmp(e, "few")) return few;
+    if (e && !std::strcmp(e, "many")) return many;
+    return many.cost < few.cost ? many : few;
+}
 
-template <int HD, int WARPS, bool SHARED>
+template <int HD>
 void run_small(const AttnArgs & a, cudaStream_t s) {
     const long long grid = (long long) a.kv.n_seq * a.row_tiles * a.chunks * a.kv.n_kv;
     if (grid > INT_MAX) fail("the batch is too large for one call");
-    constexpr int bytes = SmallTile<HD, WARPS, SHARED>::BYTES;
+    constexpr int bytes = SmallTile<HD>::BYTES;
     static std::atomic<uint64_t> ready{ 0 };
-    allow_shared_memory(kv8_attn_small_kernel<HD, WARPS, SHARED>, bytes, ready);
-    launch_chained(kv8_attn_small_kernel<HD, WARPS, SHARED>, dim3((unsigned) grid), 32 * WARPS, bytes, s, a);
-}
-template <int HD>
-void run_small(const AttnArgs & a, const Plan & p, cudaStream_t s) {
-    if (p.rows == 8) return run_small<HD, 4, false>(a, s);
-    switch (p.warps) {
-        case 2: return run_small<HD, 2, true>(a, s);
-        case 3: return run_small<HD, 3, true>(a, s);
-        case 4: return run_small<HD, 4, true>(a, s);
-        case 5: return run_small<HD, 5, true>(a, s);
-        case 6: return run_small<HD, 6, true>(a, s);
-        case 7: return run_small<HD, 7, true>(a, s);
-        default: return run_small<HD, 8, true>(a, s);
-    }
+    allow_shared_memory(kv8_attn_small_kernel<HD>, bytes, ready);
+    launch_chained(kv8_attn_small_kernel<HD>, dim3((unsigned) grid), 32 * kSmallWarps, bytes, s, a);
 }
 
 void check_attention(const bzb_kv8_cache & c, int n_head, int causal, int window) {
@@ -1144,9 +1135,9 @@ void kv8_attention(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_k
     if (p.tile) {
         launch_attn_tile(a, c.head_dim, s);
     } else if (c.head_dim == 64) {
-        run_small<64>(a, p, s);
+        run_small<64>(a, s);
     } else {
-        run_small<128>(a, p, s);
+        run_small<128>(a, s);
     }
     if (p.chunks > 1) {
         const long long warps = (long long) b.n_seq * p.row_tiles * c.n_kv * p.rows;

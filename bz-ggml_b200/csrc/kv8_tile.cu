@@ -1,5 +1,5 @@
 // Attention of many rows over the 8-bit paged cache on the tensor cores (tcgen05): prompts, and whatever
-// else has more rows to a kv head than the few-row kernel of kv8.cu is made for.
+// else the few-row kernel of kv8.cu would need more time for (its formulas; the rule stands there).
 //
 // One CTA takes up to 256 rows of one kv head -- (token, head of the group) pairs, so the group shares
 // the cache's tiles -- as two M = 128 tiles, and walks its keys 128 at a time:

@@ -2,7 +2,7 @@
 
 Tolerances, from the arithmetic: a value is stored as the nearest e4m3 of its block's scale, so values
 (which are only scaled by a power of two) and rescaled older positions must match bit for bit, and keys
-(normed and rotated in f32 first) within half a spacing, 2^-4 relative or 2^-10 scales. Attention rounds
+(normed and rotated first) within half a spacing, 2^-4 relative or 2^-10 scales. Attention rounds
 its weights to f16 (2^-11 relative; below 2^-14 of the largest 2^-25 absolute) and its result to the
 output type, and its scores carry f32 rounding of the products' sum.
 """
