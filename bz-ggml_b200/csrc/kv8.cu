@@ -1002,6 +1002,11 @@ Plan plan_of(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int c
     return many.cost < few.cost ? many : few;
 }
 
+long long workspace_of(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const Plan & p) {
+    if (p.chunks == 1) return 0;
+    return (long long) b.n_seq * p.row_tiles * c.n_kv * p.chunks * p.rows * (c.head_dim + 4) * 4;
+}
+
 template <int HD>
 void run_small(const AttnArgs & a, cudaStream_t s) {
     const long long grid = (long long) a.kv.n_seq * a.row_tiles * a.chunks * a.kv.n_kv;
@@ -1094,10 +1099,7 @@ long long kv8_attention_workspace(const bzb_kv8_cache & c, const bzb_kv8_batch &
     view(c, b);
     check_attention(c, n_head, causal, window);
     if (b.n_seq == 0 || b.n_tok == 0 || b.max_new == 0) return 0;
-    const Plan p = plan_of(c, b, n_head, causal, window);
-    if (p.chunks == 1) return 0;
-    const long long units = (long long) b.n_seq * p.row_tiles * c.n_kv;
-    return units * p.chunks * p.rows * (c.head_dim + 4) * 4;
+    return workspace_of(c, b, plan_of(c, b, n_head, causal, window));
 }
 
 void kv8_attention(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_kv8_rows & q, const bzb_kv8_rows & out,
@@ -1113,12 +1115,13 @@ void kv8_attention(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_k
     a.out_vec = check_rows(out, "out", q.n_head, c.head_dim, false, 8, b.n_tok);
     check_distinct(out, "out", c.head_dim, b.n_tok);
     if ((uintptr_t) lse % 4) fail("lse is misaligned");
-    const long long need = kv8_attention_workspace(c, b, q.n_head, causal, window);
+    const bool empty = b.n_seq == 0 || b.n_tok == 0 || b.max_new == 0;
+    const Plan p = empty ? Plan() : plan_of(c, b, q.n_head, causal, window);
+    const long long need = workspace_of(c, b, p);
     if (need > 0 && (!workspace || workspace_bytes < need))
         fail("workspace of " + std::to_string(need) + " bytes needed, " + std::to_string(workspace ? workspace_bytes : 0) + " given");
     if (need > 0 && (uintptr_t) workspace % 16) fail("workspace must be 16-byte aligned");
-    if (b.n_seq == 0 || b.n_tok == 0 || b.max_new == 0) return;
-    const Plan p = plan_of(c, b, q.n_head, causal, window);
+    if (empty) return;
     a.q = Rows{ q.data, q.row_stride, q.head_stride };
     a.out = Rows{ out.data, out.row_stride, out.head_stride };
     a.lse = lse;
