@@ -67,7 +67,8 @@ struct Shared {
     uint32_t tmem;
     int err;
     int nan_v[4][kProducers];   // a producer warp found NaN values in this tile (only where it looked)
-    float4 scale[4];            // of a stage: the keys' scale, the values' exponent, 2^-it
+    float4 scale[4];            // of a stage: the keys' scale, the values' exponent, 2^-it; not 0: each block's in block[]
+    float4 block[4][8];         // of a stage whose blocks' scales lie far apart: the same three of each
     float unit[2][128];         // power of two taken out of each query row
 };
 
@@ -209,20 +210,24 @@ __device__ __forceinline__ int tile_page(const AttnArgs & a, const Work & w, int
     return j < w.n_tiles && blk < w.blk_hi ? max(page_of(a.kv, w.s.slot, blk), 0) : -1;
 }
 
-// The blocks' scales are brought to the largest of the stage, 2^E, by multiplying the f16 values with 2^(e - E):
-// exact, but for bits below 2^-24 of that scale. One factor then serves 128 keys in the softmax.
+// The blocks' scales are brought to that of the stage, 2^(E - kLift), E the largest exponent, by multiplying the f16
+// values with 2^(e - E + kLift). One factor then serves 128 keys in the softmax. Exact while the exponents lie within
+// kSpread of each other: 448 becomes 57344 at most, and the last bit of a subnormal byte, 2^-9, no less than f16's last,
+// 2^-24. Stages with a wider spread -- a loud block, which may be one that no row of the tile sees -- keep their values as
+// they are, and the softmax applies each block's scales for itself.
+constexpr int kLift = 7, kSpread = 22;
 struct StageScale {
-    int top;         // E
-    uint32_t mine;   // lane & 7's block: 2^(e - E) twice, as f16
+    int top;         // E - kLift
+    bool apart;      // a wider spread than kSpread
+    uint32_t mine;   // lane & 7's block: its factor twice, as f16 (one where they are apart)
 };
 __device__ __forceinline__ StageScale stage_scale(float scale, bool there) {
     const int e = there ? exponent_of(scale) : -1000;
-    int top = e;
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const int d = e - top;  // f16: 2^d has exponent field d + 15, or is subnormal from -15 to -24
-    const uint32_t h = d >= -14 ? (uint32_t) (d + 15) << 10 : d >= -24 ? 1u << (d + 24) : 0u;
-    return { top, h | h << 16 };
+    const int top = __reduce_max_sync(0xffffffffu, e), low = __reduce_min_sync(0xffffffffu, there ? e : 1000);
+    const int d = max(e - top, -kSpread) + kLift;  // f16: 2^d has exponent field d + 15; 2^-15 is subnormal
+    const uint32_t h = d >= -14 ? (uint32_t) (d + 15) << 10 : 1u << (d + 24);
+    const bool apart = top - low > kSpread;
+    return { top - kLift, apart, apart ? 0x3c003c00u : h | h << 16 };
 }
 __device__ __forceinline__ uint32_t scaled(uint16_t e4m3x2, uint32_t f) {
     const uint32_t h = e4m3x2_to_h2(e4m3x2);
@@ -393,12 +398,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
             const int pos = w.first + rr / a.group;
             const int hi = !real ? INT_MAX : a.causal ? pos + 1 : w.s.len, lo = real && a.window > 0 ? pos - a.window + 1 : INT_MIN;
             const int warp_hi = __reduce_min_sync(0xffffffffu, hi), warp_lo = __reduce_max_sync(0xffffffffu, lo);
-            // (a negative scale's sign is in the queries; never zero, which times -inf would be NaN)
-            const float row_coef = fmaxf(fabsf(a.scale2) * sh.unit[i][r], 1e-37f);
+            // (a negative scale's sign is in the queries; never zero, nor with a key scale of 2^-31, which times -inf
+            // would be NaN: 1e-30 moves scores by 1e-8 at most)
+            const float row_coef = fmaxf(fabsf(a.scale2) * sh.unit[i][r], 1e-30f);
             float m = -INFINITY, l = 0.0f;
             uint32_t nan_d[HD / 32] = {};
             bool ok = true;
-            float4 c = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // the stage's keys' scale times the row's factor, values' exponent, 2^-it
+            float4 c = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // the stage's scale[], the keys' times the row's factor
             for (int u = 0; u < steps; u++) {
                 const int j = u >> 1, key0 = (w.blk0 << 4) + kStep * u;
                 ok = warp_wait(&sh.s_full[i][u & 1], j & 1, err);
@@ -418,6 +424,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
 #pragma unroll
                 for (int t = 0; t < 32; t++) s[t] = pair(x[t / 16][2 * (t % 16)], x[t / 16][2 * (t % 16) + 1]);
                 if (!whole) mask(s, key0, lo, hi);
+                float z[4] = { c.z, c.z, c.z, c.z };  // 2^-exponent of the values of the step's blocks
+                if (__builtin_expect(c.w != 0.0f, 0)) {
+                    const float4 * block = &sh.block[j & 3][4 * (u & 1)];
+#pragma unroll
+                    for (int b = 0; b < 4; b++) {
+                        const float4 f = block[b];
+#pragma unroll
+                        for (int t = 0; t < 8; t++) s[8 * b + t] = fma2(s[8 * b + t], f.x * row_coef, f.y);
+                        z[b] = f.z;
+                    }
+                    c.x = 1.0f;
+                    c.y = 0.0f;
+                }
                 float tops[4] = { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
 #pragma unroll
                 for (int t = 0; t < 32; t++) tops[t & 3] = fmaxf(fmaxf(tops[t & 3], s[t].x), s[t].y);
@@ -446,21 +465,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
                     }
                 }
                 const float ref = c.y - (m == -INFINITY ? 0.0f : m);
-                float2 sum[2] = { { 0.0f, 0.0f }, { 0.0f, 0.0f } };
 #pragma unroll
                 for (int g = 0; g < 2; g++) {
+                    float2 sum[2] = { { 0.0f, 0.0f }, { 0.0f, 0.0f } };  // a block's
                     uint32_t p[16];
 #pragma unroll
                     for (int t = 0; t < 16; t++) {
                         const float2 v = fma2(s[16 * g + t], c.x, ref);
                         const float2 e = make_float2(exp2_approx(v.x), exp2_approx(v.y));
-                        sum[t & 1] = add2(sum[t & 1], e);
+                        sum[t >> 3] = add2(sum[t >> 3], e);
                         p[t] = pack_half(e.x, e.y);
                     }
                     st16(at + 16 * g, p);
+                    l = fmaf(sum[0].x + sum[0].y, z[2 * g], fmaf(sum[1].x + sum[1].y, z[2 * g + 1], l));
                 }
-                sum[0] = add2(sum[0], sum[1]);
-                l = fmaf(sum[0].x + sum[0].y, c.z, l);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -586,10 +604,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
             const StageScale sk = stage_scale(ks, pg >= 0), sv = stage_scale(vs, pg >= 0);
             if (!warp_wait(&sh.k_empty[st], ((j >> 1) & 1) ^ 1, err)) break;
             k.store(base + M::oK + st * M::kK, sk.mine);
-            if (pw == 0 && lane == 0) sh.scale[j & 3] = make_float4(pow2f(sk.top), (float) sv.top, pow2f(-sv.top), 0.0f);
+            const bool apart = sk.apart || sv.apart;
+            if (pw == 0 && lane == 0) sh.scale[j & 3] = make_float4(pow2f(sk.top), (float) sv.top, pow2f(-sv.top), apart ? 1.0f : 0.0f);
+            if (pw == 0 && lane < 8 && apart) {
+                // (blocks that are not there: any finite numbers, their keys are masked)
+                const int ev = !sv.apart ? sv.top : pg < 0 ? 0 : exponent_of(vs);
+                sh.block[j & 3][lane] = make_float4(!sk.apart ? pow2f(sk.top) : pg < 0 ? 1.0f : ks, (float) ev, pow2f(-ev), 0.0f);
+            }
             fence_proxy_async();
             __syncwarp();
-            // (scale[] and nan_v[] are rings of four: those of stage j + 4 are stored when the products of stage
+            // (scale[], block[] and nan_v[] are rings of four: those of stage j + 4 are stored when the products of stage
             // j + 2 have been issued, which every softmax warp's weights of stage j + 1 come before)
             if (lane == 0) mbar_arrive(&sh.k_full[st]);
             pg = next;
