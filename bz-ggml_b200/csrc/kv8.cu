@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(32 * kSmallWarps, small_ctas(HD)) kv8_attn_sma
     if (row0 >= rows || chunk >= my_chunks) return;
     // the keys that all rows see: [full_lo, full_hi)
     const int last_row = min(rows, row0 + kSmallRows) - 1;
-    const int full_hi = a.causal ? first + row0 / a.group + 1 : s.len;
+    const int full_hi = keys_end(a, s, first + row0 / a.group);
     const int full_lo = a.window > 0 ? max(0, first + last_row / a.group - a.window + 1) : 0;
     const int c_lo = span.blk_lo + chunk * a.chunk_blocks, c_hi = min(span.blk_hi, c_lo + a.chunk_blocks);
 
@@ -596,7 +596,7 @@ __global__ void __launch_bounds__(32 * kSmallWarps, small_ctas(HD)) kv8_attn_sma
     for (int i = 0; i < 2; i++) {
         const int rr = row0 + 2 * t + i, pos = first + rr / a.group;
         coef[i] = a.scale2 * __shfl_sync(0xffffffffu, row_unit, (2 * t + i) * 4);
-        lim_hi[i] = rr < rows ? (a.causal ? pos + 1 : s.len) : 0;
+        lim_hi[i] = rr < rows ? keys_end(a, s, pos) : 0;
         lim_lo[i] = a.window > 0 ? pos - a.window + 1 : 0;
     }
 

@@ -165,6 +165,11 @@ struct AttnArgs {
     float * part;  // ranges' results, when there are several: [unit][range][row][head_dim, maximum, sum, 0, 0]
 };
 
+// one past the last key of the row at position pos; none for a padding row (zero or less)
+__device__ __forceinline__ int keys_end(const AttnArgs & a, const Seq & s, int pos) {
+    return a.causal ? pos + 1 : pos < 0 ? 0 : s.len;
+}
+
 // The blocks of the cache that a tile's rows look at, and the ranges they are cut into.
 struct Span {
     int first, rows;             // position of the sequence's first row (negative: padding); its (token, head) rows

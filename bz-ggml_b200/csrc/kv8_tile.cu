@@ -138,7 +138,7 @@ __device__ __forceinline__ bool find_work(const AttnArgs & a, Work & w) {
     w.first = p.first;
     w.my_chunks = p.chunks;
     const int pos_lo = w.first + w.row0 / a.group, pos_hi = w.first + min(w.rows - 1, w.row0 + kTileRows - 1) / a.group;
-    w.full_hi = a.causal ? pos_lo + 1 : w.s.len;
+    w.full_hi = keys_end(a, w.s, pos_lo);
     w.full_lo = a.window > 0 ? max(0, pos_hi - a.window + 1) : 0;
     w.blk0 = p.blk_lo + w.chunk * a.chunk_blocks;
     w.blk_hi = min(p.blk_hi, w.blk0 + a.chunk_blocks);
@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
             const uint32_t ts = tmem + lanes + i * 2 * kStep, to = tmem + lanes + M::cO + i * HD;
             const bool real = rr < w.rows;
             const int pos = w.first + rr / a.group;
-            const int hi = !real ? INT_MAX : a.causal ? pos + 1 : w.s.len, lo = real && a.window > 0 ? pos - a.window + 1 : INT_MIN;
+            const int hi = real ? keys_end(a, w.s, pos) : INT_MAX, lo = real && a.window > 0 ? pos - a.window + 1 : INT_MIN;
             const int warp_hi = __reduce_min_sync(0xffffffffu, hi), warp_lo = __reduce_max_sync(0xffffffffu, lo);
             // (a negative scale's sign is in the queries; never zero, nor with a key scale of 2^-31, which times -inf
             // would be NaN: 1e-30 moves scores by 1e-8 at most)
