@@ -1017,11 +1017,14 @@ void run_small(const AttnArgs & a, cudaStream_t s) {
     launch_chained(kv8_attn_small_kernel<HD>, dim3((unsigned) grid), 32 * kSmallWarps, bytes, s, a);
 }
 
-void check_attention(const bzb_kv8_cache & c, int n_head, int causal, int window) {
+// Checks them and gives the window that counts: none where no context fills it, so that positions less a window stay
+// far inside an int.
+int check_attention(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int causal, int window) {
     if (n_head < 1 || n_head % c.n_kv) fail("the query heads must be a multiple of n_kv");
     if (n_head > (1 << 16)) fail("too many query heads");
     if (window < 0) fail("window must not be negative");
     if (window > 0 && !causal) fail("a window needs causal attention");
+    return window < b.max_len ? window : 0;
 }
 
 }  // namespace
@@ -1097,7 +1100,7 @@ void kv8_read(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_kv8_ro
 
 long long kv8_attention_workspace(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int causal, int window) {
     view(c, b);
-    check_attention(c, n_head, causal, window);
+    window = check_attention(c, b, n_head, causal, window);
     if (b.n_seq == 0 || b.n_tok == 0 || b.max_new == 0) return 0;
     return workspace_of(c, b, plan_of(c, b, n_head, causal, window));
 }
@@ -1108,7 +1111,7 @@ void kv8_attention(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_k
     AttnArgs a;
     a.kv = view(c, b);
     if (q.n_head != out.n_head) fail("q and out must have the same heads");
-    check_attention(c, q.n_head, causal, window);
+    window = check_attention(c, b, q.n_head, causal, window);
     if (!std::isfinite(scale * kLog2e)) fail("scale must be finite");
     if (q.type != out.type) fail("q and out must be of one type");
     a.q_vec = check_rows(q, "q", q.n_head, c.head_dim, false, 8, b.n_tok);
