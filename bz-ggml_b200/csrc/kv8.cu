@@ -961,13 +961,17 @@ Plan cut(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int causa
     if (tile) p.rows = kTileRows;
     const int group = n_head / c.n_kv;
     const long long rows = (long long) b.max_new * group;
-    const long long tiles = std::max<long long>(1, (rows + p.rows - 1) / p.rows);
-    if (tiles > INT_MAX) fail("max_new x heads per kv head is too large");
-    p.row_tiles = (int) tiles;
+    // (the kernels number them in an int, up to a tile past the last)
+    if (rows > 1 << 30) fail("max_new x heads per kv head is too large (2^30 at most)");
+    p.row_tiles = (int) std::max<long long>(1, (rows + p.rows - 1) / p.rows);
     // blocks that one CTA's rows look at: its tokens' windows, at any offset within a block
     long long keys = b.max_len;
     if (causal && window > 0) keys = std::min<long long>(keys, (long long) window + (p.rows + group - 1) / group + 1 + 15);
     const int blocks = (int) std::max<long long>(1, (keys + 15) / 16 + (window > 0 ? 1 : 0));
+    if ((double) b.n_seq * c.n_kv * p.row_tiles > INT_MAX) {  // (more CTAs than a launch takes)
+        p.cost = HUGE_VAL;
+        return p;
+    }
     const long long units = std::max<long long>(1, (long long) b.n_seq * c.n_kv * p.row_tiles);
     // What a CTA's start and end cost; the join's launch and each MB of its input, written and read back.
     const double start = tile ? 43 : 32, launch = 24, mb = tile ? 3.4 : 0;
@@ -997,9 +1001,10 @@ Plan cut(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int causa
 Plan plan_of(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int causal, int window) {
     const Plan few = cut(c, b, n_head, causal, window, false), many = cut(c, b, n_head, causal, window, true);
     const char * e = std::getenv("BZB_KV8_ATTENTION");
-    if (e && !std::strcmp(e, "few")) return few;
-    if (e && !std::strcmp(e, "many")) return many;
-    return many.cost < few.cost ? many : few;
+    const bool tile = e && !std::strcmp(e, "few") ? false : e && !std::strcmp(e, "many") ? true : many.cost < few.cost;
+    const Plan & p = tile ? many : few;
+    if ((double) b.n_seq * c.n_kv * p.row_tiles * p.chunks > INT_MAX) fail("the batch is too large for one call");
+    return p;
 }
 
 long long workspace_of(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const Plan & p) {
@@ -1010,7 +1015,6 @@ long long workspace_of(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const P
 template <int HD>
 void run_small(const AttnArgs & a, cudaStream_t s) {
     const long long grid = (long long) a.kv.n_seq * a.row_tiles * a.chunks * a.kv.n_kv;
-    if (grid > INT_MAX) fail("the batch is too large for one call");
     constexpr int bytes = SmallTile<HD>::BYTES;
     static std::atomic<uint64_t> ready{ 0 };
     allow_shared_memory(kv8_attn_small_kernel<HD>, bytes, ready);

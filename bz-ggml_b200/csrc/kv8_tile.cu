@@ -708,7 +708,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
 template <int HD>
 void launch(const AttnArgs & a, cudaStream_t s) {
     const long long grid = (long long) a.kv.n_seq * a.row_tiles * a.chunks * a.kv.n_kv;
-    if (grid > INT_MAX) throw std::runtime_error("the batch is too large for one call");
     static std::atomic<uint64_t> ready{ 0 };
     if (!ready.load(std::memory_order_acquire)) {
         // the register split adds up only for the launch it was made for: a build that gives the kernel
