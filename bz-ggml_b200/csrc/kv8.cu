@@ -91,9 +91,10 @@ __device__ __forceinline__ float to_odd(double x) {
     const float f = __double2float_rz(x);
     return (double) f == x ? f : __int_as_float(__float_as_int(f) | 1);
 }
-// a row's norm and rotation in 64 bits, for the lanes of RowMap (without a rotation: cos 1, sin 0)
+// a row's norm and rotation in 64 bits, for the lanes of RowMap
 template <int HD>
-__device__ __forceinline__ void turn_exactly(float4 & lo, float4 & hi, bool norm, float4 wl, float4 wh, float eps, float4 t0, float4 t1) {
+__device__ __forceinline__ void turn_exactly(float4 & lo, float4 & hi, bool norm, float4 wl, float4 wh, float eps, bool turn, float4 t0,
+                                             float4 t1) {
     double x[4] = { lo.x, lo.y, lo.z, lo.w }, y[4] = { hi.x, hi.y, hi.z, hi.w };
     if (norm) {
         const float u[4] = { wl.x, wl.y, wl.z, wl.w }, v[4] = { wh.x, wh.y, wh.z, wh.w };
@@ -110,8 +111,9 @@ __device__ __forceinline__ void turn_exactly(float4 & lo, float4 & hi, bool norm
     float p[4], q[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        p[j] = to_odd(fma(x[j], (double) c[j], -(y[j] * s[j])));
-        q[j] = to_odd(fma(x[j], (double) s[j], y[j] * c[j]));
+        // (not a turn by nothing: 0 times an infinite partner is NaN)
+        p[j] = to_odd(turn ? fma(x[j], (double) c[j], -(y[j] * s[j])) : x[j]);
+        q[j] = to_odd(turn ? fma(x[j], (double) s[j], y[j] * c[j]) : y[j]);
     }
     lo = make_float4(p[0], p[1], p[2], p[3]);
     hi = make_float4(q[0], q[1], q[2], q[3]);
@@ -212,10 +214,13 @@ __device__ __forceinline__ void append_block(const AppendArgs & a, const Seq & s
             }
             const float4 t0 = turn[i][0], t1 = turn[i][1];
             if (!live[i]) continue;
-            store4(a.q_out_type, a.q_out_vec, a.q_out.p, to,
-                   make_float4(x.x * t0.x - y.x * t0.y, x.y * t0.z - y.y * t0.w, x.z * t1.x - y.z * t1.y, x.w * t1.z - y.w * t1.w));
-            store4(a.q_out_type, a.q_out_vec, a.q_out.p, to + HD / 2,
-                   make_float4(x.x * t0.y + y.x * t0.x, x.y * t0.w + y.y * t0.z, x.z * t1.y + y.z * t1.x, x.w * t1.w + y.w * t1.z));
+            float4 u = x, v = y;
+            if (a.rope) {
+                u = make_float4(x.x * t0.x - y.x * t0.y, x.y * t0.z - y.y * t0.w, x.z * t1.x - y.z * t1.y, x.w * t1.z - y.w * t1.w);
+                v = make_float4(x.x * t0.y + y.x * t0.x, x.y * t0.w + y.y * t0.z, x.z * t1.y + y.z * t1.x, x.w * t1.w + y.w * t1.z);
+            }
+            store4(a.q_out_type, a.q_out_vec, a.q_out.p, to, u);
+            store4(a.q_out_type, a.q_out_vec, a.q_out.p, to + HD / 2, v);
         }
     } else {
         const bool exact = kind == 1 && (w || a.rope);
@@ -228,7 +233,7 @@ __device__ __forceinline__ void append_block(const AppendArgs & a, const Seq & s
             if (exact && (FULL || __any_sync(0xffffffffu, live[i]))) {
                 float4 t0, t1;
                 turn_of(i, t0, t1);
-                turn_exactly<HD>(lo[i], hi[i], w != nullptr, wl, wh, a.eps, t0, t1);
+                turn_exactly<HD>(lo[i], hi[i], w != nullptr, wl, wh, a.eps, a.rope != nullptr, t0, t1);
             }
             // (a row that is not there has norm zero, which without eps is no number)
             if (!live[i]) lo[i] = hi[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
