@@ -85,6 +85,10 @@ struct AppendArgs {
     bool q_out_vec, norm_vec;
 };
 
+// Mean squares between these need no second look: the products of elements that matter are normal numbers. Below, every
+// element is less than 2^-36 and grows to 2^60 at most (2^-149 to 2^-53); above, none exceeds 2^128, which becomes 2^58.
+constexpr float kTinySquares = 0x1p-80f, kHugeSquares = 0x1p120f, kSmallLift = 0x1p96f, kLargeDrop = 0x1p-70f;
+
 // the f32 next to x towards zero, its last bit set where it is not x: rounded once more to fewer bits, it goes
 // the way x would
 __device__ __forceinline__ float to_odd(double x) {
@@ -196,14 +200,29 @@ __device__ __forceinline__ void append_block(const AppendArgs & a, const Seq & s
             if (!FULL && !__any_sync(0xffffffffu, live[i])) continue;
             float4 x = lo_raw[i].value(), y = hi_raw[i].value();
             if (w) {
-                float2 sq = __fmul2_rn(make_float2(x.x, x.y), make_float2(x.x, x.y));
-                sq = __ffma2_rn(make_float2(x.z, x.w), make_float2(x.z, x.w), sq);
-                sq = __ffma2_rn(make_float2(y.x, y.y), make_float2(y.x, y.y), sq);
-                sq = __ffma2_rn(make_float2(y.z, y.w), make_float2(y.z, y.w), sq);
-                float ss = sq.x + sq.y;
+                auto mean_sq = [&] {
+                    float2 sq = __fmul2_rn(make_float2(x.x, x.y), make_float2(x.x, x.y));
+                    sq = __ffma2_rn(make_float2(x.z, x.w), make_float2(x.z, x.w), sq);
+                    sq = __ffma2_rn(make_float2(y.x, y.y), make_float2(y.x, y.y), sq);
+                    sq = __ffma2_rn(make_float2(y.z, y.w), make_float2(y.z, y.w), sq);
+                    float ss = sq.x + sq.y;
 #pragma unroll
-                for (int o = R::LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                const float r = rsqrtf(ss * (1.0f / HD) + a.eps);
+                    for (int o = R::LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                    return ss * (1.0f / HD);
+                };
+                float eps = a.eps, ms = mean_sq();
+                // Squares outside f32's range, above or (where eps does not outweigh them) below: once more with the row
+                // times a power of two, which the norm takes out again. (f16's squares stay inside: 2^-48 to 2^32.)
+                const bool out = TYPE != BZB_F16 && !(ms + eps > kTinySquares && ms < kHugeSquares);
+                if (TYPE != BZB_F16 && __builtin_expect(__any_sync(0xffffffffu, out), 0)) {
+                    if (out) {
+                        const float f = ms < 1.0f ? kSmallLift : kLargeDrop;
+                        x.x *= f, x.y *= f, x.z *= f, x.w *= f, y.x *= f, y.y *= f, y.z *= f, y.w *= f;
+                        eps = eps * f * f;
+                    }
+                    ms = mean_sq();
+                }
+                const float r = rsqrtf(ms + eps);
                 auto scale = [&](float4 & v, const float4 & w) {
                     const float2 p = __fmul2_rn(__fmul2_rn(make_float2(v.x, v.y), make_float2(r, r)), make_float2(w.x, w.y));
                     const float2 q = __fmul2_rn(__fmul2_rn(make_float2(v.z, v.w), make_float2(r, r)), make_float2(w.z, w.w));
