@@ -599,13 +599,13 @@ __global__ void __launch_bounds__(32 * kSmallWarps, small_ctas(HD)) kv8_attn_sma
         float amax = 0.0f;
 #pragma unroll
         for (int k = 0; k < T::KS; k++) load_q16(a, at + 64 * k, 1.0f, qf[k], &amax);
-        // bf16 may lie outside f16: the row is brought to about [1, 2) by a power of two (which the
-        // scores' factor takes back), so at most its elements below 2^-25 of the largest are lost
+        // bf16 may lie outside f16: the row is brought up to [2^14, 2^15) by a power of two (which the scores'
+        // factor takes back); elements keep all their bits down to 2^-31 of the largest, and some down to 2^-38
         if (a.type == BZB_BF16) {
             const unsigned quad = 0xfu << (lane & 28);
             amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(quad, amax, 2));
-            const int e = amax < INFINITY && amax > 0.0f ? min(126, max(-125, (__float_as_int(amax) >> 23) - 127)) : 0;
+            const int e = row_exponent(amax);
             row_unit = pow2f(e);
 #pragma unroll
             for (int k = 0; k < T::KS; k++) load_q16(a, at + 64 * k, pow2f(-e), qf[k], nullptr);

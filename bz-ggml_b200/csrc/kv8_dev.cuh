@@ -87,6 +87,10 @@ __device__ __forceinline__ float * scale_ptr(const Kv & kv, int pg, int blk, int
 
 __device__ __forceinline__ float pow2f(int e) { return __int_as_float((e + 127) << 23); }
 __device__ __forceinline__ int exponent_of(float pow2) { return (__float_as_int(pow2) >> 23) - 127; }
+// e such that a bf16 row of largest magnitude x, times 2^-e, fills f16 from the top: [2^14, 2^15)
+__device__ __forceinline__ int row_exponent(float x) {
+    return x < INFINITY && x > 0.0f ? max(-125, (__float_as_int(x) >> 23) - 127 - 14) : 0;
+}
 // smallest e with 448 2^e >= x (448 = 1.75 2^8), clamped; x >= 0 and finite
 __device__ __forceinline__ int block_exponent(float x) {
     const int bits = __float_as_int(x);

@@ -176,7 +176,7 @@ __device__ __forceinline__ void load_queries(const AttnArgs & a, const Work & w,
         float unit = 1.0f;
         if (a.scale2 < 0.0f) u[p] = make_uint4(u[p].x ^ 0x80008000u, u[p].y ^ 0x80008000u, u[p].z ^ 0x80008000u, u[p].w ^ 0x80008000u);
         if (a.type == BZB_BF16) {
-            // bf16 may lie outside f16: the row is brought to about [1, 2) by a power of two
+            // bf16 may lie outside f16: the row is brought up to [2^14, 2^15) by a power of two
             const uint32_t v[4] = { u[p].x, u[p].y, u[p].z, u[p].w };
             float x[8], amax = 0.0f;
 #pragma unroll
@@ -185,7 +185,7 @@ __device__ __forceinline__ void load_queries(const AttnArgs & a, const Work & w,
             for (int j = 0; j < 8; j += 2) amax = fmaxf(fmaxf(amax, fabsf(x[j])), fabsf(x[j + 1]));
 #pragma unroll
             for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-            const int e = amax < INFINITY && amax > 0.0f ? min(126, max(-125, (__float_as_int(amax) >> 23) - 127)) : 0;
+            const int e = row_exponent(amax);
             unit = pow2f(e);
             const float f = pow2f(-e);
             u[p] = make_uint4(pack_half(x[0] * f, x[1] * f), pack_half(x[2] * f, x[3] * f), pack_half(x[4] * f, x[5] * f),
