@@ -124,6 +124,7 @@ SIGNATURES = {
     "bzb_generator_bench_gemv": (ctypes.c_double, [ctypes.c_void_p, ctypes.c_char_p, ctypes.c_int, ctypes.c_int,
                                                     ctypes.c_int, ctypes.c_int]),
     "bzb_generator_depth_trace": (ctypes.c_int, [ctypes.c_void_p, _c_double_p, ctypes.c_int]),
+    "bzb_debug_kv8_polls": (None, [ctypes.c_longlong]),
     "bzb_kv8_append": (ctypes.c_int, [ctypes.c_void_p] * 8 + [ctypes.c_float, ctypes.c_void_p, ctypes.c_int,
                                                                ctypes.c_void_p]),
     "bzb_kv8_read": (ctypes.c_int, [ctypes.c_void_p] * 5),
@@ -700,6 +701,11 @@ def mbar_timeout_probe(polls: int, device: int = 0) -> int:
     if code < 0:
         raise RuntimeError(lib().last_error())
     return code
+
+
+def set_debug_kv8_polls(polls: int) -> None:
+    """Poll limit of the waits in the 8-bit cache's many-row attention (0: none, negative: the default)."""
+    lib().lib.bzb_debug_kv8_polls(int(polls))
 
 
 def split_text(text: str, budget: int, first_budget: int = 0) -> List[str]:

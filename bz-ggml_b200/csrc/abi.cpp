@@ -1031,6 +1031,8 @@ int bzb_kv8_attention(const bzb_kv8_cache * cache, const bzb_kv8_batch * batch, 
     });
 }
 
+void bzb_debug_kv8_polls(long long polls) { bzb::kv8_debug_polls(polls); }
+
 int bzb_generator_depth_trace(breeze_generator * gen, double * out, int capacity) {
     if (!gen) return -1;
     try {

@@ -1057,6 +1057,11 @@ int check_attention(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head
 
 }  // namespace
 
+namespace {
+std::atomic<long long> debug_polls{ -1 };
+}
+void kv8_debug_polls(long long polls) { debug_polls.store(polls, std::memory_order_relaxed); }
+
 void kv8_append(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_kv8_rows * q, const bzb_kv8_rows & k,
                 const bzb_kv8_rows & v, const bzb_kv8_rows * q_out, const float * q_norm, const float * k_norm, float eps,
                 const float * rope, int rope_len, cudaStream_t s) {
@@ -1166,6 +1171,7 @@ void kv8_attention(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_k
     a.chunks = p.chunks;
     a.chunk_blocks = p.chunk_blocks;
     a.part = static_cast<float *>(workspace);
+    a.polls = debug_polls.load(std::memory_order_relaxed);
     if (p.tile) {
         launch_attn_tile(a, c.head_dim, s);
     } else if (c.head_dim == 64) {

@@ -19,4 +19,7 @@ void kv8_attention(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_k
                    float * lse, float scale, int causal, int window, void * workspace, long long workspace_bytes,
                    cudaStream_t s);
 
+// the many-row kernel's poll limit in the calls that follow (tests; negative: the default)
+void kv8_debug_polls(long long polls);
+
 }  // namespace bzb

@@ -47,8 +47,8 @@ struct Seq {
     int row0, n, len, slot;  // first packed row, rows, cached positions, page table row (-1: skip the sequence)
 };
 
-__device__ __forceinline__ void complain(const Kv & kv) {
-    if (kv.status) atomicExch(kv.status, 1);
+__device__ __forceinline__ void complain(const Kv & kv, int what) {
+    if (kv.status) atomicOr(kv.status, what);
 }
 
 __device__ __forceinline__ Seq load_seq(const Kv & kv, int b) {
@@ -61,7 +61,7 @@ __device__ __forceinline__ Seq load_seq(const Kv & kv, int b) {
     // (end and row0 are compared before their difference is used: it may overflow)
     if (s.row0 < 0 || end < s.row0 || end > kv.n_tok || s.n > kv.max_new || s.len < 0 || s.len > kv.max_len || s.slot < 0 ||
         s.slot >= kv.n_slots) {
-        complain(kv);
+        complain(kv, BZB_KV8_OUT_OF_RANGE);
         s.slot = -1;
     }
     return s;
@@ -71,7 +71,7 @@ __device__ __forceinline__ Seq load_seq(const Kv & kv, int b) {
 __device__ __forceinline__ int page_of(const Kv & kv, int slot, int blk) {
     const int pg = kv.table[(size_t) slot * kv.max_pages + (blk >> (kv.page_shift - 4))];
     if ((unsigned) pg >= (unsigned) kv.n_pages) {
-        complain(kv);
+        complain(kv, BZB_KV8_OUT_OF_RANGE);
         return -1;
     }
     return pg;
@@ -166,6 +166,7 @@ struct AttnArgs {
     int type;      // of q and out
     bool q_vec, out_vec;
     int row_tiles, chunks, chunk_blocks;  // chunk_blocks: blocks of 16 positions in a range
+    long long polls;  // of a wait in the many rows' kernel before it gives up (negative: the default)
     float * part;  // ranges' results, when there are several: [unit][range][row][head_dim, maximum, sum, 0, 0]
 };
 
@@ -240,7 +241,7 @@ __device__ __forceinline__ void start_after_previous() {
 
 // the attention of many rows (kv8_tile.cu): rows of a kv head in tiles of kTileRows
 constexpr int kTileRows = 256;
-void launch_attn_tile(const AttnArgs & a, int head_dim, cudaStream_t s);
+void launch_attn_tile(AttnArgs a, int head_dim, cudaStream_t s);
 
 }  // namespace kv8
 }  // namespace bzb

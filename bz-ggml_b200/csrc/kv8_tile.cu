@@ -106,8 +106,8 @@ __device__ __forceinline__ bool elect_one() {
 }
 
 // a whole warp's bounded wait: all lanes succeed, or all take it as failed
-__device__ __forceinline__ bool warp_wait(uint64_t * bar, uint32_t parity, int * err) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, err));
+__device__ __forceinline__ bool warp_wait(uint64_t * bar, uint32_t parity, int * err, long long polls) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, polls));
 }
 
 // The part of the cache and the rows that a CTA works on.
@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
             float4 c = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // the stage's scale[], the keys' times the row's factor
             for (int u = 0; u < steps; u++) {
                 const int j = u >> 1, key0 = (w.blk0 << 4) + kStep * u;
-                ok = warp_wait(&sh.s_full[i][u & 1], j & 1, err);
+                ok = warp_wait(&sh.s_full[i][u & 1], j & 1, err, a.polls);
                 if (!ok) break;
                 if (!(u & 1)) {
                     c = sh.scale[j & 3];
@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
                     l *= f;
                     if (u > 0) {
                         // the last product into these outputs must be in before they are scaled
-                        ok = warp_wait(&sh.pv_done[i][(u - 1) & 1], ((u - 1) >> 1) & 1, err);
+                        ok = warp_wait(&sh.pv_done[i][(u - 1) & 1], ((u - 1) >> 1) & 1, err, a.polls);
                         if (!ok) break;
                         tc_fence_after();
 #pragma unroll 1
@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
                 // out; the rows that see one get it at the end
                 const int stage0 = (w.blk0 + 8 * j) << 4;
                 if (stage0 < w.full_lo || stage0 + kKeys > w.full_hi) {
-                    ok = warp_wait(&sh.n_full[j & 3], (j >> 2) & 1, err);
+                    ok = warp_wait(&sh.n_full[j & 3], (j >> 2) & 1, err, a.polls);
                     if (!ok) break;
                     bool any = false;
                     for (int q = 0; q < kProducers; q++) any |= sh.nan_v[j & 3][q] != 0;
@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
                     __syncwarp();
                 }
             }
-            if (ok && n > 0) ok = warp_wait(&sh.o_full[i], 0, err);
+            if (ok && n > 0) ok = warp_wait(&sh.o_full[i], 0, err, a.polls);
             if (ok) {
                 tc_fence_after();
                 // rows go out through this tile's query buffer, whose products are done, so that a warp writes whole
@@ -602,7 +602,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
         for (int j = 0; j < n; j++) {
             const int st = j & 1, key0 = (w.blk0 + 8 * j) << 4;
             const StageScale sk = stage_scale(ks, pg >= 0), sv = stage_scale(vs, pg >= 0);
-            if (!warp_wait(&sh.k_empty[st], ((j >> 1) & 1) ^ 1, err)) break;
+            if (!warp_wait(&sh.k_empty[st], ((j >> 1) & 1) ^ 1, err, a.polls)) break;
             k.store(base + M::oK + st * M::kK, sk.mine);
             const bool apart = sk.apart || sv.apart;
             if (pw == 0 && lane == 0) sh.scale[j & 3] = make_float4(pow2f(sk.top), (float) sv.top, pow2f(-sv.top), apart ? 1.0f : 0.0f);
@@ -623,7 +623,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
             bool bad = false;
             if (key0 < w.full_lo || key0 + kKeys > w.full_hi) bad = v.clear_nan();
             bad = __any_sync(0xffffffffu, bad);
-            if (!warp_wait(&sh.v_empty[st], ((j >> 1) & 1) ^ 1, err)) break;
+            if (!warp_wait(&sh.v_empty[st], ((j >> 1) & 1) ^ 1, err, a.polls)) break;
             v.store(base + M::oV + st * M::kV, sv.mine);
             if (lane == 0) sh.nan_v[j & 3][pw] = bad;
             fence_proxy_async();
@@ -646,13 +646,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
                 const int st = (u >> 1) & 1;
                 // the buffer's last weights have been read (MMAs of different accumulators have no guaranteed
                 // order, so that product is waited for; the other buffer's scores keep the softmax busy)
-                if (u >= 2) ok = warp_wait(&sh.pv_done[mt][u & 1], ((u - 2) >> 1) & 1, err);
-                else if (u == 0 && mt == 0) ok = warp_wait(&sh.q_full[0], 0, err);
+                if (u >= 2) ok = warp_wait(&sh.pv_done[mt][u & 1], ((u - 2) >> 1) & 1, err, a.polls);
+                else if (u == 0 && mt == 0) ok = warp_wait(&sh.q_full[0], 0, err, a.polls);
                 // the second tile starts when the first has done its first step: the two softmaxes then take the
                 // exponential units in turn instead of both at once and both not at all. (A barrier that completes
                 // once: this wait may come any time after)
-                else if (u == 0) ok = warp_wait(&sh.q_full[1], 0, err) && warp_wait(&sh.lead, 0, err);
-                if (ok && !(u & 1)) ok = warp_wait(&sh.k_full[st], (u >> 2) & 1, err);
+                else if (u == 0) ok = warp_wait(&sh.q_full[1], 0, err, a.polls) && warp_wait(&sh.lead, 0, err, a.polls);
+                if (ok && !(u & 1)) ok = warp_wait(&sh.k_full[st], (u >> 2) & 1, err, a.polls);
                 if (!ok) break;
                 tc_fence_after();
                 if (elect_one()) {
@@ -675,8 +675,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
             const uint64_t v0 = sw128_desc(smem_u32(base + M::oV));
             for (int u = 0; u < steps; u++) {
                 const int st = (u >> 1) & 1;
-                if (!(u & 1)) ok = warp_wait(&sh.v_full[st], (u >> 2) & 1, err);
-                if (ok) ok = warp_wait(&sh.w_full[mt][u & 1], (u >> 1) & 1, err);
+                if (!(u & 1)) ok = warp_wait(&sh.v_full[st], (u >> 2) & 1, err, a.polls);
+                if (ok) ok = warp_wait(&sh.w_full[mt][u & 1], (u >> 1) & 1, err, a.polls);
                 if (!ok) break;
                 tc_fence_after();
                 if (elect_one()) {
@@ -702,7 +702,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
     __syncthreads();
     tc_fence_after();
     if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
-    if (threadIdx.x == 0 && sh.err && a.kv.status) atomicExch(a.kv.status, 2);
+    if (threadIdx.x == 0 && sh.err) complain(a.kv, BZB_KV8_TIMED_OUT);
 }
 
 template <int HD>
@@ -722,7 +722,8 @@ void launch(const AttnArgs & a, cudaStream_t s) {
 
 }  // namespace
 
-void launch_attn_tile(const AttnArgs & a, int head_dim, cudaStream_t s) {
+void launch_attn_tile(AttnArgs a, int head_dim, cudaStream_t s) {
+    if (a.polls < 0) a.polls = kSpinLimit;
     if (head_dim == 64) launch<64>(a, s);
     else launch<128>(a, s);
 }

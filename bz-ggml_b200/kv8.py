@@ -127,7 +127,11 @@ class KV8Cache:
         self._attention(self._at, batch._at, batch._workspaces, q, out, scale, causal, window, lse)
 
     def check(self) -> None:
-        """Waits for the device and raises if a call met a page, slot or length out of range since the last check."""
-        if int(self.status.item()):
+        """Waits for the device and raises if a call met a page, slot or length out of range, or a wait inside the
+        attention ran out, since the last check."""
+        status = int(self.status.item())
+        if status:
             self.status.zero_()
-            raise RuntimeError("kv8: a page, slot or length was out of range; that sequence was skipped")
+            what = {1: "a page, slot or length was out of range; that sequence was skipped",
+                    2: "a bounded wait inside the attention ran out; its rows are missing or wrong"}
+            raise RuntimeError("kv8: " + "; ".join(text for bit, text in what.items() if status & bit))

@@ -125,6 +125,9 @@ BREEZE_API int bzb_generator_debug_sample(breeze_generator * gen, const float * 
                                           float temp, float top_p, unsigned int seed, int draws, int force_sort,
                                           int * out_picks);
 BREEZE_API int bzb_debug_mbar_timeout(int device, long long polls);
+/* polls of every wait in the 8-bit cache's many-row attention, in the calls of this process that follow (0: each
+   wait gives up at once; negative: the default). A captured call keeps the limit it was captured with. */
+BREEZE_API void bzb_debug_kv8_polls(long long polls);
 
 /* ---- 8-bit paged key/value cache (no counterpart in the reference, whose cache is f32) ----
  * Keys and values in 8 bits (e4m3) with one scale for each block of 16 positions and head: half the
@@ -150,9 +153,11 @@ BREEZE_API int bzb_debug_mbar_timeout(int device, long long polls);
  * runs; max_new >= every n_b and max_len >= every kv_len[b] are bounds that the host knows.
  *
  * What only the device can see -- a page or slot out of range, a sequence that breaks its bounds -- is
- * not followed: `status` (one int on the device, may be NULL) is set to 1 and the sequence is skipped
- * (its outputs are not written) or the page read as page 0, never written. The caller clears it. */
+ * not followed: BZB_KV8_OUT_OF_RANGE is set in `status` (one int on the device, may be NULL) and the sequence is
+ * skipped (its outputs are not written) or the page read as page 0, never written. BZB_KV8_TIMED_OUT is set
+ * when a bounded wait inside the attention ran out: rows of that call are missing or wrong. The caller clears `status`. */
 enum { BZB_F32 = 0, BZB_F16 = 1, BZB_BF16 = 2 };
+enum { BZB_KV8_OUT_OF_RANGE = 1, BZB_KV8_TIMED_OUT = 2 };
 typedef struct bzb_kv8_cache {
     void * pages;
     float * scales;
