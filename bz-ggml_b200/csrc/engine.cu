@@ -402,6 +402,8 @@ void Engine::alloc_buffers() {
     const DdConfig & dd = cfg.dd;
     const int H = cfg.hidden, nc = cfg.nc;
     const size_t page_elems = (size_t) bb.n_layer * 2 * bb.n_kv * 16 * bb.hd;
+    err_ = dalloc<int>(2);
+    CK(cudaMemsetAsync(err_, 0, 2 * sizeof(int), stream_));
     size_t free_b = 0, total_b = 0;
     CK(cudaMemGetInfo(&free_b, &total_b));
     size_t pool_bytes = (size_t) 8 << 30;
@@ -470,8 +472,6 @@ void Engine::alloc_buffers() {
     step_ctr_ = dalloc<int>(1);
     any_active_ = dalloc<int>(kmax_);
     slot_scalar_ = dalloc<int>(1);
-    err_ = dalloc<int>(1);
-    CK(cudaMemsetAsync(err_, 0, sizeof(int), stream_));
     din16_ = dalloc<half>((size_t) R2 * H);
     dx_ = dalloc<float>((size_t) R2 * dd.hidden);
     dh16_ = dalloc<half>((size_t) R2 * dd.hidden);
@@ -597,6 +597,7 @@ bzb_kv8_cache Engine::kv8_cache(int layer) const {
     c.pages = kv8_pages_ + layer * bytes;
     c.scales = kv8_scales_ + layer * scales;
     c.page_table = page_table_;
+    c.status = err_ + 1;
     c.page_stride = bb.n_layer * bytes;
     c.scale_stride = bb.n_layer * scales;
     c.n_pages = n_pages_;
@@ -825,10 +826,20 @@ int Engine::depth_trace(double * out, int max_phases) {
 }
 
 void Engine::raise_device_error(int code, const std::string & what) {
-    // the failure is reported once: clear the word so that the next launches start clean
-    CK(cudaMemsetAsync(err_, 0, sizeof(int), stream_));
+    // the failure is reported once: clear the words so that the next launches start clean
+    CK(cudaMemsetAsync(err_, 0, 2 * sizeof(int), stream_));
     CK(cudaStreamSynchronize(stream_));
     throw std::runtime_error(what + " (device error code " + std::to_string(code) + ")");
+}
+
+void Engine::fetch_errors(DeviceErrors & e) {
+    CK(cudaMemcpyAsync(&e, err_, sizeof(e), cudaMemcpyDeviceToHost, stream_));
+}
+
+void Engine::raise_errors(const DeviceErrors & e, const std::string & where) {
+    if (e.wait) raise_device_error(e.wait, "a bounded wait timed out inside " + where);
+    if (e.kv8 & BZB_KV8_TIMED_OUT) raise_device_error(e.kv8, "a bounded wait timed out inside the 8-bit cache's attention of " + where);
+    if (e.kv8) raise_device_error(e.kv8, "8-bit cache: a page, slot or length was out of range inside " + where);
 }
 
 void Engine::enqueue_depth(int R, const int * forced_dev, float * logits_dev, unsigned long long * trace,
@@ -1104,10 +1115,10 @@ StepResult Engine::step(const int * sids, int n, int K, const uint32_t * seeds, 
     CK(cudaMemcpyAsync(fr.data(), frames_all_, fr.size() * sizeof(int), cudaMemcpyDeviceToHost, stream_));
     CK(cudaMemcpyAsync(nx.data(), next_, R * sizeof(int), cudaMemcpyDeviceToHost, stream_));
     CK(cudaMemcpyAsync(aa.data(), any_active_, K * sizeof(int), cudaMemcpyDeviceToHost, stream_));
-    int errv = 0;
-    CK(cudaMemcpyAsync(&errv, err_, sizeof(int), cudaMemcpyDeviceToHost, stream_));
+    DeviceErrors errors;
+    fetch_errors(errors);
     CK(cudaStreamSynchronize(stream_));
-    if (errv) raise_device_error(errv, "a bounded wait timed out inside the frame step");
+    raise_errors(errors, "the frame step");
     for (int k = 0; k < K; k++) res.steps_executed += aa[k] ? 1 : 0;
     const int wcopy = std::min(width, nc);
     for (int k = 0; k < K; k++) {
@@ -1432,8 +1443,11 @@ void Engine::session_create_tokens(int sid, const std::vector<std::vector<int>> 
         sm.seeds = nullptr; sm.step_ctr = nullptr; sm.next_out = next_; sm.update_hist_first = 1;
         launch_sample(sm, stream_);
         int cb0 = -1;
+        DeviceErrors errors;
         CK(cudaMemcpyAsync(&cb0, next_, sizeof(int), cudaMemcpyDeviceToHost, stream_));
+        fetch_errors(errors);
         CK(cudaStreamSynchronize(stream_));
+        raise_errors(errors, "the prompt");
         SlotHost & sh = slots_[slot];
         sh.active = true;
         sh.max_tokens = est;
@@ -1737,8 +1751,11 @@ void Engine::sessions_create_batch(const std::vector<CreateSpec> & specs, int * 
             sm.next_out = pnext_; sm.update_hist_first = 1;
             launch_sample(sm, stream_);
             std::vector<int> nx(nb);
+            DeviceErrors errors;
             CK(cudaMemcpyAsync(nx.data(), pnext_, nb * sizeof(int), cudaMemcpyDeviceToHost, stream_));
+            fetch_errors(errors);
             CK(cudaStreamSynchronize(stream_));
+            raise_errors(errors, "the prompts");
             for (int i = g0; i < g1; i++) {
                 const Prep & p = prep[i];
                 SlotHost & sh = slots_[slot_c[i - g0]];

@@ -237,8 +237,14 @@ private:
     const DpPlan * depth_plan(int R);
     void enqueue_depth(int R, const int * forced_dev, float * logits_dev, unsigned long long * trace = nullptr,
                        const int * row_set = nullptr, long long grid_spin = 0);
-    // clears the device error word, then throws `what` with the code
+    // clears the device error words, then throws `what` with the code
     [[noreturn]] void raise_device_error(int code, const std::string & what);
+    // the device error words after a prompt or a step: copied with its results, looked at when they are there
+    struct DeviceErrors {
+        int wait = 0, kv8 = 0;
+    };
+    void fetch_errors(DeviceErrors & e);
+    void raise_errors(const DeviceErrors & e, const std::string & where);
     long long dbg_grid_spin_ = 0;  // grid-barrier poll limit of debug_depth launches (0: default)
     bool dp_supported(int R) const;
     int acquire_slot(int sid, int n_pages, bool register_sid = true);
@@ -352,7 +358,7 @@ private:
     size_t dp_P_floats_ = 0;
     float * dp_ss_ = nullptr;
     unsigned * dp_bar_ = nullptr;
-    int * err_ = nullptr;
+    int * err_ = nullptr;  // DeviceErrors: the tcgen05 pipelines' and the grid barriers' code, the 8-bit cache's status
     cudaEvent_t dprof_a_ = nullptr, dprof_b_ = nullptr;
 };
 
