@@ -35,6 +35,17 @@ struct Batch : bzb_kv8_batch {
     throw Refused{};
 }
 
+// a new reference, given back at the end of its scope (at::empty may throw)
+struct Ref {
+    PyObject * o;
+    explicit Ref(PyObject * p) : o(p) {
+        if (!o) throw Refused{};
+    }
+    ~Ref() { Py_DECREF(o); }
+    Ref(const Ref &) = delete;
+    Ref & operator=(const Ref &) = delete;
+};
+
 template <typename T>
 T * address(PyObject * o) {
     T * p = static_cast<T *>(PyLong_AsVoidPtr(o));
@@ -164,21 +175,27 @@ PyObject * attention(PyObject *, PyObject * const * a, Py_ssize_t n) {
         if (need < 0) return done(-1);
         void * space = nullptr;
         if (need > 0) {
-            // (one for each stream and size, kept as long as the batch: a captured graph may hold it)
-            PyObject * key = Py_BuildValue("(KL)", (unsigned long long) reinterpret_cast<uintptr_t>(stream), need);
-            if (!key) return nullptr;
-            PyObject * held = PyDict_GetItemWithError(a[2], key);  // (borrowed)
+            // One for each stream and size, kept as long as the batch, and one for each capture: a graph runs on
+            // whatever stream it is launched on, beside other graphs that were captured on the same one.
+            cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+            unsigned long long graph = 0;
+            if (cudaStreamGetCaptureInfo(stream, &capture, &graph) != cudaSuccess) {
+                (void) cudaGetLastError();
+                PyErr_SetString(PyExc_RuntimeError, "kv8_attention: the stream's capture is not valid");
+                throw Refused{};
+            }
+            const Ref key(Py_BuildValue("(KLK)", (unsigned long long) reinterpret_cast<uintptr_t>(stream), need,
+                                        capture == cudaStreamCaptureStatusNone ? 0ull : graph + 1));
+            PyObject * held = PyDict_GetItemWithError(a[2], key.o);  // (borrowed)
+            if (!held && PyErr_Occurred()) throw Refused{};
             if (held) {
                 space = THPVariable_Unpack(held).data_ptr();
-            } else if (!PyErr_Occurred()) {
-                at::Tensor t = at::empty({ (int64_t) need }, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, c.device));
+            } else {
+                const at::Tensor t = at::empty({ (int64_t) need }, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, c.device));
                 space = t.data_ptr();
-                PyObject * py = THPVariable_Wrap(t);
-                if (py) PyDict_SetItem(a[2], key, py);
-                Py_XDECREF(py);
+                const Ref py(THPVariable_Wrap(t));
+                if (PyDict_SetItem(a[2], key.o, py.o) != 0) throw Refused{};
             }
-            Py_DECREF(key);
-            if (PyErr_Occurred()) return nullptr;
         }
         return done(f_attention(&c, &b, &q, &o, lse, (float) number(a[5]), causal, window, space, need, stream));
     });

@@ -3,7 +3,9 @@
 A program keeps one KV8Cache for each layer's pages and one KV8Batch for each shape of step, refills the
 batch's device arrays, and calls append() and attention() in turn. Every call enqueues on the current
 stream of the cache's device and returns; nothing is copied, converted or allocated, but for the attention
-workspace, which a batch allocates at its first use on a stream.
+workspace, which a batch allocates at its first use on a stream, and once in each CUDA graph that captures it. The
+batch holds its workspaces as long as it lives, and has to outlive the graphs that captured it; one graph is not to be
+launched again while it runs.
 """
 from __future__ import annotations
 
@@ -77,7 +79,7 @@ class KV8Batch:
         self._c = _Batch(q_start.data_ptr(), kv_len.data_ptr(), None if slots is None else slots.data_ptr(), n, n_tok,
                          max_new, max_len, dev)
         self._at = ctypes.addressof(self._c)
-        self._workspaces: dict = {}  # attention's, one for each stream and size
+        self._workspaces: dict = {}  # attention's, one for each stream, size and capture
 
 
 class KV8Cache:
