@@ -487,7 +487,8 @@ __device__ __forceinline__ void load_q16(const AttnArgs & a, long long i, float 
 // of 64, 4 rows: 70 MB in 23 us, 3.0 TB/s) are bound by latency: 5 us from the sequence through its page to the data,
 // then the longest contexts; 17 us remain without the arithmetic. One sequence of 218 positions: 4.3 us, a launch.
 constexpr int kSmallWarps = 4, kSmallRows = 8;
-constexpr int kSmallBlocks = 512;  // blocks of a range at most
+constexpr int kTable = 128;  // blocks that a warp looks up at a time
+constexpr int kShortRange = kSmallWarps * kTable;  // blocks of a range that needs one look-up
 
 // CTAs that an SM holds, by their registers (96 and 128 a thread)
 constexpr int small_ctas(int hd) { return (hd == 64 ? 20 : 16) / kSmallWarps; }
@@ -510,14 +511,17 @@ __device__ __forceinline__ uint4 lds16(uint32_t a) {
     return v;
 }
 
-template <int HD>
+// LONG: ranges of more than kShortRange blocks, looked up part by part. (A form of its own, for the registers that the
+// outer loop keeps: with it, 64 sequences of 90 to 2030 positions take 24.9 us instead of 23.2. Ranges of any
+// length keep the workspace small: with short ones only, 512 sequences bounded by 131072 positions needed 277 MB.)
+template <int HD, bool LONG>
 __global__ void __launch_bounds__(32 * kSmallWarps, small_ctas(HD)) kv8_attn_small_kernel(const AttnArgs a) {
     using T = SmallTile<HD>;
     extern __shared__ __align__(16) uint8_t ring[];
     __shared__ float sm_ml[kSmallWarps][kSmallRows][2];
-    // the range's blocks: the head's keys (its values lie one plane on), the scales of both
-    __shared__ const uint8_t * block_at[kSmallBlocks];
-    __shared__ float2 scales[kSmallBlocks];
+    // the warps' next blocks: the head's keys (its values lie one plane on), the scales of both
+    __shared__ const uint8_t * block_at[kSmallWarps * kTable];
+    __shared__ float2 scales[kSmallWarps * kTable];
     const Kv & kv = a.kv;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     // (heads fastest: neighbouring CTAs read neighbouring bytes of the same pages)
@@ -540,16 +544,9 @@ __global__ void __launch_bounds__(32 * kSmallWarps, small_ctas(HD)) kv8_attn_sma
     const int full_lo = a.window > 0 ? max(0, first + last_row / a.group - a.window + 1) : 0;
     const int c_lo = span.blk_lo + chunk * a.chunk_blocks, c_hi = min(span.blk_hi, c_lo + a.chunk_blocks);
 
-    // this warp's blocks: base, base + kSmallWarps, ..., looked up by itself
-    const int base = c_lo + warp, n = max(0, (c_hi - base + kSmallWarps - 1) / kSmallWarps), mine0 = warp * (kSmallBlocks / kSmallWarps);
-    // (the first blocks' copies do not wait for their scales)
-    float2 sc0 = make_float2(0.0f, 0.0f);
-    if (lane < n) {
-        const int blk = base + lane * kSmallWarps, pg = max(page_of(kv, s.slot, blk), 0);
-        block_at[mine0 + lane] = block_ptr(kv, pg, blk, 0, h, HD);
-        sc0 = make_float2(*scale_ptr(kv, pg, blk, 0, h), *scale_ptr(kv, pg, blk, 1, h));
-    }
-    __syncwarp();
+    // this warp's blocks: base, base + kSmallWarps, ..., looked up by itself, n at a time
+    int base = c_lo + warp, n = 0;
+    const int mine0 = warp * kTable;
     const int kpos = (g >> 1) * 4 + (g & 1);  // the lane's key rows: kpos and kpos + 2 (see the patches' position order)
     const long long v_at = (long long) kv.n_kv * kv.page_tokens * HD;
     const uint32_t slots = (uint32_t) __cvta_generic_to_shared(ring) + warp * (T::AHEAD * 2 * T::PIECES * 512);
@@ -572,21 +569,34 @@ __global__ void __launch_bounds__(32 * kSmallWarps, small_ctas(HD)) kv8_attn_sma
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    if (n > 0) {
-#pragma unroll
-        for (int i = 0; i < T::AHEAD; i++) {
-            // (a range's first 32 blocks are in the table by now)
-            fetch(2 * i, false);
-            fetch(2 * i, true);
+    auto look_up = [&] {
+        n = max(0, (c_hi - base + kSmallWarps - 1) / kSmallWarps);
+        if (LONG) n = min(n, kTable);
+        // (the first blocks' copies do not wait for their scales)
+        float2 sc0 = make_float2(0.0f, 0.0f);
+        if (lane < n) {
+            const int blk = base + lane * kSmallWarps, pg = max(page_of(kv, s.slot, blk), 0);
+            block_at[mine0 + lane] = block_ptr(kv, pg, blk, 0, h, HD);
+            sc0 = make_float2(*scale_ptr(kv, pg, blk, 0, h), *scale_ptr(kv, pg, blk, 1, h));
         }
-    }
-    if (lane < n) scales[mine0 + lane] = sc0;
-    for (int i = lane + 32; i < n; i += 32) {
-        const int blk = base + i * kSmallWarps, pg = max(page_of(kv, s.slot, blk), 0);
-        block_at[mine0 + i] = block_ptr(kv, pg, blk, 0, h, HD);
-        scales[mine0 + i] = make_float2(*scale_ptr(kv, pg, blk, 0, h), *scale_ptr(kv, pg, blk, 1, h));
-    }
-    __syncwarp();
+        __syncwarp();
+        if (n > 0) {
+#pragma unroll
+            for (int i = 0; i < T::AHEAD; i++) {
+                // (the first 32 blocks are in the table by now)
+                fetch(2 * i, false);
+                fetch(2 * i, true);
+            }
+        }
+        if (lane < n) scales[mine0 + lane] = sc0;
+        for (int i = lane + 32; i < n; i += 32) {
+            const int blk = base + i * kSmallWarps, pg = max(page_of(kv, s.slot, blk), 0);
+            block_at[mine0 + i] = block_ptr(kv, pg, blk, 0, h, HD);
+            scales[mine0 + i] = make_float2(*scale_ptr(kv, pg, blk, 0, h), *scale_ptr(kv, pg, blk, 1, h));
+        }
+        __syncwarp();
+    };
+    look_up();
 
     // queries as the 8-column operand: lane (g, t) holds the warp's row g, elements 64 k + 16 t ..+15
     uint32_t qf[T::KS][8];
@@ -627,6 +637,7 @@ __global__ void __launch_bounds__(32 * kSmallWarps, small_ctas(HD)) kv8_attn_sma
     float o[T::MT][4] = {}, m[2], l[2] = {};
     m[0] = m[1] = -INFINITY;
 
+  for (;;) {  // once, or for each part of a long range
     for (int i = 0; i < n; i += 2) {
         asm volatile("cp.async.wait_group %0;" ::"n"(2 * T::AHEAD - 1) : "memory");  // the keys
         __syncwarp();
@@ -765,6 +776,13 @@ __global__ void __launch_bounds__(32 * kSmallWarps, small_ctas(HD)) kv8_attn_sma
         fetch(i + 2 * T::AHEAD, true);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (!LONG) break;
+    base += kTable * kSmallWarps;
+    if (base >= c_hi) break;
+    // the next of the range's blocks (the copies of zeros behind the last have landed, and no lane looks back)
+    __syncwarp();
+    look_up();
+  }
     __syncthreads();  // the rings become the warps' outputs
     float (*sm_o)[8][HD + 4] = reinterpret_cast<float (*)[8][HD + 4]>(ring);
 
@@ -1002,7 +1020,7 @@ Plan cut(const bzb_kv8_cache & c, const bzb_kv8_batch & b, int n_head, int causa
     // (the many-row kernel's block: one tile of 128 rows, or two whose waits overlap)
     const double block = !tile ? 1 : rows <= 128 ? 1.7 : 2.1;
     const long long slots = tile ? 148 : 148ll * small_ctas(c.head_dim);
-    for (long long n = tile ? 1 : (blocks + kSmallBlocks - 1) / kSmallBlocks; n <= blocks; n++) {
+    for (long long n = 1; n <= blocks; n++) {
         int size = (int) ((blocks + n - 1) / n);
         if (tile) size = (size + 7) / 8 * 8;  // whole stages
         // whole waves of the CTAs that the SMs hold: the last range to end is what counts
@@ -1036,13 +1054,13 @@ long long workspace_of(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const P
     return (long long) b.n_seq * p.row_tiles * c.n_kv * p.chunks * p.rows * (c.head_dim + 4) * 4;
 }
 
-template <int HD>
+template <int HD, bool LONG>
 void run_small(const AttnArgs & a, cudaStream_t s) {
     const long long grid = (long long) a.kv.n_seq * a.row_tiles * a.chunks * a.kv.n_kv;
     constexpr int bytes = SmallTile<HD>::BYTES;
     static std::atomic<uint64_t> ready{ 0 };
-    allow_shared_memory(kv8_attn_small_kernel<HD>, bytes, ready);
-    launch_chained(kv8_attn_small_kernel<HD>, dim3((unsigned) grid), 32 * kSmallWarps, bytes, s, a);
+    allow_shared_memory(kv8_attn_small_kernel<HD, LONG>, bytes, ready);
+    launch_chained(kv8_attn_small_kernel<HD, LONG>, dim3((unsigned) grid), 32 * kSmallWarps, bytes, s, a);
 }
 
 // Checks them and gives the window that counts: none where no context fills it, so that positions less a window stay
@@ -1175,9 +1193,11 @@ void kv8_attention(const bzb_kv8_cache & c, const bzb_kv8_batch & b, const bzb_k
     if (p.tile) {
         launch_attn_tile(a, c.head_dim, s);
     } else if (c.head_dim == 64) {
-        run_small<64>(a, s);
+        if (p.chunk_blocks > kShortRange) run_small<64, true>(a, s);
+        else run_small<64, false>(a, s);
     } else {
-        run_small<128>(a, s);
+        if (p.chunk_blocks > kShortRange) run_small<128, true>(a, s);
+        else run_small<128, false>(a, s);
     }
     if (p.chunks > 1) {
         const long long warps = (long long) b.n_seq * p.row_tiles * c.n_kv * p.rows;

@@ -36,3 +36,19 @@ def test_the_largest_counts_of_rows_are_planned(lib):  # noqa: F811
     for max_new, n_head in ((1 << 24, 64), (1 << 14, 1 << 16), (1 << 24, 1)):
         b = batch(n_seq=1, n_tok=5, max_new=max_new, max_len=1 << 22)
         assert lib.bzb_kv8_attention_workspace(ref(c), ref(b), n_head, 1, 0) >= 0, lib.breeze_last_error()
+
+
+@pytest.mark.parametrize("hd,most", [(64, 24 << 20), (128, 36 << 20)])
+def test_workspaces_stay_small_whatever_the_bounds(lib, hd, most):  # noqa: F811
+    """Ranges are made to fill the GPU and for no other reason: their results take tens of MB however many
+    sequences and positions a batch may have. (A range held 512 blocks at most, which made 277 MB of 512 sequences
+    bounded by 131072 positions and 11 GB of 5000 by 2^20.)"""
+    c = cache(max_pages=1 << 16, n_kv=8, head_dim=hd, page_stride=2 * 8 * 16 * hd, scale_stride=16, n_slots=1 << 16)
+    for n_seq in (1, 3, 17, 64, 200, 512, 5000, 60000):
+        for max_new in (1, 2, 5, 40, 300):
+            for max_len in (64, 2000, 8192, 8200, 131072, 1 << 20):
+                for n_head in (8, 32, 64):
+                    for window in (0, 500, 30000):
+                        b = batch(n_seq=n_seq, n_tok=n_seq * max_new, max_new=max_new, max_len=max_len)
+                        n = lib.bzb_kv8_attention_workspace(ref(c), ref(b), n_head, 1, window)
+                        assert 0 <= n <= most, (n_seq, max_new, max_len, n_head, window, n)
