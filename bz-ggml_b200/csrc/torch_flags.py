@@ -1,8 +1,18 @@
 """Prints the compiler flags of a PyTorch extension for this interpreter (used by the Makefile); fails, with the
-reason, where there is no PyTorch with CUDA or no Python headers."""
+reason, where there is no PyTorch with CUDA or no Python headers. With --stamp: what they depend on, without importing it."""
 import os
 import sys
 import sysconfig
+
+if sys.argv[1:] == ["--stamp"]:
+    import importlib.metadata
+    import importlib.util
+    try:
+        torch = importlib.metadata.version("torch"), importlib.util.find_spec("torch").origin
+    except (importlib.metadata.PackageNotFoundError, AttributeError):
+        torch = ("none",)
+    print(sys.executable, sys.version.split()[0], "torch", *torch)
+    sys.exit(0)
 
 try:
     import torch

@@ -52,3 +52,23 @@ def test_a_binding_that_does_not_compile_is_an_error(tree):
     script(tmp / "cxx", "exit 1\n")
     r, _ = make(script(tmp / "py", "echo -DFLAGS\n"))
     assert r.returncode != 0
+
+
+def test_another_interpreter_or_pytorch_builds_the_binding_again(tree):
+    tmp, pkg, make = tree
+    version = tmp / "version"
+    version.write_text("torch 1\n")
+    python = script(tmp / "py", f'if [ "$2" = --stamp ]; then cat {version}; else echo -DFLAGS; fi\n')
+    assert len(make(python)[1]) == 1
+    assert len(make(python)[1]) == 1, "nothing changed"
+    version.write_text("torch 2\n")
+    assert len(make(python)[1]) == 2
+    assert len(make(python)[1]) == 2
+
+
+def test_the_stamp_names_interpreter_and_pytorch():
+    import sys
+    import torch
+    out = subprocess.run([sys.executable, os.path.join(ROOT, "bz-ggml_b200", "csrc", "torch_flags.py"), "--stamp"], capture_output=True,
+                         text=True, check=True).stdout
+    assert sys.version.split()[0] in out and torch.__version__ in out
