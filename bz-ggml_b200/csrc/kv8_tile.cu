@@ -638,6 +638,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
     if (mma >= 0 && mt < tiles && n > 0) {
         // (offsets are added to the descriptors' 16-byte address field, which no tile here carries out of)
         const uint32_t sc = tmem + mt * 2 * kStep;
+        // a producer waits for step u's stage to be free. (The last two stages' are not signalled: an arrival that
+        // nothing waits for could come when the CTA has left and its shared memory is another's)
+        const auto freed = [&](int u) { return (u >> 1) + 2 < n; };
         bool ok = true;
         if (mma < 2) {
             constexpr uint32_t idesc = (1u << 4) | ((uint32_t) (kStep >> 3) << 17) | (8u << 24);
@@ -666,7 +669,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
                     // (and this thread's own arrival, which hands on what the wait for the keys made visible: the
                     // stage's scales)
                     mbar_arrive(&sh.s_full[mt][u & 1]);
-                    if (u & 1) umma_commit(&sh.k_empty[st]);
+                    if ((u & 1) && freed(u)) umma_commit(&sh.k_empty[st]);
                 }
                 __syncwarp();
             }
@@ -685,7 +688,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) kv8_attn_tile_kernel(const At
                     for (int kk = 0; kk < kStep / 16; kk++)
                         umma_f16_tmem_a(tmem + M::cO + mt * HD, sc + (u & 1) * kStep + kk * 8, v + (kk * 32 >> 4), idesc, u > 0 || kk > 0);
                     umma_commit(u + 1 == steps ? &sh.o_full[mt] : &sh.pv_done[mt][u & 1]);
-                    if (u & 1) umma_commit(&sh.v_empty[st]);
+                    if ((u & 1) && freed(u)) umma_commit(&sh.v_empty[st]);
                 }
                 __syncwarp();
             }
