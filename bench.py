@@ -910,6 +910,7 @@ def main():
                                    "(prompts U[16,512] tok, voice 0-125 frames, gen U[50,400] frames, page 16, top-k 50 "
                                    "T 0.9, greedy depth per the batched ABI)",
                        "sessions_per_gpu": args.sessions, "nc": nc, "quant": "Q8_0", "parallelism": f"replicas x{world}",
+                       "kv_cache": os.environ.get("BZB_KV_CACHE") or "f16",
                        "l2": "per-step working set > 126 MB L2 (no flush needed)", "ramp_steps": args.ramp,
                        "ramp_s": t_ramp, "admissions_in_timed_steps": admits_timed, "mean_context": mean_ctx,
                        "model_load_s": t_load},
