@@ -31,9 +31,9 @@ using namespace kv8;
 // same bytes whatever the launch's shape.
 //
 // Bound by loads and the arithmetic between them, not by DRAM: 16384 rows of 32 + 2 x 8 heads of 128 in bf16 are
-// appended in 100 us (363 MB, 3.6 TB/s), 14 of them the (cos, sin) loads, which every head repeats (from L1
-// and L2), and 12 the keys' 64-bit arithmetic. Reading 16 x 700 to 4096 positions of 8 heads of 128 takes 48 us (236 MB,
-// 4.9 TB/s). A batch of 64 single rows: 8.8 us. With a lane on one row the first took 246 us; with 8 warps
+// appended in 105 us (363 MB, 3.5 TB/s), 14 of them the (cos, sin) loads, which every head repeats (from L1
+// and L2), and 12 the keys' 64-bit arithmetic; at 80 registers 212 to 466 bytes a thread are spilled. Reading 16 x 700 to
+// 4096 positions of 8 heads of 128 takes 48 us (236 MB, 4.9 TB/s). A batch of 64 single rows: 5.9 us. With a lane on one row the first took 246 us; with 8 warps
 // a CTA it takes 8 us more, with 5 CTAs an SM (fewer spills) 6 more, with one launch for q and one for the cache 10 more.
 constexpr int kRowWarps = 4;
 template <int HD>

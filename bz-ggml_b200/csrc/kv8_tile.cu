@@ -18,14 +18,15 @@
 // weights then stay below 2^8, which f16 holds as precisely), so that the tile of outputs in
 // tensor memory is seldom read back.
 //
-// 8192 rows behind 4100 positions, 32 query and 8 kv heads of 128: 1.19 ms, 920 TFLOP/s, tensor pipes 44 % active.
+// 8192 rows behind 4100 positions, 32 query and 8 kv heads of 128: 1.19 to 1.23 ms, 900 to 920 TFLOP/s, tensor pipes 43 % active;
+// 1.26 ms where every stage has blocks 2^30 apart (see stage_scale).
 // What bounds it is one softmax's chain (scores from tensor memory, maximum, 64 exponentials, weights back): about 2200
 // clocks for a step of 64 keys of both tiles, whose MMAs take 1280 and exponentials 1024. It was 2.36 ms with one
 // warp issuing both tiles' MMAs and 128-key steps, 1.42 with a warp for each chain, 64-key steps and two buffers of
 // scores, 1.25 with the scales of a whole stage put beside it by the producers, 1.20 with the second tile half a
 // step late. Two CTAs an SM with 128 rows each: 2.16 ms (twice the conversions); a quarter to a half of the exponentials as a
 // polynomial on the FMA units: 1.15 to 1.23 against 1.16, prompts slower. 24 packed prompts of 17 to 301 tokens, 8 kv heads
-// of 64: 49 us, about 9 us of set-up, first loads and output in each of four waves of CTAs.
+// of 64: 50 us (49 without the check of the stages' spread), about 9 us of set-up, first loads and output in each of four waves of CTAs.
 #include "kv8_dev.cuh"
 #include "tc_ptx.cuh"
 

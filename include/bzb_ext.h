@@ -186,7 +186,7 @@ typedef struct bzb_kv8_rows {
  *   (16-byte aligned) holds (cos, sin).
  * q_norm / k_norm [head_dim] or NULL (no norm), rope or NULL (no rotation); q and q_out both NULL
  * when only keys and values are wanted. q, k, v of one type (f32, f16 or bf16), q_out f16 or bf16; q_out
- * may not overlap q. A block that already holds earlier positions of its sequence takes the larger of
+ * may not overlap q, k or v. A block that already holds earlier positions of its sequence takes the larger of
  * its scale and the new values' one; the earlier values are then rescaled (exactly, except where they
  * fall below the smallest e4m3). Infinities and NaN are stored as NaN and do not count for the scale.
  * Positions of a written block past kv_len become zero. Two sequences of one call may not share a
